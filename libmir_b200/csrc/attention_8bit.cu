@@ -1,0 +1,411 @@
+// Attention over the 8-bit cache on mma.sync, for every size the operators take (head_dim 64 and 128, any page size):
+//
+//   out = sum_j p_j S_v[page of j] V_j / sum_j p_j,   p_j = exp(scale q . (S_k[page of j] K_j) - max)
+//
+// over the keys j <= position (inside the window, if any) whose page the block table has.  K and V are e4m3, S_k and S_v
+// one power of two per page and kv head: a number times its scale is exact in bf16, so a tile of keys and values is
+// scaled on its way into shared memory and everything behind that is bf16 attention with 32-bit scores, maxima,
+// exponentials and sums (the weights p are rounded to bf16 for the product with V, as in the kernels over bf16 pages).
+//
+// A CTA takes 64 rows of one request and one kv head, and one partition of the keys.  A row is a (token, query head of the
+// group) pair: all heads of the group share the tile's keys, so that the cache is read once per group.  Four warps of 16
+// rows; the next tile's bytes are on their way in registers while this one is worked on.  Partitions' results are joined by
+// a second kernel (merge_8bit_kernel), a warp for each token and head.
+#include <algorithm>
+#include "eight_bit.cuh"
+#include "eight_bit.h"
+
+using namespace mir;
+typedef __nv_bfloat16 bf16;
+
+namespace {
+
+constexpr int kRows = 64, kKeys = 64, kThreads = 128;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack(float low, float high) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+template <int DIM>
+__global__ void __launch_bounds__(kThreads)
+attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __restrict__ out, Cache8 cache,
+                      const int* __restrict__ block_table, int table_width, const int* __restrict__ positions,
+                      const int* __restrict__ query_starts, const int* __restrict__ context_lens, int num_rows, int group,
+                      float scale_log2, int window, int partition, int num_partitions, float* __restrict__ partial_o,
+                      float* __restrict__ partial_ml, const float* __restrict__ sinks) {
+  constexpr int kStride = DIM + 8;              // bf16 elements of a shared row: an odd number of 16-byte pieces
+  constexpr int kPieces = DIM / 16;             // 16-byte pieces of a cached row
+  constexpr int kRounds = kKeys * kPieces / kThreads;
+  __shared__ __align__(16) bf16 k_tile[kKeys * kStride];
+  __shared__ __align__(16) bf16 v_tile[kKeys * kStride];
+  __shared__ unsigned long long there_bits[2];  // [tile parity]: keys of the tile whose page the table has
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int part = blockIdx.x % num_partitions, tile = blockIdx.x / num_partitions, kv_head = blockIdx.y;
+  // the request and its rows: one token for each request, or portions
+  int request = -1, first_row = 0, first_token = 0, count = 1, first_position = 0;
+  if (query_starts == nullptr) {
+    const int per_request = (group + kRows - 1) / kRows;
+    request = tile / per_request;
+    first_row = tile % per_request * kRows;
+    first_token = request;
+    first_position = positions[request];
+    if (first_position < 0) return;                               // a padding row: left as it is
+  } else {
+    int remaining = tile;
+    for (int r = 0; r < num_rows; ++r) {
+      const int tokens = query_starts[r + 1] - query_starts[r];
+      const int tiles = (tokens * group + kRows - 1) / kRows;
+      if (remaining < tiles) { request = r; break; }
+      remaining -= tiles;
+    }
+    if (request < 0) return;
+    first_row = remaining * kRows;
+    first_token = query_starts[request];
+    count = query_starts[request + 1] - first_token;
+    first_position = context_lens[request] - count;
+  }
+  const int rows = min(kRows, count * group - first_row);
+  const int lowest = first_position + first_row / group, highest = first_position + (first_row + rows - 1) / group;
+  const int* table = block_table + (size_t)request * table_width;
+  const int heads = group * cache.kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // this thread's two rows of the accumulators: their tokens and heads
+  int token[2], head[2], position[2];
+  bool valid[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int local = warp * 16 + lane / 4 + 8 * i;
+    valid[i] = local < rows;
+    const int row = first_row + min(local, rows - 1);
+    token[i] = first_token + row / group;
+    head[i] = kv_head * group + row % group;
+    position[i] = first_position + row / group;
+  }
+  uint32_t query[DIM / 16][4];
+#pragma unroll
+  for (int kk = 0; kk < DIM / 16; ++kk)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      query[kk][i] = *reinterpret_cast<const uint32_t*>(q + (size_t)token[i & 1] * q_stride + (size_t)head[i & 1] * DIM +
+                                                        kk * 16 + (i >> 1) * 8 + (lane & 3) * 2);
+
+  const int from = max(part * partition, (window > 0 ? max(0, lowest - window + 1) : 0) / kKeys * kKeys);
+  const int end = (int)min((long long)highest + 1, (long long)(part + 1) * partition);
+  float o[DIM / 8][4];
+#pragma unroll
+  for (int n = 0; n < DIM / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+
+  uint4 k_raw[kRounds], v_raw[kRounds];
+  float k_scale[kRounds], v_scale[kRounds];
+  unsigned there = 0;                                              // which of this thread's pieces are of keys that are there
+  auto fetch = [&](int key0) {
+    there = 0;
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int piece = threadIdx.x + i * kThreads;
+      const int key = key0 + piece / kPieces;
+      k_raw[i] = v_raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      k_scale[i] = v_scale[i] = 0.0f;
+      if (key < end) {
+        const int block = key / cache.page_size;
+        const int page = page_of_block(table, table_width, block, cache.pages);
+        if (page >= 0) {
+          const size_t row = (size_t)page * cache.page_size + (key - block * cache.page_size);
+          const size_t at = (row * cache.kv_heads + kv_head) * DIM + piece % kPieces * 16;
+          k_raw[i] = *reinterpret_cast<const uint4*>(cache.k + at);
+          v_raw[i] = *reinterpret_cast<const uint4*>(cache.v + at);
+          k_scale[i] = cache.k_scales[(size_t)page * cache.kv_heads + kv_head];
+          v_scale[i] = cache.v_scales[(size_t)page * cache.kv_heads + kv_head];
+          there |= 1u << i;
+        }
+      }
+    }
+  };
+  auto put = [&](bf16* tile_rows, const uint4& raw, float scale, int piece) {
+    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t packed[8];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      packed[2 * w] = scaled_bf16(e4m3_low(words[w]), scale);
+      packed[2 * w + 1] = scaled_bf16(e4m3_high(words[w]), scale);
+    }
+    uint4* to = reinterpret_cast<uint4*>(tile_rows + piece / kPieces * kStride + piece % kPieces * 16);
+    to[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    to[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
+  };
+
+  if (threadIdx.x == 0) there_bits[0] = 0ull;
+  if (from < end) fetch(from);
+  int parity = 0;
+  for (int key0 = from; key0 < end; key0 += kKeys, parity ^= 1) {
+    __syncthreads();                                               // (the last tile has been read)
+    unsigned long long mine = 0ull;
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int piece = threadIdx.x + i * kThreads;
+      put(k_tile, k_raw[i], k_scale[i], piece);
+      put(v_tile, v_raw[i], v_scale[i], piece);
+      if ((there >> i & 1u) && piece % kPieces == 0) mine |= 1ull << (piece / kPieces);
+    }
+    if (mine) atomicOr(&there_bits[parity], mine);
+    __syncthreads();
+    const unsigned long long seen = there_bits[parity];
+    if (threadIdx.x == 0) there_bits[parity ^ 1] = 0ull;           // (the tile before's: every thread has read it)
+    if (key0 + kKeys < end) fetch(key0 + kKeys);
+
+    float s[kKeys / 8][4];
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < DIM / 16; kk += 2) {
+        uint32_t b[4];
+        ldmatrix_x4(b, smem_u32(k_tile + (n * 8 + (lane & 7)) * kStride + kk * 16 + (lane >> 3) * 8));
+        mma_bf16(s[n], query[kk], b[0], b[1]);
+        mma_bf16(s[n], query[kk + 1], b[2], b[3]);
+      }
+    }
+    float best[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int column = n * 8 + (lane & 3) * 2 + (i & 1), key = key0 + column, at = position[i >> 1];
+        const bool visible = key <= at && (window == 0 || key > at - window) && (seen >> column & 1ull) && key < end;
+        s[n][i] = visible ? s[n][i] * scale_log2 : -INFINITY;
+        best[i >> 1] = fmaxf(best[i >> 1], s[n][i]);
+      }
+    float shift[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float now = fmaxf(top[i], quad_max(best[i]));
+      const float factor = now == top[i] ? 1.0f : approximate_exp2(top[i] - now);    // 0 where nothing was seen before
+      top[i] = now;
+      sum[i] *= factor;
+#pragma unroll
+      for (int n = 0; n < DIM / 8; ++n) {
+        o[n][2 * i] *= factor;
+        o[n][2 * i + 1] *= factor;
+      }
+      shift[i] = now == -INFINITY ? 0.0f : now;
+    }
+    uint32_t weights[kKeys / 16][4];
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[n][i] = approximate_exp2(s[n][i] - shift[i >> 1]);
+        sum[i >> 1] += s[n][i];
+      }
+      weights[n / 2][(n & 1) * 2] = pack(s[n][0], s[n][1]);
+      weights[n / 2][(n & 1) * 2 + 1] = pack(s[n][2], s[n][3]);
+    }
+#pragma unroll
+    for (int kk = 0; kk < kKeys / 16; ++kk)
+#pragma unroll
+      for (int n = 0; n < DIM / 8; n += 2) {
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, smem_u32(v_tile + (kk * 16 + (lane & 15)) * kStride + n * 8 + (lane >> 4) * 8));
+        mma_bf16(o[n], weights[kk], b[0], b[1]);
+        mma_bf16(o[n + 1], weights[kk], b[2], b[3]);
+      }
+  }
+
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float total = quad_sum(sum[i]);
+    if (!valid[i]) continue;
+    const size_t row = (size_t)token[i] * heads + head[i];
+    if (num_partitions == 1) {
+      if (total > 0.0f && sinks != nullptr) total += exp2f(sinks[head[i]] * kLog2e - top[i]);
+      const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+      for (int n = 0; n < DIM / 8; ++n)
+        *reinterpret_cast<uint32_t*>(out + row * DIM + n * 8 + (lane & 3) * 2) = pack(o[n][2 * i] * inverse, o[n][2 * i + 1] * inverse);
+    } else {
+      const size_t at = row * num_partitions + part;
+      if ((lane & 3) == 0) *reinterpret_cast<float2*>(partial_ml + at * 2) = make_float2(top[i], total);
+      if (total > 0.0f) {
+#pragma unroll
+        for (int n = 0; n < DIM / 8; ++n)
+          *reinterpret_cast<float2*>(partial_o + at * DIM + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+      }
+    }
+  }
+}
+
+// A warp for each token and head: the partitions' parts, each relative to a maximum of its own, to one result.  A part
+// whose denominator is 0 holds nothing (no key of it was visible) and is not read.
+template <int DIM>
+__global__ void __launch_bounds__(256)
+merge_8bit_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, bf16* __restrict__ out,
+                  const int* __restrict__ positions, const int* __restrict__ query_starts, int num_rows, int tokens, int heads,
+                  int num_partitions, const float* __restrict__ sinks) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= (long long)tokens * heads) return;
+  const int token = (int)(row / heads), head = (int)(row % heads);
+  if (query_starts == nullptr ? positions[token] < 0 : (token < query_starts[0] || token >= query_starts[num_rows])) return;
+  const float2* ml = reinterpret_cast<const float2*>(partial_ml) + row * num_partitions;
+  float top = -INFINITY;
+  for (int p = lane; p < num_partitions; p += 32)
+    if (ml[p].y > 0.0f) top = fmaxf(top, ml[p].x);
+  top = warp_max(top);
+  constexpr int kColumns = DIM / 32;
+  float o[kColumns], total = 0.0f;
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c) o[c] = 0.0f;
+  const float* part = partial_o + (size_t)row * num_partitions * DIM + lane * kColumns;
+  for (int p = 0; p < num_partitions; ++p, part += DIM) {
+    const float2 mine = ml[p];
+    if (!(mine.y > 0.0f)) continue;
+    const float factor = exp2f(mine.x - top);
+    total += mine.y * factor;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) o[c] += part[c] * factor;
+  }
+  if (total > 0.0f && sinks != nullptr) total += exp2f(sinks[head] * kLog2e - top);
+  const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+  uint32_t* to = reinterpret_cast<uint32_t*>(out + (size_t)row * DIM + lane * kColumns);
+#pragma unroll
+  for (int c = 0; c < kColumns; c += 2) to[c / 2] = pack(o[c] * inverse, o[c + 1] * inverse);
+}
+
+}  // namespace
+
+int mir_merge_8bit(const Attention8& a, int tokens) {
+  const long long blocks = ((long long)tokens * a.heads + 7) / 8;
+  return mir_launch("merge_8bit", a.head_dim == 128 ? merge_8bit_kernel<128> : merge_8bit_kernel<64>, dim3((unsigned)blocks),
+                    dim3(256), 0, a.stream, 0, a.partial_o(tokens), a.partial_ml(tokens), (bf16*)a.out, a.positions, a.query_starts,
+                    a.num_rows, tokens, a.heads, a.num_partitions, a.sinks);
+}
+
+int mir_attention_8bit_general(const Attention8& a, int tokens) {
+  const int group = a.heads / a.cache.kv_heads;
+  // tiles of 64 rows; of portions an upper bound (spare ones find no request and end)
+  const long long tiles = a.query_starts == nullptr ? (long long)a.num_rows * ((group + kRows - 1) / kRows)
+                                                    : ((long long)tokens * group + kRows - 1) / kRows + a.num_rows;
+  if (tiles * a.num_partitions > 0x7fffffffll || a.cache.kv_heads > 65535) {
+    mir_set_error("%s: %d tokens are more than one launch takes", a.what, tokens);
+    return MIR_BAD_ARGUMENT;
+  }
+  const dim3 grid((unsigned)(tiles * a.num_partitions), a.cache.kv_heads);
+  const int status = mir_launch("attention_8bit", a.head_dim == 128 ? attention_8bit_kernel<128> : attention_8bit_kernel<64>, grid,
+                                dim3(kThreads), 0, a.stream, 0, (const bf16*)a.q, a.q_stride, (bf16*)a.out, a.cache, a.block_table,
+                                a.table_width, a.positions, a.query_starts, a.context_lens, a.num_rows, group,
+                                a.scale * kLog2e, a.window, a.partition, a.num_partitions, a.partial_o(tokens), a.partial_ml(tokens),
+                                a.sinks);
+  if (status != MIR_OK || a.num_partitions == 1) return status;
+  return mir_merge_8bit(a, tokens);
+}
+
+static bool attention_8bit_refused(const Attention8& a, int tokens) {
+  const bool bad =
+      (a.head_dim != 64 && a.head_dim != 128) || a.heads <= 0 || a.cache.kv_heads <= 0 || a.heads % a.cache.kv_heads ||
+      a.cache.page_size <= 0 || a.cache.pages <= 0 || (long long)a.cache.pages * a.cache.page_size > 0x7fffffffll || a.table_width <= 0 ||
+      !(a.scale > 0.0f) || a.window < 0 || (a.q_stride % 8) || a.q_stride < (long long)a.heads * a.head_dim || ((uintptr_t)a.q & 15) ||
+      ((uintptr_t)a.out & 15) || ((uintptr_t)a.cache.k & 15) || ((uintptr_t)a.cache.v & 15) || a.partition <= 0 || a.partition % 128 ||
+      a.num_partitions <= 0 || a.num_partitions > 65535 || a.num_rows < 0 || tokens < 0;
+  if (bad) {
+    mir_set_error("%s: takes head_dim 64 or 128, a positive scale, partitions of whole 128 keys and 16-byte aligned tensors (head_dim "
+                  "%d, heads %d, kv heads %d, page %d, pages %d, partition %d x %d, row stride %lld)", a.what, a.head_dim, a.heads,
+                  a.cache.kv_heads, a.cache.page_size, a.cache.pages, a.partition, a.num_partitions, a.q_stride);
+    return true;
+  }
+  const long long need = a.num_partitions == 1 ? 0 : (long long)tokens * a.heads * a.num_partitions * (a.head_dim + 2);
+  if (need > 0 && (a.scratch == nullptr || a.scratch_floats < need)) {
+    mir_set_error("%s: scratch of %lld floats is needed, got %lld", a.what, need, a.scratch_floats);
+    return true;
+  }
+  return false;
+}
+
+// How single tokens are split over the keys: partitions of `keys`, `count` of them, and the floats of scratch.
+MIR_EXPORT int mir_decode_attention_8bit_plan(int rows, int heads, int kv_heads, int head_dim, int page_size, int max_context,
+                                              int* keys, int* count, long long* floats) {
+  if (rows < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context < 0 || page_size <= 0) {
+    mir_set_error("decode_attention_8bit_plan: bad sizes (rows %d, heads %d, kv heads %d, context %d)", rows, heads, kv_heads, max_context);
+    return MIR_BAD_ARGUMENT;
+  }
+  const int group = heads / kv_heads;
+  const long long ctas = std::max(1ll, (long long)rows * kv_heads * ((group + kRows - 1) / kRows));
+  const long long wanted = std::max(1ll, (long long)mir_sm_count() * 4 / ctas);
+  const long long tiles = std::max(1ll, (max_context + 127ll) / 128);
+  const long long each = std::max(1ll, (tiles + wanted - 1) / wanted);
+  *keys = (int)(each * 128);
+  *count = (int)((tiles + each - 1) / each);
+  *floats = *count == 1 ? 0 : (long long)rows * heads * *count * (head_dim + 2);
+  return MIR_OK;
+}
+
+// One token per request: row r of q at positions[r] (below 0: a padding row, whose result is left as it is).
+MIR_EXPORT int mir_decode_attention_8bit(const void* q, long long q_stride, void* out, const void* k_pages, const void* v_pages,
+                                         const float* k_scales, const float* v_scales, int pages, const int* block_table,
+                                         int table_width, const int* positions, int rows, int page_size, int heads, int kv_heads,
+                                         int head_dim, float scale, int window, int partition, int num_partitions, float* scratch,
+                                         long long scratch_floats, const float* sinks, cudaStream_t stream) {
+  Attention8 a;
+  a.what = "decode_attention_8bit";
+  a.q = q; a.q_stride = q_stride; a.out = out;
+  a.cache = Cache8{(const uint8_t*)k_pages, (const uint8_t*)v_pages, k_scales, v_scales, pages, page_size, kv_heads};
+  a.block_table = block_table; a.table_width = table_width; a.positions = positions;
+  a.num_rows = rows; a.heads = heads; a.head_dim = head_dim; a.scale = scale; a.window = window;
+  a.partition = partition; a.num_partitions = num_partitions; a.scratch = scratch; a.scratch_floats = scratch_floats;
+  a.sinks = sinks; a.stream = stream;
+  if (attention_8bit_refused(a, rows)) return MIR_BAD_ARGUMENT;
+  if (rows == 0) return MIR_OK;
+  return mir_attention_8bit_general(a, rows);
+}
+
+// Portions: request r has tokens query_starts[r] .. query_starts[r + 1] - 1 of the packed rows, and its context_lens[r]
+// cached tokens include them.  Rows that no request has are left as they are.
+MIR_EXPORT int mir_prefill_attention_8bit(const void* q, long long q_stride, void* out, const void* k_pages, const void* v_pages,
+                                          const float* k_scales, const float* v_scales, int pages, const int* block_table,
+                                          int table_width, const int* query_starts, const int* context_lens, int num_rows, int tokens,
+                                          int page_size, int heads, int kv_heads, int head_dim, float scale, int window, int partition,
+                                          int num_partitions, float* scratch, long long scratch_floats, const float* sinks,
+                                          cudaStream_t stream) {
+  Attention8 a;
+  a.what = "prefill_attention_8bit";
+  a.q = q; a.q_stride = q_stride; a.out = out;
+  a.cache = Cache8{(const uint8_t*)k_pages, (const uint8_t*)v_pages, k_scales, v_scales, pages, page_size, kv_heads};
+  a.block_table = block_table; a.table_width = table_width; a.query_starts = query_starts; a.context_lens = context_lens;
+  a.num_rows = num_rows; a.heads = heads; a.head_dim = head_dim; a.scale = scale; a.window = window;
+  a.partition = partition; a.num_partitions = num_partitions; a.scratch = scratch; a.scratch_floats = scratch_floats;
+  a.sinks = sinks; a.stream = stream;
+  if (attention_8bit_refused(a, tokens)) return MIR_BAD_ARGUMENT;
+  if (num_rows == 0 || tokens == 0) return MIR_OK;
+  return mir_attention_8bit_general(a, tokens);
+}

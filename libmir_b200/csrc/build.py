@@ -1,10 +1,11 @@
 """Compiling the CUDA sources for sm_100a with nvcc into shared libraries, and finding them again.
 
-There are two libraries so that a run compiles only what its model needs:
+There are three libraries so that a run compiles only what its model needs:
   core   kernels of both engine dtypes (norms, rotary + cache write, reference attention, 32-bit
          matrix product, sampling) and the layer executor for the float32 engine
   bf16   the same, and what only the bfloat16 engine uses (tensor-core attention, cuBLASLt and tcgen05
          products, the choice between them), with the layer executor for both engine dtypes
+  eight_bit  the operators over 8-bit caches and weights
 A library is rebuilt when the hash of its sources and flags changes.  Objects are compiled in
 parallel, and a line is printed for each so that a first call shows progress.  The libraries are
 written beside the package (libmir_b200/_lib) when that folder can be written, else under the
@@ -47,6 +48,13 @@ LIBRARIES = {
         "headers": ["no_alloc.h", "tcgen05.cuh"],
         "link": ["-lcublasLt"],
         "defines": ["-DMIR_WITH_BF16"],
+    },
+    # the operators for serving in 8 bits
+    "eight_bit": {
+        "sources": ["runtime.cu", "store_8bit.cu", "attention_8bit.cu", "linear_8bit.cu"],
+        "headers": ["eight_bit.h", "eight_bit.cuh", "tcgen05.cuh"],
+        "link": [],
+        "defines": [],
     },
 }
 # the bfloat16 library with time stamps inside its kernels (trace.cuh), for bench.py --phase trace

@@ -1,0 +1,69 @@
+// What the kernels of the 8-bit operators share: e4m3 numbers, scales that are powers of two, and the page of a key.
+//
+// An e4m3 number has four significant bits (the leading one included), 448 is the largest and 2^-9 the smallest.  It and
+// its product with a power of two are exact in float16 or bfloat16 wherever that format's range reaches.
+#pragma once
+#include <cuda_fp8.h>
+#include "common.cuh"
+
+namespace mir {
+
+constexpr int kLeastScaleExponent = -118;    // of a scale that is a power of two: its inverse is a number too
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^e for a whole e; 0 below the normal numbers.
+__device__ __forceinline__ float power_of_two(int e) { return e < -126 ? 0.0f : __int_as_float((e + 127) << 23); }
+
+// The exponent of a scale; kLeastScaleExponent for 0 (a page that was never written).
+__device__ __forceinline__ int scale_exponent_of(float scale) {
+  return max(((__float_as_int(scale) >> 23) & 0xff) - 127, kLeastScaleExponent);
+}
+
+// The least e >= kLeastScaleExponent with largest <= 448 * 2^e; `largest` is finite and not negative.  448 is
+// 1.75 * 2^8, so the mantissa decides whether the exponent less 8 is enough.
+__device__ __forceinline__ int least_scale_exponent(float largest) {
+  const int bits = __float_as_int(largest);
+  return max((bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0), kLeastScaleExponent);
+}
+
+// Two numbers rounded to nearest even to e4m3, beyond 448 (infinities too) to 448; the first in the low byte.
+__device__ __forceinline__ uint32_t to_e4m3x2(float first, float second) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(first, second), __NV_SATFINITE, __NV_E4M3);
+}
+// The two e4m3 numbers of the low (high) half of a word as float16, exact.
+__device__ __forceinline__ __half2 e4m3_low(uint32_t word) {
+  return __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word & 0xffffu), __NV_E4M3));
+}
+__device__ __forceinline__ __half2 e4m3_high(uint32_t word) {
+  return __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word >> 16), __NV_E4M3));
+}
+// Two of them times a power of two, as packed bfloat16 (exact).
+__device__ __forceinline__ uint32_t scaled_bf16(__half2 pair, float scale) {
+  const float2 f = __half22float2(pair);
+  const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * scale, f.y * scale);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+__device__ __forceinline__ float approximate_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The paged 8-bit cache of one layer.
+struct Cache8 {
+  const uint8_t* k;              // [pages * page_size, kv_heads, head_dim]
+  const uint8_t* v;
+  const float* k_scales;         // [pages, kv_heads], powers of two
+  const float* v_scales;
+  int pages, page_size, kv_heads;
+};
+
+// The page of block `block` of a request: -1 where its table ends, has no page, or names one that the pool does not have.
+__device__ __forceinline__ int page_of_block(const int* table, int table_width, int block, int pages) {
+  if (block >= table_width) return -1;
+  const int page = table[block];
+  return page >= 0 && page < pages ? page : -1;
+}
+
+}  // namespace mir

@@ -1,0 +1,32 @@
+// One call of attention over the 8-bit cache, as the entry points hand it to the kernels' launchers.
+#pragma once
+#include "eight_bit.cuh"
+
+struct Attention8 {
+  const char* what = "";
+  const void* q = nullptr;             // packed bf16 rows whose first heads * head_dim columns are the rotated queries
+  long long q_stride = 0;
+  void* out = nullptr;                 // [tokens, heads * head_dim] bf16
+  mir::Cache8 cache{};
+  const int* block_table = nullptr;    // [num_rows, table_width]
+  int table_width = 0;
+  const int* positions = nullptr;      // one token per request: its position; else
+  const int* query_starts = nullptr;   // portions
+  const int* context_lens = nullptr;
+  int num_rows = 0, heads = 0, head_dim = 0;
+  float scale = 0.0f;
+  int window = 0;
+  int partition = 0, num_partitions = 1;   // keys split over this many partitions, joined by mir_merge_8bit
+  float* scratch = nullptr;
+  long long scratch_floats = 0;
+  const float* sinks = nullptr;        // [heads] or null
+  cudaStream_t stream = nullptr;
+
+  float* partial_o(long long) const { return scratch; }
+  float* partial_ml(long long tokens) const {
+    return scratch == nullptr ? nullptr : scratch + tokens * heads * num_partitions * head_dim;
+  }
+};
+
+int mir_attention_8bit_general(const Attention8& a, int tokens);
+int mir_merge_8bit(const Attention8& a, int tokens);

@@ -1,0 +1,215 @@
+// Products with 8-bit weights:  out = x . w^T (+ bias) (+ out)  where
+//
+//   w[n, k] = wq[n, k] * sw[n / 128, k / 128]      wq e4m3, sw any 32-bit number (as checkpoints bring them),
+//   x[m, k] is rounded to xq[m, k] * sx[m, k / 128]  on its way in: sx the least power of two with |x| <= 448 sx over the 128
+//   columns, xq = x / sx rounded to nearest even to e4m3,
+//
+// so out[m, n] = sum over blocks b of 128 columns of  sx[m, b] sw[n / 128, b] (sum over k in b of xq[m, k] wq[n, k]), the inner
+// sums and the outer one in 32 bits.
+#include <algorithm>
+#include "eight_bit.cuh"
+
+using namespace mir;
+typedef __nv_bfloat16 bf16;
+
+namespace {
+
+constexpr int kBlock = 128;             // columns (and rows of a weight) that share a scale
+
+// A warp rounds 128 columns of one row: a lane four of them.
+__global__ void __launch_bounds__(256)
+quantize_rows_kernel(const bf16* __restrict__ x, long long stride, uint8_t* __restrict__ codes, float* __restrict__ scales, int rows,
+                     int columns, int blocks) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= (long long)rows * blocks) return;
+  const int row = (int)(unit / blocks), block = (int)(unit % blocks);
+  const int column = block * kBlock + lane * 4;
+  const bool there = column < columns;                        // columns is a multiple of 16
+  uint2 raw = make_uint2(0u, 0u);
+  if (there) raw = *reinterpret_cast<const uint2*>(x + (size_t)row * stride + column);
+  const float v[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
+                      __uint_as_float(raw.y & 0xffff0000u)};
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+    if (b < 0x7f800000u) bits = max(bits, b);
+  }
+  bits = __reduce_max_sync(0xffffffffu, bits);
+  const int exponent = least_scale_exponent(__uint_as_float(bits));
+  const float inverse = power_of_two(-exponent);
+  if (there)
+    *reinterpret_cast<uint32_t*>(codes + (size_t)row * columns + column) =
+        to_e4m3x2(v[0] * inverse, v[1] * inverse) | (to_e4m3x2(v[2] * inverse, v[3] * inverse) << 16);
+  if (lane == 0) scales[unit] = power_of_two(exponent);
+}
+
+// A weight's blocks of 128 x 128 to e4m3 with scale largest / 448: what a checkpoint would hold.
+template <typename T>
+__global__ void __launch_bounds__(256)
+quantize_weight_kernel(const T* __restrict__ weight, uint8_t* __restrict__ codes, float* __restrict__ scales, int rows, int columns) {
+  __shared__ float largest[8];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int row0 = blockIdx.y * kBlock, column0 = blockIdx.x * kBlock;
+  const int row_end = min(rows, row0 + kBlock), columns_here = min(kBlock, columns - column0);
+  float top = 0.0f;
+  for (int i = threadIdx.x; i < kBlock * kBlock; i += blockDim.x) {
+    const int row = row0 + i / kBlock, column = i % kBlock;
+    if (row < row_end && column < columns_here) {
+      const float v = fabsf(to_float<T>(weight[(size_t)row * columns + column0 + column]));
+      if (v < INFINITY) top = fmaxf(top, v);
+    }
+  }
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, largest[i]);
+  const float scale = top > 0.0f ? fmaxf(top / 448.0f, 1.17549435e-38f) : 1.0f;
+  for (int i = threadIdx.x; i < kBlock * kBlock; i += blockDim.x) {
+    const int row = row0 + i / kBlock, column = i % kBlock;
+    if (row < row_end && column < columns_here) {
+      const size_t at = (size_t)row * columns + column0 + column;
+      codes[at] = (uint8_t)to_e4m3x2(to_float<T>(weight[at]) / scale, 0.0f);
+    }
+  }
+  if (threadIdx.x == 0) scales[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = scale;
+}
+
+constexpr int kTile = 64, kStride = kBlock + 8;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// A tile of 64 rows and 64 columns of the result; codes are taken to float16 (exact) on their way into shared memory.
+__global__ void __launch_bounds__(128)
+linear_8bit_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_scales, const uint8_t* __restrict__ weight,
+                   const float* __restrict__ w_scales, const void* __restrict__ bias, void* __restrict__ out, long long out_stride,
+                   int m, int n, int k, bool out_float, bool accumulate) {
+  __shared__ __align__(16) __half a_tile[kTile * kStride];
+  __shared__ __align__(16) __half b_tile[kTile * kStride];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int row0 = blockIdx.y * kTile, column0 = blockIdx.x * kTile;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int blocks = (k + kBlock - 1) / kBlock;
+  float total[kTile / 8][4] = {};
+  auto put = [&](__half* tile, const uint8_t* codes, int first, int limit, int block) {
+    for (int i = threadIdx.x; i < kTile * 8; i += 128) {
+      const int row = first + i / 8, column = block * kBlock + i % 8 * 16;
+      uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+      if (row < limit && column < k) raw = *reinterpret_cast<const uint4*>(codes + (size_t)row * k + column);
+      __half2* to = reinterpret_cast<__half2*>(tile + i / 8 * kStride + i % 8 * 16);
+      const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        to[2 * w] = e4m3_low(words[w]);
+        to[2 * w + 1] = e4m3_high(words[w]);
+      }
+    }
+  };
+  const int rows[2] = {row0 + warp * 16 + lane / 4, row0 + warp * 16 + lane / 4 + 8};
+  for (int block = 0; block < blocks; ++block) {
+    __syncthreads();
+    put(a_tile, x, row0, m, block);
+    put(b_tile, weight, column0, n, block);
+    __syncthreads();
+    float part[kTile / 8][4] = {};
+#pragma unroll
+    for (int kk = 0; kk < kBlock / 16; ++kk) {
+      uint32_t a[4];
+      const uint32_t at = smem_u32(a_tile + (warp * 16 + (lane & 15)) * kStride + kk * 16 + (lane >> 4) * 8);
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(at));
+#pragma unroll
+      for (int c = 0; c < kTile / 8; ++c) {
+        const uint32_t* b = reinterpret_cast<const uint32_t*>(b_tile + (c * 8 + lane / 4) * kStride + kk * 16 + (lane & 3) * 2);
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(part[c][0]), "+f"(part[c][1]), "+f"(part[c][2]), "+f"(part[c][3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[4]));
+      }
+    }
+    const float w_scale = w_scales[(size_t)(column0 / kBlock) * blocks + block];
+    float scale[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) scale[i] = rows[i] < m ? x_scales[(size_t)rows[i] * blocks + block] * w_scale : 0.0f;
+#pragma unroll
+    for (int c = 0; c < kTile / 8; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total[c][i] = fmaf(part[c][i], scale[i >> 1], total[c][i]);
+  }
+#pragma unroll
+  for (int c = 0; c < kTile / 8; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = rows[i >> 1], column = column0 + c * 8 + (lane & 3) * 2 + (i & 1);
+      if (row >= m || column >= n) continue;
+      float value = total[c][i];
+      const size_t at = (size_t)row * out_stride + column;
+      if (out_float) {
+        if (bias != nullptr) value += static_cast<const float*>(bias)[column];
+        float* to = static_cast<float*>(out) + at;
+        *to = accumulate ? *to + value : value;
+      } else {
+        if (bias != nullptr) value += __bfloat162float(static_cast<const bf16*>(bias)[column]);
+        static_cast<bf16*>(out)[at] = __float2bfloat16_rn(value);
+      }
+    }
+}
+
+}  // namespace
+
+// Bytes of workspace for m rows of k columns: the rounded rows, then their scales.
+MIR_EXPORT long long mir_linear_8bit_workspace(int m, int k) {
+  if (m <= 0 || k <= 0) return 0;
+  const long long codes = ((long long)m * k + 255) / 256 * 256;
+  return codes + (long long)m * ((k + kBlock - 1) / kBlock) * (long long)sizeof(float);
+}
+
+MIR_EXPORT int mir_quantize_weight_8bit(int is_bf16, const void* weight, void* codes, float* scales, int rows, int columns,
+                                        cudaStream_t stream) {
+  if (rows <= 0 || columns <= 0 || (rows + kBlock - 1) / kBlock > 65535) {
+    mir_set_error("quantize_weight_8bit: a weight of %d x %d is not one it takes", rows, columns);
+    return MIR_BAD_ARGUMENT;
+  }
+  const dim3 grid((columns + kBlock - 1) / kBlock, (rows + kBlock - 1) / kBlock);
+  if (is_bf16)
+    return mir_launch("quantize_weight_8bit", quantize_weight_kernel<bf16>, grid, dim3(256), 0, stream, 0, (const bf16*)weight,
+                      (uint8_t*)codes, scales, rows, columns);
+  return mir_launch("quantize_weight_8bit", quantize_weight_kernel<float>, grid, dim3(256), 0, stream, 0, (const float*)weight,
+                    (uint8_t*)codes, scales, rows, columns);
+}
+
+MIR_EXPORT int mir_linear_8bit(const void* x, long long x_stride, const void* weight, const float* w_scales, const void* bias, void* out,
+                               long long out_stride, int out_float, int accumulate, int m, int n, int k, void* workspace,
+                               long long workspace_bytes, cudaStream_t stream) {
+  if (m == 0 || n == 0) return MIR_OK;
+  if (m < 0 || n < 0 || k <= 0 || (k % 16) || x_stride < k || (x_stride % 4) || out_stride < n || ((uintptr_t)x & 7) ||
+      ((uintptr_t)weight & 15) || (accumulate && !out_float) || (m + kTile - 1) / kTile > 65535) {
+    mir_set_error("linear_8bit: takes columns in multiples of 16, rows of x on 8-byte boundaries and weights on 16-byte ones, "
+                  "and accumulates into float32 (m %d, n %d, k %d, row strides %lld and %lld)", m, n, k, x_stride, out_stride);
+    return MIR_BAD_ARGUMENT;
+  }
+  if (workspace == nullptr || workspace_bytes < mir_linear_8bit_workspace(m, k) || ((uintptr_t)workspace & 15)) {
+    mir_set_error("linear_8bit: %lld bytes of 16-byte aligned workspace are needed, got %lld", mir_linear_8bit_workspace(m, k),
+                  workspace_bytes);
+    return MIR_BAD_ARGUMENT;
+  }
+  const int blocks = (k + kBlock - 1) / kBlock;
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  float* scales = reinterpret_cast<float*>(codes + ((size_t)m * k + 255) / 256 * 256);
+  const long long units = (long long)m * blocks;
+  if ((units + 7) / 8 > 0x7fffffffll) {
+    mir_set_error("linear_8bit: %d rows of %d columns are more than one launch takes", m, k);
+    return MIR_BAD_ARGUMENT;
+  }
+  const int status = mir_launch("quantize_rows_8bit", quantize_rows_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream, 0,
+                                (const bf16*)x, x_stride, codes, scales, m, k, blocks);
+  if (status != MIR_OK) return status;
+  const dim3 grid((n + kTile - 1) / kTile, (m + kTile - 1) / kTile);
+  return mir_launch("linear_8bit", linear_8bit_kernel, grid, dim3(128), 0, stream, 0, codes, scales, (const uint8_t*)weight, w_scales,
+                    bias, out, out_stride, m, n, k, out_float != 0, accumulate != 0);
+}

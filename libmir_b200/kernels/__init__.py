@@ -229,7 +229,24 @@ _SIGNATURES = {
         "mir_gemm_bf16_lt": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                              c_float, c_void_p, c_size_t, c_void_p],
     },
+    "eight_bit": {
+        "mir_store_8bit": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                           c_int, c_void_p],
+        "mir_decode_attention_8bit_plan": [c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
+        "mir_decode_attention_8bit": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                      c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_longlong,
+                                      c_void_p, c_void_p],
+        "mir_prefill_attention_8bit": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                       c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
+                                       c_void_p, c_longlong, c_void_p, c_void_p],
+        "mir_linear_8bit_workspace": [c_int, c_int],
+        "mir_quantize_weight_8bit": [c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
+        "mir_linear_8bit": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int,
+                            c_void_p, c_longlong, c_void_p],
+    },
 }
+# functions that return something else than a status or a small number
+_RESULTS = {"mir_linear_8bit_workspace": c_longlong}
 
 
 def set_build_verbosity(verbose: bool) -> None:
@@ -300,7 +317,7 @@ def library(name: str) -> ctypes.CDLL:
     for symbol, argtypes in _SIGNATURES.get(name, {}).items():
         function = getattr(lib, symbol)
         function.argtypes = argtypes
-        function.restype = c_int
+        function.restype = _RESULTS.get(symbol, c_int)
     _LIBS[name] = lib
     return lib
 
@@ -321,7 +338,7 @@ def set_programmatic_launch(mode) -> None:
     first weights are then on their way while the kernel before them drains.  What is read ahead of that wait (weights of
     products and norms, slots, positions, block tables) must not come from the launches in front of it: between the kernel
     that writes it and the one that reads it lies a copy, a library's kernel or decode_prepare, and one launch more."""
-    for name in ("core", "bf16"):
+    for name in ("core", "bf16", "eight_bit"):
         lib = library(name)
         lib.mir_set_pdl.argtypes = [c_int]
         lib.mir_set_pdl.restype = None
@@ -2364,3 +2381,7 @@ def repetition_penalty(logits: torch.Tensor, ids: torch.Tensor, id_rows: torch.T
     lib = library("core")
     _check(lib, lib.mir_repetition_penalty(logits.data_ptr(), logits.stride(0), vocab, ids.data_ptr(),
                                            id_rows.data_ptr(), penalties.data_ptr(), ids.numel(), _stream()))
+
+
+from .eight_bit import (decode_attention_8bit, decode_attention_8bit_plan, linear_8bit,  # noqa: E402,F401
+                        prefill_attention_8bit, quantize_weight_8bit, store_kv_8bit)
