@@ -51,8 +51,8 @@ LIBRARIES = {
     },
     # the operators for serving in 8 bits
     "eight_bit": {
-        "sources": ["runtime.cu", "store_8bit.cu", "attention_8bit.cu", "linear_8bit.cu"],
-        "headers": ["eight_bit.h", "eight_bit.cuh", "tcgen05.cuh"],
+        "sources": ["runtime.cu", "store_8bit.cu", "attention_8bit.cu", "linear_8bit.cu", "linear_8bit_tc.cu"],
+        "headers": ["eight_bit.h", "eight_bit.cuh", "eight_bit_tc.cuh", "tcgen05.cuh"],
         "link": [],
         "defines": [],
     },

@@ -7,7 +7,7 @@
 // so out[m, n] = sum over blocks b of 128 columns of  sx[m, b] sw[n / 128, b] (sum over k in b of xq[m, k] wq[n, k]), the inner
 // sums and the outer one in 32 bits.
 #include <algorithm>
-#include "eight_bit.cuh"
+#include "eight_bit.h"
 
 using namespace mir;
 typedef __nv_bfloat16 bf16;
@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kBlock = 128;             // columns (and rows of a weight) that share a scale
 
-// A warp rounds 128 columns of one row: a lane four of them.
+// A warp rounds 128 columns of one row: a lane four of them.  scales: [blocks, rows], so that neighbouring rows' are side by side.
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const bf16* __restrict__ x, long long stride, uint8_t* __restrict__ codes, float* __restrict__ scales, int rows,
                      int columns, int blocks) {
@@ -44,7 +44,7 @@ quantize_rows_kernel(const bf16* __restrict__ x, long long stride, uint8_t* __re
   if (there)
     *reinterpret_cast<uint32_t*>(codes + (size_t)row * columns + column) =
         to_e4m3x2(v[0] * inverse, v[1] * inverse) | (to_e4m3x2(v[2] * inverse, v[3] * inverse) << 16);
-  if (lane == 0) scales[unit] = power_of_two(exponent);
+  if (lane == 0) scales[(size_t)block * rows + row] = power_of_two(exponent);
 }
 
 // A weight's blocks of 128 x 128 to e4m3 with scale largest / 448: what a checkpoint would hold.
@@ -135,7 +135,7 @@ linear_8bit_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_sc
     const float w_scale = w_scales[(size_t)(column0 / kBlock) * blocks + block];
     float scale[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) scale[i] = rows[i] < m ? x_scales[(size_t)rows[i] * blocks + block] * w_scale : 0.0f;
+    for (int i = 0; i < 2; ++i) scale[i] = rows[i] < m ? x_scales[(size_t)block * m + rows[i]] * w_scale : 0.0f;
 #pragma unroll
     for (int c = 0; c < kTile / 8; ++c)
 #pragma unroll
@@ -209,6 +209,9 @@ MIR_EXPORT int mir_linear_8bit(const void* x, long long x_stride, const void* we
   const int status = mir_launch("quantize_rows_8bit", quantize_rows_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream, 0,
                                 (const bf16*)x, x_stride, codes, scales, m, k, blocks);
   if (status != MIR_OK) return status;
+  if (m > 128)
+    return mir_linear_8bit_tiles(codes, scales, static_cast<const uint8_t*>(weight), w_scales, bias, out, out_stride, m, n, k,
+                                 out_float != 0, accumulate != 0, stream);
   const dim3 grid((n + kTile - 1) / kTile, (m + kTile - 1) / kTile);
   return mir_launch("linear_8bit", linear_8bit_kernel, grid, dim3(128), 0, stream, 0, codes, scales, (const uint8_t*)weight, w_scales,
                     bias, out, out_stride, m, n, k, out_float != 0, accumulate != 0);

@@ -1,0 +1,252 @@
+// Products of many rounded rows with an 8-bit weight on the 5th-generation tensor cores:
+//
+//   out[m, n] = sum over blocks b of 128 columns of  sx[b, m] sw[n / 128, b] (xq[m, b] . wq[n, b])
+//
+// One CTA per SM walks over tiles of 128 rows x 256 columns.  A block of 128 columns is one stage of the ring (16 KB of xq,
+// 32 KB of wq: rows of 128 bytes, TMA with the 128-byte swizzle) and four tcgen05.mma kind::f8f6f4 (K = 32 each) into one of
+// two accumulators in tensor memory.  The blocks' scales differ, so a block's sums cannot stay there: eight warps read them
+// (tcgen05.ld), multiply them with the block's scale and add them to 32-bit sums in registers, 128 columns of one row per thread
+// (a weight's scale is the same for 128 columns: one factor per thread and block), while the tensor cores fill the other
+// accumulator.  The tensor cores need 512 cycles for a block of a tile; a warp reads 4 x 32 columns and adds them with 64
+// two-wide FMAs, two warps a scheduler, so the adding hides behind the products.
+#include <algorithm>
+#include "eight_bit_tc.cuh"
+
+using namespace mir;
+using namespace mir::tc;
+typedef __nv_bfloat16 bf16;
+
+namespace {
+
+constexpr int kRows = 128, kColumns = 256, kBlock = 128;
+constexpr int kStages = 4, kStageBytes = (kRows + kColumns) * kBlock;
+// Loader, issuer and two warps that only make up the first warpgroup, then the adders: registers are handed out to four warps at a
+// time.  Launched with 168 a thread (3 * 168 = 504); the first four warps give theirs up, 56 + 2 * 224 = 504.
+constexpr int kAddingWarps = 8, kThreads = (4 + kAddingWarps) * 32;
+constexpr int kFewRegisters = 56, kManyRegisters = 224;
+static_assert(kFewRegisters + 2 * kManyRegisters <= 3 * 168, "no more registers than the launch holds");
+constexpr uint32_t kTmemColumns = 512;
+constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+static_assert(kSmemBytes + kLeastSharedBeside > kSharedOfSm, "no other kernel with tensor memory beside this one");
+
+enum { FULL = 0, EMPTY = FULL + kStages, SUM_FULL = EMPTY + kStages, SUM_FREE = SUM_FULL + 2, BARRIERS = SUM_FREE + 2 };
+
+__device__ int g_error = 0;
+
+template <bool OUT_FLOAT>
+__global__ void __launch_bounds__(kThreads, 1)
+linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
+                         const float* __restrict__ x_scales, const float* __restrict__ w_scales, const void* __restrict__ bias,
+                         void* __restrict__ out, long long out_stride, int m, int n, int k, int row_tiles, int tiles, bool accumulate) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) unsigned long long barriers[BARRIERS];
+  __shared__ uint32_t tmem_slot;
+  if (*reinterpret_cast<volatile int*>(&g_error) != 0) {       // an earlier wait ran out: do not queue up more
+    grid_dependency_wait();
+    return;
+  }
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
+  auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int blocks = (k + kBlock - 1) / kBlock;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < BARRIERS; ++i) barrier_init(bar(i), i >= SUM_FREE ? (uint32_t)kAddingWarps : 1u);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tensor_fence_before_sync();
+  __syncthreads();
+  tensor_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+  if (warp == 0) {
+    // ------------------------------------------------------------------ loader
+    if (lane == 0) {
+      uint32_t stage = 0, parity = 0;
+      bool alive = true;
+      for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
+        const int row0 = tile % row_tiles * kRows, column0 = tile / row_tiles * kColumns;
+        for (int b = 0; b < blocks; ++b) {
+          if (!wait_barrier(bar(EMPTY + stage), parity ^ 1u)) { g_error = 1; alive = false; break; }
+          const uint32_t full = bar(FULL + stage), to = smem_base + stage * (uint32_t)kStageBytes;
+          barrier_expect_bytes(full, (uint32_t)kStageBytes);
+          tma_load_2d(to, &x_map, full, b * kBlock, row0);
+          tma_load_2d(to + kRows * kBlock, &w_map, full, b * kBlock, column0);
+          if (++stage == (uint32_t)kStages) { stage = 0; parity ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ issuer (tcgen05.cuh: from a whole warp)
+    constexpr uint32_t idesc = instruction_descriptor_8bit(kRows, kColumns, E4M3, E4M3);
+    const uint32_t elected = elect_one();
+    const uint32_t a0 = operand_low(smem_base), b0 = operand_low(smem_base + kRows * kBlock);
+    uint32_t stage = 0, parity = 0, sum = 0, sum_parity = 0;
+    bool alive = true;
+    auto check = [&](int index, uint32_t phase) {
+      if (alive && !wait_barrier(bar(index), phase)) { g_error = 2; alive = false; }
+    };
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x)
+      for (int b = 0; b < blocks; ++b) {
+        check(SUM_FREE + (int)sum, sum_parity ^ 1u);
+        check(FULL + (int)stage, parity);
+        tensor_fence_after_sync();
+        const uint32_t offset = stage * (uint32_t)(kStageBytes >> 4), d = tmem + sum * (uint32_t)kColumns;
+#pragma unroll
+        for (int kk = 0; kk < kBlock / 32; ++kk)
+          mma_8bit_ss_halves(d, a0 + offset + 2u * kk, b0 + offset + 2u * kk, idesc, kk > 0 ? 1u : 0u, elected);
+        mma_commit_elected(bar(EMPTY + (int)stage), elected);
+        mma_commit_elected(bar(SUM_FULL + (int)sum), elected);
+        if (++stage == (uint32_t)kStages) { stage = 0; parity ^= 1u; }
+        if (++sum == 2u) { sum = 0; sum_parity ^= 1u; }
+      }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    // ------------------------------------------------------------------ adders: 128 columns of a row per thread
+    const int quarter = warp & 3, half = (warp - 4) >> 2;      // a warp may read the accumulator lanes 32 quarter .. + 31
+    const uint32_t lane_bits = (uint32_t)(quarter * 32) << 16;
+    uint32_t sum = 0, sum_parity = 0;
+    bool alive = true;
+    for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
+      const int row = tile % row_tiles * kRows + quarter * 32 + lane, column0 = tile / row_tiles * kColumns + half * 128;
+      const float* mine = x_scales + min(row, m - 1);
+      const float* theirs = w_scales + (size_t)min(column0 / kBlock, (n - 1) / kBlock) * blocks;
+      float2 total[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) total[i] = make_float2(0.0f, 0.0f);
+      float x_next = mine[0], w_next = theirs[0];
+      for (int b = 0; b < blocks; ++b) {
+        const float factor = x_next * w_next;
+        if (b + 1 < blocks) {
+          x_next = mine[(size_t)(b + 1) * m];
+          w_next = theirs[b + 1];
+        }
+        if (!wait_barrier(bar(SUM_FULL + (int)sum), sum_parity)) { g_error = 3; alive = false; break; }
+        tensor_fence_after_sync();
+        const uint32_t from = tmem + sum * (uint32_t)kColumns + (uint32_t)(half * 128) + lane_bits;
+        const float2 both = make_float2(factor, factor);
+        uint32_t v[2][32];
+        tmem_load_32_ahead(from, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_load_done(v[c & 1]);
+          if (c < 3) tmem_load_32_ahead(from + 32u * (c + 1), v[(c + 1) & 1]);
+          if (c == 3) {                                        // all of this warp's columns are in registers
+            tensor_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(bar(SUM_FREE + (int)sum));
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            total[c * 16 + i] = fma_two(make_float2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), both,
+                                        total[c * 16 + i]);
+        }
+        if (++sum == 2u) { sum = 0; sum_parity ^= 1u; }
+      }
+      if (!alive || row >= m || column0 >= n) continue;
+      const int columns = min(128, n - column0);
+      const size_t at = (size_t)row * out_stride + column0;
+      if (OUT_FLOAT) {
+        float* to = static_cast<float*>(out) + at;
+        const float* extra = static_cast<const float*>(bias);
+        const bool wide = columns == 128 && (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+          float4 value = make_float4(total[i].x, total[i].y, total[i + 1].x, total[i + 1].y);
+          float* part = reinterpret_cast<float*>(&value);
+          if (extra != nullptr)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (2 * i + j < columns) part[j] += extra[column0 + 2 * i + j];
+          if (wide) {
+            if (accumulate) {
+              const float4 old = *reinterpret_cast<const float4*>(to + 2 * i);
+              value.x += old.x; value.y += old.y; value.z += old.z; value.w += old.w;
+            }
+            *reinterpret_cast<float4*>(to + 2 * i) = value;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (2 * i + j < columns) to[2 * i + j] = accumulate ? to[2 * i + j] + part[j] : part[j];
+          }
+        }
+      } else {
+        bf16* to = static_cast<bf16*>(out) + at;
+        const bf16* extra = static_cast<const bf16*>(bias);
+        const bool wide = columns == 128 && (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+          if (extra != nullptr)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (2 * (i + j) < columns) total[i + j].x += __bfloat162float(extra[column0 + 2 * (i + j)]);
+              if (2 * (i + j) + 1 < columns) total[i + j].y += __bfloat162float(extra[column0 + 2 * (i + j) + 1]);
+            }
+          if (wide) {
+            uint4 packed;
+            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(total[i + j].x, total[i + j].y);
+            *reinterpret_cast<uint4*>(to + 2 * i) = packed;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (2 * (i + j) < columns) to[2 * (i + j)] = __float2bfloat16_rn(total[i + j].x);
+              if (2 * (i + j) + 1 < columns) to[2 * (i + j) + 1] = __float2bfloat16_rn(total[i + j].y);
+            }
+          }
+        }
+      }
+    }
+    tensor_fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tensor_fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
+  }
+}
+
+}  // namespace
+
+// 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 loader, 2 issuer, 3 adders).
+// Synchronises the device.
+MIR_EXPORT int mir_linear_8bit_tiles_error() {
+  int flag = 0;
+  if (cudaMemcpyFromSymbol(&flag, g_error, sizeof(int)) != cudaSuccess) return -1;
+  return flag;
+}
+
+int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, const uint8_t* weight, const float* w_scales, const void* bias,
+                          void* out, long long out_stride, int m, int n, int k, bool out_float, bool accumulate, cudaStream_t stream) {
+  CUtensorMap x_map, w_map;
+  int status = tensor_map_of_bytes(codes, m, k, k, kRows, &x_map);
+  if (status != MIR_OK) return status;
+  status = tensor_map_of_bytes(weight, n, k, k, kColumns, &w_map);
+  if (status != MIR_OK) return status;
+  const int row_tiles = (m + kRows - 1) / kRows;
+  const long long tiles = (long long)row_tiles * ((n + kColumns - 1) / kColumns);
+  if (tiles > 0x7fffffffll) {
+    mir_set_error("linear_8bit: %d rows of %d columns are more than one launch takes", m, n);
+    return MIR_BAD_ARGUMENT;
+  }
+  auto kernel = out_float ? linear_8bit_tiles_kernel<true> : linear_8bit_tiles_kernel<false>;
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (err != cudaSuccess) {
+    mir_set_error("linear_8bit: cannot reserve %d bytes of shared memory: %s", kSmemBytes, cudaGetErrorString(err));
+    return MIR_CUDA_ERROR;
+  }
+  const int ctas = (int)std::min<long long>(tiles, mir_sm_count());
+  return mir_launch("linear_8bit_tiles", kernel, dim3(ctas), dim3(kThreads), (size_t)kSmemBytes, stream, 0, x_map, w_map, scales, w_scales,
+                    bias, out, out_stride, m, n, k, row_tiles, (int)tiles, accumulate);
+}
