@@ -31,7 +31,8 @@ struct Attention8 {
 int mir_attention_8bit_general(const Attention8& a, int tokens);
 int mir_merge_8bit(const Attention8& a, int tokens);
 
-// The product of rounded rows (codes [m, k], scales [blocks of 128 columns, m]) with an 8-bit weight, by tiles of 128 rows
+// The product of rounded rows (codes [m, k], scales [blocks of 128 columns, scale_stride], scale_stride m
+// filled up to whole 128) with an 8-bit weight, by tiles of 128 rows
 // on the tensor cores (linear_8bit_tc.cu).
-int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, const uint8_t* weight, const float* w_scales, const void* bias,
-                          void* out, long long out_stride, int m, int n, int k, bool out_float, bool accumulate, cudaStream_t stream);
+int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, int scale_stride, const uint8_t* weight, const float* w_scales,
+                          const void* bias, void* out, long long out_stride, int m, int n, int k, bool out_float, bool accumulate, cudaStream_t stream);

@@ -33,14 +33,16 @@ __device__ __forceinline__ void mma_8bit_ss_halves(uint32_t tmem_d, uint32_t a_l
       : "memory");
 }
 
-// Tensor map of a row-major matrix of bytes [rows, bytes] with row stride `ld` bytes (a multiple of 16): boxes of box_rows rows x
-// 128 bytes, 128-byte swizzle, out-of-range elements read as zero.  A map says no more than its arguments do.
-inline int tensor_map_of_bytes(const void* base, long long rows, long long bytes, long long ld, int box_rows, CUtensorMap* map) {
+// Tensor map of a row-major matrix [rows, columns] of bytes, bf16 or float32 with row stride `ld` bytes (a multiple of 16): boxes of
+// box_rows rows x box_bytes (64 or 128) with the swizzle of that width, out-of-range elements read as zero and not written.  A map says no more than its
+// arguments do, and is looked up by all of them.
+inline int tensor_map_of(const void* base, CUtensorMapDataType type, int width, long long rows, long long columns, long long ld,
+                         int box_rows, int box_bytes, CUtensorMap* map) {
   static std::mutex g_mutex;
   static EncodeTiled g_encode = nullptr;
-  static std::map<std::tuple<const void*, long long, long long, long long, int>, CUtensorMap> g_maps;
+  static std::map<std::tuple<const void*, int, long long, long long, long long, int, int>, CUtensorMap> g_maps;
   std::lock_guard<std::mutex> lock(g_mutex);
-  const auto key = std::make_tuple(base, rows, bytes, ld, box_rows);
+  const auto key = std::make_tuple(base, (int)type, rows, columns, ld, box_rows, box_bytes);
   const auto found = g_maps.find(key);
   if (found != g_maps.end()) {
     *map = found->second;
@@ -56,23 +58,31 @@ inline int tensor_map_of_bytes(const void* base, long long rows, long long bytes
     }
     g_encode = reinterpret_cast<EncodeTiled>(entry);
   }
-  const cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
+  const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)ld};
-  const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {(cuuint32_t)(box_bytes / width), (cuuint32_t)box_rows};
   const cuuint32_t element_strides[2] = {1, 1};
   CUtensorMap made;
-  const CUresult status = g_encode(&made, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, element_strides,
-                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const CUresult status = g_encode(&made, type, 2, const_cast<void*>(base), dims, strides, box, element_strides,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (status != CUDA_SUCCESS) {
-    mir_set_error("tensor map: cuTensorMapEncodeTiled refused %lld rows of %lld bytes with row stride %lld (status %d)", rows, bytes, ld,
-                  (int)status);
+    mir_set_error("tensor map: cuTensorMapEncodeTiled refused %lld rows of %lld columns with row stride %lld (status %d)", rows, columns,
+                  ld, (int)status);
     return MIR_LIBRARY_ERROR;
   }
   if (g_maps.size() > 4096) g_maps.clear();
   g_maps.emplace(key, made);
   *map = made;
   return MIR_OK;
+}
+inline int tensor_map_of_bytes(const void* base, long long rows, long long bytes, long long ld, int box_rows, CUtensorMap* map) {
+  return tensor_map_of(base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, bytes, ld, box_rows, 128, map);
+}
+inline int tensor_map_of_results(const void* base, bool is_float, long long rows, long long columns, long long ld, CUtensorMap* map) {
+  return tensor_map_of(base, is_float ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, is_float ? 4 : 2, rows, columns,
+                       ld, 32, 64, map);
 }
 
 // a * b + c of two numbers side by side.

@@ -16,10 +16,10 @@ namespace {
 
 constexpr int kBlock = 128;             // columns (and rows of a weight) that share a scale
 
-// A warp rounds 128 columns of one row: a lane four of them.  scales: [blocks, rows], so that neighbouring rows' are side by side.
+// A warp rounds 128 columns of one row: a lane four of them.  scales: [blocks, scale_stride], rows side by side.
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const bf16* __restrict__ x, long long stride, uint8_t* __restrict__ codes, float* __restrict__ scales, int rows,
-                     int columns, int blocks) {
+                     int columns, int blocks, int scale_stride) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -44,7 +44,7 @@ quantize_rows_kernel(const bf16* __restrict__ x, long long stride, uint8_t* __re
   if (there)
     *reinterpret_cast<uint32_t*>(codes + (size_t)row * columns + column) =
         to_e4m3x2(v[0] * inverse, v[1] * inverse) | (to_e4m3x2(v[2] * inverse, v[3] * inverse) << 16);
-  if (lane == 0) scales[(size_t)block * rows + row] = power_of_two(exponent);
+  if (lane == 0) scales[(size_t)block * scale_stride + row] = power_of_two(exponent);
 }
 
 // A weight's blocks of 128 x 128 to e4m3 with scale largest / 448: what a checkpoint would hold.
@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 
 // A tile of 64 rows and 64 columns of the result; codes are taken to float16 (exact) on their way into shared memory.
 __global__ void __launch_bounds__(128)
-linear_8bit_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_scales, const uint8_t* __restrict__ weight,
+linear_8bit_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_scales, int scale_stride, const uint8_t* __restrict__ weight,
                    const float* __restrict__ w_scales, const void* __restrict__ bias, void* __restrict__ out, long long out_stride,
                    int m, int n, int k, bool out_float, bool accumulate) {
   __shared__ __align__(16) __half a_tile[kTile * kStride];
@@ -135,7 +135,7 @@ linear_8bit_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_sc
     const float w_scale = w_scales[(size_t)(column0 / kBlock) * blocks + block];
     float scale[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) scale[i] = rows[i] < m ? x_scales[(size_t)block * m + rows[i]] * w_scale : 0.0f;
+    for (int i = 0; i < 2; ++i) scale[i] = rows[i] < m ? x_scales[(size_t)block * scale_stride + rows[i]] * w_scale : 0.0f;
 #pragma unroll
     for (int c = 0; c < kTile / 8; ++c)
 #pragma unroll
@@ -162,11 +162,14 @@ linear_8bit_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_sc
 
 }  // namespace
 
+// Scales of a block: one for each row, filled up to whole tiles of 128 rows.
+static int scale_stride_of(int m) { return (m + kBlock - 1) / kBlock * kBlock; }
+
 // Bytes of workspace for m rows of k columns: the rounded rows, then their scales.
 MIR_EXPORT long long mir_linear_8bit_workspace(int m, int k) {
   if (m <= 0 || k <= 0) return 0;
   const long long codes = ((long long)m * k + 255) / 256 * 256;
-  return codes + (long long)m * ((k + kBlock - 1) / kBlock) * (long long)sizeof(float);
+  return codes + (long long)scale_stride_of(m) * ((k + kBlock - 1) / kBlock) * (long long)sizeof(float);
 }
 
 MIR_EXPORT int mir_quantize_weight_8bit(int is_bf16, const void* weight, void* codes, float* scales, int rows, int columns,
@@ -207,12 +210,12 @@ MIR_EXPORT int mir_linear_8bit(const void* x, long long x_stride, const void* we
     return MIR_BAD_ARGUMENT;
   }
   const int status = mir_launch("quantize_rows_8bit", quantize_rows_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream, 0,
-                                (const bf16*)x, x_stride, codes, scales, m, k, blocks);
+                                (const bf16*)x, x_stride, codes, scales, m, k, blocks, scale_stride_of(m));
   if (status != MIR_OK) return status;
   if (m > 128)
-    return mir_linear_8bit_tiles(codes, scales, static_cast<const uint8_t*>(weight), w_scales, bias, out, out_stride, m, n, k,
+    return mir_linear_8bit_tiles(codes, scales, scale_stride_of(m), static_cast<const uint8_t*>(weight), w_scales, bias, out, out_stride, m, n, k,
                                  out_float != 0, accumulate != 0, stream);
   const dim3 grid((n + kTile - 1) / kTile, (m + kTile - 1) / kTile);
-  return mir_launch("linear_8bit", linear_8bit_kernel, grid, dim3(128), 0, stream, 0, codes, scales, (const uint8_t*)weight, w_scales,
-                    bias, out, out_stride, m, n, k, out_float != 0, accumulate != 0);
+  return mir_launch("linear_8bit", linear_8bit_kernel, grid, dim3(128), 0, stream, 0, codes, scales, scale_stride_of(m),
+                    (const uint8_t*)weight, w_scales, bias, out, out_stride, m, n, k, out_float != 0, accumulate != 0);
 }

@@ -21,25 +21,45 @@ namespace {
 constexpr int kRows = 128, kColumns = 256, kBlock = 128;
 constexpr int kStages = 4, kStageBytes = (kRows + kColumns) * kBlock;
 // Loader, issuer and two warps that only make up the first warpgroup, then the adders: registers are handed out to four warps at a
-// time.  Launched with 168 a thread (3 * 168 = 504); the first four warps give theirs up, 56 + 2 * 224 = 504.
+// time.  Launched with 168 a thread (3 * 168 = 504); the first four warps give theirs up, 40 + 2 * 232 = 504.
 constexpr int kAddingWarps = 8, kThreads = (4 + kAddingWarps) * 32;
-constexpr int kFewRegisters = 56, kManyRegisters = 224;
+constexpr int kFewRegisters = 40, kManyRegisters = 232;
 static_assert(kFewRegisters + 2 * kManyRegisters <= 3 * 168, "no more registers than the launch holds");
 constexpr uint32_t kTmemColumns = 512;
-constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+constexpr int kBox = 32 * 64;               // bytes of a warp's box of results: 32 rows of 64 bytes
+constexpr int kSmemBytes = kStages * kStageBytes + kAddingWarps * kBox + 1024;
 static_assert(kSmemBytes + kLeastSharedBeside > kSharedOfSm, "no other kernel with tensor memory beside this one");
 
-enum { FULL = 0, EMPTY = FULL + kStages, SUM_FULL = EMPTY + kStages, SUM_FREE = SUM_FULL + 2, BARRIERS = SUM_FREE + 2 };
+// Rows' scales of a block, 512 bytes a slot.  The slot of block b is written again for block b + kScaleSlots, which the loader asks for
+// when the products of block b + kScaleSlots - kStages = b + 2 are over; those were issued when every adder had read the sums (and the
+// scales) of block b.
+constexpr int kScaleSlots = kStages + 2;
+
+enum { FULL = 0, EMPTY = FULL + kStages, SUM_FULL = EMPTY + kStages, SCALE_FULL = SUM_FULL + 2, SUM_FREE = SCALE_FULL + kScaleSlots,
+       BARRIERS = SUM_FREE + 2 };
 
 __device__ int g_error = 0;
+
+// A box of results out of shared memory (in the swizzled layout), stored or, ADD, added in 32 bits.
+template <bool ADD>
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+  if (ADD)
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(x), "r"(y) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 
 template <bool OUT_FLOAT>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
-                         const float* __restrict__ x_scales, const float* __restrict__ w_scales, const void* __restrict__ bias,
-                         void* __restrict__ out, long long out_stride, int m, int n, int k, int row_tiles, int tiles, bool accumulate) {
+                         const __grid_constant__ CUtensorMap out_map, bool boxes, const float* __restrict__ x_scales, const float* __restrict__ w_scales, const void* __restrict__ bias,
+                         void* __restrict__ out, long long out_stride, int m, int n, int k, int scale_stride, int row_tiles, int tiles, bool accumulate) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long barriers[BARRIERS];
+  __shared__ __align__(16) float scales_here[kScaleSlots * kRows];
   __shared__ uint32_t tmem_slot;
   if (*reinterpret_cast<volatile int*>(&g_error) != 0) {       // an earlier wait ran out: do not queue up more
     grid_dependency_wait();
@@ -71,7 +91,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
   if (warp == 0) {
     // ------------------------------------------------------------------ loader
     if (lane == 0) {
-      uint32_t stage = 0, parity = 0;
+      uint32_t stage = 0, parity = 0, slot = 0;
       bool alive = true;
       for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
         const int row0 = tile % row_tiles * kRows, column0 = tile / row_tiles * kColumns;
@@ -81,6 +101,12 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
           barrier_expect_bytes(full, (uint32_t)kStageBytes);
           tma_load_2d(to, &x_map, full, b * kBlock, row0);
           tma_load_2d(to + kRows * kBlock, &w_map, full, b * kBlock, column0);
+          barrier_expect_bytes(bar(SCALE_FULL + (int)slot), (uint32_t)(kRows * sizeof(float)));
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                           smem_u32(scales_here + slot * kRows)), "l"(x_scales + (size_t)b * scale_stride + row0),
+                       "r"((uint32_t)(kRows * sizeof(float))), "r"(bar(SCALE_FULL + (int)slot))
+                       : "memory");
+          if (++slot == (uint32_t)kScaleSlots) slot = 0;
           if (++stage == (uint32_t)kStages) { stage = 0; parity ^= 1u; }
         }
       }
@@ -115,23 +141,26 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
     // ------------------------------------------------------------------ adders: 128 columns of a row per thread
     const int quarter = warp & 3, half = (warp - 4) >> 2;      // a warp may read the accumulator lanes 32 quarter .. + 31
     const uint32_t lane_bits = (uint32_t)(quarter * 32) << 16;
-    uint32_t sum = 0, sum_parity = 0;
+    uint32_t sum = 0, sum_parity = 0, slot = 0, slot_parity = 0;
     bool alive = true;
     for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
       const int row = tile % row_tiles * kRows + quarter * 32 + lane, column0 = tile / row_tiles * kColumns + half * 128;
-      const float* mine = x_scales + min(row, m - 1);
+      // A weight's scales come 32 blocks at a time, a block to a lane, the next 32 ahead of their use.
       const float* theirs = w_scales + (size_t)min(column0 / kBlock, (n - 1) / kBlock) * blocks;
+      float w_held = theirs[min(lane, blocks - 1)], w_next = theirs[min(32 + lane, blocks - 1)];
       float2 total[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) total[i] = make_float2(0.0f, 0.0f);
-      float x_next = mine[0], w_next = theirs[0];
       for (int b = 0; b < blocks; ++b) {
-        const float factor = x_next * w_next;
-        if (b + 1 < blocks) {
-          x_next = mine[(size_t)(b + 1) * m];
-          w_next = theirs[b + 1];
+        if (b > 0 && (b & 31) == 0) {
+          w_held = w_next;
+          w_next = theirs[min(b + 32 + lane, blocks - 1)];
         }
-        if (!wait_barrier(bar(SUM_FULL + (int)sum), sum_parity)) { g_error = 3; alive = false; break; }
+        if (alive && !wait_barrier(bar(SCALE_FULL + (int)slot), slot_parity)) { g_error = 3; alive = false; }
+        const float factor = scales_here[slot * kRows + quarter * 32 + lane] * __shfl_sync(0xffffffffu, w_held, b & 31);
+        if (++slot == (uint32_t)kScaleSlots) { slot = 0; slot_parity ^= 1u; }
+        if (alive && !wait_barrier(bar(SUM_FULL + (int)sum), sum_parity)) { g_error = 3; alive = false; }
+        __syncwarp();
         tensor_fence_after_sync();
         const uint32_t from = tmem + sum * (uint32_t)kColumns + (uint32_t)(half * 128) + lane_bits;
         const float2 both = make_float2(factor, factor);
@@ -152,6 +181,51 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
                                         total[c * 16 + i]);
         }
         if (++sum == 2u) { sum = 0; sum_parity ^= 1u; }
+      }
+      alive = __all_sync(0xffffffffu, alive);
+      if (boxes) {
+        // Results by way of shared memory, a box of 32 rows of 64 bytes a warp: the stores are whole sectors, and the next tile's
+        // sums are waited for while they are on their way (a thread that stores its own row, 16 bytes of a line at a time, took
+        // a tenth of the kernel's time).
+        constexpr int kPart = OUT_FLOAT ? 16 : 32;             // columns of a box
+        const int row_first = tile % row_tiles * kRows + quarter * 32;
+        const uint32_t box = smem_base + (uint32_t)(kStages * kStageBytes + (warp - 4) * kBox);
+#pragma unroll
+        for (int part = 0; part < 128 / kPart; ++part) {
+          const int column = column0 + part * kPart;
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");          // the box before has been read
+          __syncwarp();
+#pragma unroll
+          for (int chunk = 0; chunk < 4; ++chunk) {            // 16 bytes of this thread's row
+            uint32_t words[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (OUT_FLOAT) {
+                const float2 pair = total[part * 8 + chunk * 2 + i / 2];
+                float value = i % 2 ? pair.y : pair.x;
+                if (bias != nullptr && column + chunk * 4 + i < n) value += static_cast<const float*>(bias)[column + chunk * 4 + i];
+                words[i] = __float_as_uint(value);
+              } else {
+                float2 pair = total[part * 16 + chunk * 4 + i];
+                const int at = column + chunk * 8 + 2 * i;
+                if (bias != nullptr && at < n) pair.x += __bfloat162float(static_cast<const bf16*>(bias)[at]);
+                if (bias != nullptr && at + 1 < n) pair.y += __bfloat162float(static_cast<const bf16*>(bias)[at + 1]);
+                const __nv_bfloat162 both = __floats2bfloat162_rn(pair.x, pair.y);
+                words[i] = *reinterpret_cast<const uint32_t*>(&both);
+              }
+            }
+            const uint32_t to = box + (uint32_t)(lane * 64 + ((chunk ^ (lane >> 1 & 3)) << 4));      // (64-byte swizzle)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(words[0]), "r"(words[1]), "r"(words[2]), "r"(words[3])
+                         : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && alive && row_first < m && column < n) {
+            if (OUT_FLOAT && accumulate) tma_store_2d<true>(&out_map, box, column, row_first);
+            else tma_store_2d<false>(&out_map, box, column, row_first);
+          }
+        }
+        continue;
       }
       if (!alive || row >= m || column0 >= n) continue;
       const int columns = min(128, n - column0);
@@ -208,6 +282,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
         }
       }
     }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     tensor_fence_before_sync();
   }
   __syncthreads();
@@ -227,7 +302,7 @@ MIR_EXPORT int mir_linear_8bit_tiles_error() {
   return flag;
 }
 
-int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, const uint8_t* weight, const float* w_scales, const void* bias,
+int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, int scale_stride, const uint8_t* weight, const float* w_scales, const void* bias,
                           void* out, long long out_stride, int m, int n, int k, bool out_float, bool accumulate, cudaStream_t stream) {
   CUtensorMap x_map, w_map;
   int status = tensor_map_of_bytes(codes, m, k, k, kRows, &x_map);
@@ -246,7 +321,15 @@ int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, const uint8
     mir_set_error("linear_8bit: cannot reserve %d bytes of shared memory: %s", kSmemBytes, cudaGetErrorString(err));
     return MIR_CUDA_ERROR;
   }
+  // results by way of shared memory where their rows begin and lie on 16-byte boundaries
+  const int width = out_float ? 4 : 2;
+  const bool boxes = ((uintptr_t)out & 15) == 0 && (out_stride * width) % 16 == 0;
+  CUtensorMap out_map = x_map;
+  if (boxes) {
+    status = tensor_map_of_results(out, out_float, m, n, out_stride * width, &out_map);
+    if (status != MIR_OK) return status;
+  }
   const int ctas = (int)std::min<long long>(tiles, mir_sm_count());
-  return mir_launch("linear_8bit_tiles", kernel, dim3(ctas), dim3(kThreads), (size_t)kSmemBytes, stream, 0, x_map, w_map, scales, w_scales,
-                    bias, out, out_stride, m, n, k, row_tiles, (int)tiles, accumulate);
+  return mir_launch("linear_8bit_tiles", kernel, dim3(ctas), dim3(kThreads), (size_t)kSmemBytes, stream, 0, x_map, w_map, out_map, boxes,
+                    scales, w_scales, bias, out, out_stride, m, n, k, scale_stride, row_tiles, (int)tiles, accumulate);
 }
