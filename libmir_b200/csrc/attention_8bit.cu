@@ -247,15 +247,15 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
     if (!valid[i]) continue;
     const size_t row = (size_t)token[i] * heads + head[i];
     if (num_partitions == 1) {
-      if (total > 0.0f && sinks != nullptr) total += exp2f(sinks[head[i]] * kLog2e - top[i]);
-      const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+      if (total != 0.0f && sinks != nullptr) total += exp2f(sinks[head[i]] * kLog2e - top[i]);
+      const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
       for (int n = 0; n < DIM / 8; ++n)
         *reinterpret_cast<uint32_t*>(out + row * DIM + n * 8 + (lane & 3) * 2) = pack(o[n][2 * i] * inverse, o[n][2 * i + 1] * inverse);
     } else {
       const size_t at = row * num_partitions + part;
       if ((lane & 3) == 0) *reinterpret_cast<float2*>(partial_ml + at * 2) = make_float2(top[i], total);
-      if (total > 0.0f) {
+      if (total != 0.0f) {
 #pragma unroll
         for (int n = 0; n < DIM / 8; ++n)
           *reinterpret_cast<float2*>(partial_o + at * DIM + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
@@ -281,7 +281,7 @@ merge_8bit_kernel(const float* __restrict__ partial_o, const float* __restrict__
   const float2* ml = reinterpret_cast<const float2*>(partial_ml) + row * num_partitions;
   float top = -INFINITY;
   for (int p = lane; p < num_partitions; p += 32)
-    if (ml[p].y > 0.0f) top = fmaxf(top, ml[p].x);
+    if (ml[p].y != 0.0f) top = fmaxf(top, ml[p].x);
   top = warp_max(top);
   constexpr int kColumns = DIM / 32;
   float o[kColumns], total = 0.0f;
@@ -290,14 +290,14 @@ merge_8bit_kernel(const float* __restrict__ partial_o, const float* __restrict__
   const float* part = partial_o + (size_t)row * num_partitions * DIM + lane * kColumns;
   for (int p = 0; p < num_partitions; ++p, part += DIM) {
     const float2 mine = ml[p];
-    if (!(mine.y > 0.0f)) continue;
+    if (mine.y == 0.0f) continue;
     const float factor = exp2f(mine.x - top);
     total += mine.y * factor;
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) o[c] += part[c] * factor;
   }
-  if (total > 0.0f && sinks != nullptr) total += exp2f(sinks[head] * kLog2e - top);
-  const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+  if (total != 0.0f && sinks != nullptr) total += exp2f(sinks[head] * kLog2e - top);
+  const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
   uint32_t* to = reinterpret_cast<uint32_t*>(out + (size_t)row * DIM + lane * kColumns);
 #pragma unroll
   for (int c = 0; c < kColumns; c += 2) to[c / 2] = pack(o[c] * inverse, o[c + 1] * inverse);
@@ -386,7 +386,7 @@ MIR_EXPORT int mir_decode_attention_8bit(const void* q, long long q_stride, void
   a.sinks = sinks; a.stream = stream;
   if (attention_8bit_refused(a, rows)) return MIR_BAD_ARGUMENT;
   if (rows == 0) return MIR_OK;
-  return mir_attention_8bit_general(a, rows);
+  return mir_decode_8bit_takes(head_dim, page_size) ? mir_attention_8bit_decode(a) : mir_attention_8bit_general(a, rows);
 }
 
 // Portions: request r has tokens query_starts[r] .. query_starts[r + 1] - 1 of the packed rows, and its context_lens[r]

@@ -30,6 +30,9 @@ struct Attention8 {
 
 int mir_attention_8bit_general(const Attention8& a, int tokens);
 int mir_merge_8bit(const Attention8& a, int tokens);
+// Single tokens on the 5th-generation tensor cores (attention_8bit_decode.cu), where it takes the sizes.
+bool mir_decode_8bit_takes(int head_dim, int page_size);
+int mir_attention_8bit_decode(const Attention8& a);
 
 // The product of rounded rows (codes [m, k], scales [blocks of 128 columns, scale_stride], scale_stride m
 // filled up to whole 128) with an 8-bit weight, by tiles of 128 rows
