@@ -331,20 +331,20 @@ int mir_attention_8bit_general(const Attention8& a, int tokens) {
   return mir_merge_8bit(a, tokens);
 }
 
-static bool attention_8bit_refused(const Attention8& a, int tokens) {
+static bool attention_8bit_refused(const Attention8& a, int tokens, bool shared_out) {
   const bool bad =
       (a.head_dim != 64 && a.head_dim != 128) || a.heads <= 0 || a.cache.kv_heads <= 0 || a.heads % a.cache.kv_heads ||
       a.cache.page_size <= 0 || a.cache.pages <= 0 || (long long)a.cache.pages * a.cache.page_size > 0x7fffffffll || a.table_width <= 0 ||
       !(a.scale > 0.0f) || a.window < 0 || (a.q_stride % 8) || a.q_stride < (long long)a.heads * a.head_dim || ((uintptr_t)a.q & 15) ||
-      ((uintptr_t)a.out & 15) || ((uintptr_t)a.cache.k & 15) || ((uintptr_t)a.cache.v & 15) || a.partition <= 0 || a.partition % 128 ||
-      a.num_partitions <= 0 || a.num_partitions > 65535 || a.num_rows < 0 || tokens < 0;
+      ((uintptr_t)a.out & 15) || ((uintptr_t)a.cache.k & 15) || ((uintptr_t)a.cache.v & 15) ||
+      (shared_out ? a.partition != 0 : a.partition <= 0 || a.partition % 128 != 0) || a.num_partitions <= 0 || a.num_partitions > 65535 || a.num_rows < 0 || tokens < 0;
   if (bad) {
-    mir_set_error("%s: takes head_dim 64 or 128, a positive scale, partitions of whole 128 keys and 16-byte aligned tensors (head_dim "
+    mir_set_error("%s: takes head_dim 64 or 128, a positive scale, a plan's partitions and 16-byte aligned tensors (head_dim "
                   "%d, heads %d, kv heads %d, page %d, pages %d, partition %d x %d, row stride %lld)", a.what, a.head_dim, a.heads,
                   a.cache.kv_heads, a.cache.page_size, a.cache.pages, a.partition, a.num_partitions, a.q_stride);
     return true;
   }
-  const long long need = a.num_partitions == 1 ? 0 : (long long)tokens * a.heads * a.num_partitions * (a.head_dim + 2);
+  const long long need = shared_out ? mir_decode_8bit_floats(a.num_partitions, a.heads / a.cache.kv_heads) : a.num_partitions == 1 ? 0 : (long long)tokens * a.heads * a.num_partitions * (a.head_dim + 2);
   if (need > 0 && (a.scratch == nullptr || a.scratch_floats < need)) {
     mir_set_error("%s: scratch of %lld floats is needed, got %lld", a.what, need, a.scratch_floats);
     return true;
@@ -352,7 +352,8 @@ static bool attention_8bit_refused(const Attention8& a, int tokens) {
   return false;
 }
 
-// How single tokens are split over the keys: partitions of `keys`, `count` of them, and the floats of scratch.
+// How single tokens are split over the keys: partitions of `keys`, `count` of them, and the floats of scratch.  keys 0: shared out
+// evenly over `count` CTAs.
 MIR_EXPORT int mir_decode_attention_8bit_plan(int rows, int heads, int kv_heads, int head_dim, int page_size, int max_context,
                                               int* keys, int* count, long long* floats) {
   if (rows < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context < 0 || page_size <= 0) {
@@ -360,6 +361,14 @@ MIR_EXPORT int mir_decode_attention_8bit_plan(int rows, int heads, int kv_heads,
     return MIR_BAD_ARGUMENT;
   }
   const int group = heads / kv_heads;
+  if (mir_decode_8bit_takes(head_dim, page_size)) {
+    // the tcgen05 kernel shares all requests' keys out over its CTAs by the positions that it finds
+    const long long units = (long long)kv_heads * ((group + 15) / 16);
+    *keys = 0;
+    *count = mir_decode_8bit_ctas(rows * units * std::max(1ll, (max_context + 127ll) / 128));
+    *floats = mir_decode_8bit_floats(*count, group);
+    return MIR_OK;
+  }
   const long long ctas = std::max(1ll, (long long)rows * kv_heads * ((group + kRows - 1) / kRows));
   const long long wanted = std::max(1ll, (long long)mir_sm_count() * 4 / ctas);
   const long long tiles = std::max(1ll, (max_context + 127ll) / 128);
@@ -384,9 +393,10 @@ MIR_EXPORT int mir_decode_attention_8bit(const void* q, long long q_stride, void
   a.num_rows = rows; a.heads = heads; a.head_dim = head_dim; a.scale = scale; a.window = window;
   a.partition = partition; a.num_partitions = num_partitions; a.scratch = scratch; a.scratch_floats = scratch_floats;
   a.sinks = sinks; a.stream = stream;
-  if (attention_8bit_refused(a, rows)) return MIR_BAD_ARGUMENT;
+  const bool shared_out = mir_decode_8bit_takes(head_dim, page_size);
+  if (attention_8bit_refused(a, rows, shared_out)) return MIR_BAD_ARGUMENT;
   if (rows == 0) return MIR_OK;
-  return mir_decode_8bit_takes(head_dim, page_size) ? mir_attention_8bit_decode(a) : mir_attention_8bit_general(a, rows);
+  return shared_out ? mir_attention_8bit_decode(a) : mir_attention_8bit_general(a, rows);
 }
 
 // Portions: request r has tokens query_starts[r] .. query_starts[r + 1] - 1 of the packed rows, and its context_lens[r]
@@ -405,7 +415,7 @@ MIR_EXPORT int mir_prefill_attention_8bit(const void* q, long long q_stride, voi
   a.num_rows = num_rows; a.heads = heads; a.head_dim = head_dim; a.scale = scale; a.window = window;
   a.partition = partition; a.num_partitions = num_partitions; a.scratch = scratch; a.scratch_floats = scratch_floats;
   a.sinks = sinks; a.stream = stream;
-  if (attention_8bit_refused(a, tokens)) return MIR_BAD_ARGUMENT;
+  if (attention_8bit_refused(a, tokens, false)) return MIR_BAD_ARGUMENT;
   if (num_rows == 0 || tokens == 0) return MIR_OK;
   return mir_attention_8bit_general(a, tokens);
 }

@@ -1,8 +1,12 @@
 // Attention of single tokens over the 8-bit cache on the 5th-generation tensor cores, head_dim 128, pages of 8 to 128 keys:
 // the bytes of the cache go from memory into the products as they are, nothing is widened.
 //
-// A CTA takes one request, one kv head (up to 16 query heads of its group) and one partition of the keys, and walks over it in
-// tiles of 128 keys.  The products are transposed, so that the keys (then the elements of the head) are the 128 rows of the tensor
+// The work is all requests' tiles of 128 keys, times their kv heads (16 query heads of a group at most), one behind the other; every
+// CTA takes the same number of tiles of that row, so that requests of any lengths load all SMs alike (a CTA for each request and
+// kv head left the SMs idle for 29% of the time with 64 contexts of 1,024 to 2,048 keys).  A stretch of one request and kv head that
+// lies within a CTA is finished there; the parts of one that is cut are joined by a second kernel.  What is cut where
+// follows from the positions alone, on the device: a captured launch fits contexts that have grown.
+// The products are transposed, so that the keys (then the elements of the head) are the 128 rows of the tensor
 // cores and the query heads the 16 columns:
 //
 //   S^T = K Q^T    kind::f8f6f4, A = the key tile as the cache holds it (a key is a row of 128 bytes), B = the queries in two parts:
@@ -17,10 +21,13 @@
 // stay below 448 and those of quiet ones are no smaller than their share of the result; the denominator sums exp2(s - m) in 32
 // bits.  Both references rise only when a tile's maximum exceeds them by 2^8.
 //
-// Four warps of softmax (a thread is a key, then an element of the head), a loader (TMA, one box for each page, or one for the tile
-// where its pages lie one behind the other), an issuer.  Two stages of keys and values, 72 KB a CTA, three CTAs an SM.  A hidden key's
-// score becomes -inf by selection, and its row of values is zeroed in shared memory (0 times what lies behind a context could
-// be NaN).  The kernel is bound by the cache's bytes.
+// Roles: four warps of softmax (a thread is a key of the tile, then an element of the head); a scout, which reads block table, scales
+// and queries ahead of everyone and leaves them in shared memory (read where they are used, those dependent loads cost every
+// tile 2,000 to 3,400 of its 4,000 cycles); a loader each for keys and values (TMA, one box for each page, or one for the tile
+// where its pages lie one behind the other); an issuer.  Two score accumulators and two weight buffers: the scores of the next tile
+// are formed while the softmax works on this one, across the borders of requests and heads too.  Three stages of keys and
+// values, two CTAs an SM.  A hidden key's score becomes -inf by selection, and its row of values is zeroed in shared memory (0
+// times what lies behind a context could be NaN).  The kernel is bound by the cache's bytes.
 #include <algorithm>
 #include "eight_bit_tc.cuh"
 
@@ -30,18 +37,32 @@ typedef __nv_bfloat16 bf16;
 
 namespace {
 
-constexpr int kKeys = 128, kDim = 128, kHeads = 16, kStages = 2;
+constexpr int kKeys = 128, kDim = 128, kHeads = 16;
 constexpr int kTile = kKeys * kDim;                    // bytes of a tile of keys or of values
-constexpr int kPart = kHeads * 128;                    // bytes of 16 rows of one part of Q or P
-constexpr int kOffK = 0, kOffV = kStages * kTile, kOffQ = 2 * kStages * kTile, kOffP = kOffQ + 2 * kPart;
-constexpr int kSmemBytes = kOffP + 2 * kPart + 1024;
-constexpr int kSoftmaxThreads = 128, kThreads = kSoftmaxThreads + 64;
-constexpr uint32_t kTmemColumns = 32;                  // S^T at 0, O^T at 16
+constexpr int kSoftmaxThreads = 128, kThreads = kSoftmaxThreads + 4 * 32;
+constexpr int kKeyLoader = 4, kValueLoader = 5, kIssuer = 6, kScout = 7;      // warps
+constexpr uint32_t kTmemColumns = 64;                  // S^T of even and odd tiles at 0 and 16, O^T at 32
 constexpr float kRises = 8.0f, kHeadroom = 4.0f;       // log2: a reference rises when it is exceeded by kRises; M to kHeadroom below the maximum
-static_assert(kSmemBytes >= kLeastSharedBeside, "never beside a kernel that takes all tensor memory");
+constexpr int kChunk = 4, kSlots = 16;                 // tiles that the scout looks up together, pages of a tile at most
+constexpr int kHeldRows = 512;                         // positions that a CTA keeps in shared memory
 
-enum { K_FULL = 0, K_FREE = K_FULL + kStages, V_FULL = K_FREE + kStages, V_FREE = V_FULL + kStages, S_FULL = V_FREE + kStages, P_READY,
-       Q_READY, O_DONE, BARRIERS };
+// Shared memory for G heads.  A part (hi or lo) of Q or P is 16 rows of 128 bytes, the columns of the products; up to 8 heads need only
+// 8 of them, and the product then reads the next part's (or what follows) as the other columns, which nobody looks at.
+template <int G> struct Layout {
+  static constexpr int kStages = G <= 8 ? 3 : 2;
+  static constexpr int kPart = (G <= 8 ? 8 : 16) * 128;
+  static constexpr int kOffK = 0, kOffV = kStages * kTile, kOffQ = 2 * kStages * kTile, kOffP = kOffQ + 4 * kPart;
+  static constexpr int kSmemBytes = kOffP + 4 * kPart + 1024 /* what the last part's product reads */ + 1024 /* alignment */;
+};
+static_assert(Layout<16>::kSmemBytes >= kLeastSharedBeside, "never beside a kernel that takes all tensor memory");
+
+enum { K_FULL = 0, K_FREE = K_FULL + 3, V_FULL = K_FREE + 3, V_FREE = V_FULL + 3, S_FULL = V_FREE + 3, P_READY = S_FULL + 2,
+       Q_READY = P_READY + 2, Q_FREE = Q_READY + 4, CHUNK_FULL = Q_FREE + 2, CHUNK_FREE = CHUNK_FULL + 2, PV_DONE = CHUNK_FREE + 2,
+       BARRIERS = PV_DONE + 2 };
+// Tiles are counted over the CTA's whole stretch (g): stage g % kStages of the rings, g & 1 of S_FULL, P_READY and PV_DONE (who waits for
+// tile g of one of them knows that tile g - 2 is over, so the parity says which), chunk g / kChunk.
+// Parts are counted too (n): the queries' buffers and Q_FREE go by n & 1, Q_READY by n & 3: the softmax may begin part n when the
+// queries of part n + 2 are there already, but never those of part n + 4 (see `factors`).
 
 __device__ int g_error = 0;
 
@@ -88,323 +109,559 @@ __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& 
   lo = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a - taken.x, b - taken.y), __NV_SATFINITE, __NV_E5M2);
 }
 
-// G: heads that the softmax threads handle (the CTA's heads rounded up to 4, 8 or 16).
+// A row's share of the work: its tiles of keys, from the tile that holds its first visible key.
+struct Row {
+  int position, first_key, begin, tiles;
+};
+__device__ __forceinline__ Row row_at(const int* __restrict__ positions, int row, int window) {
+  Row r;
+  r.position = positions[row];
+  r.first_key = (window > 0 && r.position >= window) ? r.position + 1 - window : 0;
+  r.begin = r.first_key / kKeys * kKeys;
+  r.tiles = r.position >= 0 ? (int)(((long long)r.position + kKeys - r.begin) / kKeys) : 0;     // (a padding row: none)
+  return r;
+}
+
+// Where a CTA's stretch begins, and how long it is.  Stretches are `each` tiles; tile index = units * (tiles of the rows before) +
+// unit * (the row's tiles) + tile.
+struct Stretch {
+  int row, unit, tile;
+  long long count;
+};
+
+// One part of a stretch: tiles [first, last) of a row and unit.
+struct Part {
+  int row, unit, first, last;
+  Row of;
+  __device__ __forceinline__ bool whole() const { return first == 0 && last == of.tiles; }
+};
+
+// The parts of a stretch, one after the other.
+struct Walk {
+  Stretch at;
+  const int* positions;
+  int num_rows, units, window;
+  __device__ __forceinline__ bool next(Part& part) {
+    if (at.count <= 0) return false;
+    Row r = row_at(positions, at.row, window);
+    while (at.tile >= r.tiles) {                         // the row's next unit, or the next row that has tiles
+      at.tile = 0;
+      if (r.tiles == 0 || ++at.unit >= units) {
+        at.unit = 0;
+        if (++at.row >= num_rows) return false;
+        r = row_at(positions, at.row, window);
+      }
+    }
+    part.row = at.row;
+    part.unit = at.unit;
+    part.first = at.tile;
+    part.last = (int)min((long long)r.tiles, at.tile + at.count);
+    part.of = r;
+    at.count -= part.last - part.first;
+    at.tile = part.last;
+    return true;
+  }
+};
+
+// What the scout leaves of a chunk of tiles.
+struct Chunk {
+  int row[kChunk][kSlots];                             // a page's first row of the cache; below 0 where it is not there or not wanted
+  float2 scale[kChunk][kSlots];                        // its scales, of keys and of values
+  int column[kChunk], first[kChunk], last[kChunk];     // the kv head's bytes within a row; whether the tile is its part's first, its last
+};
+
+// G: heads that the softmax threads handle (a unit's heads rounded up to 4, 8 or 16).
 template <int G>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                    const __grid_constant__ CUtensorMap k_tile_map, const __grid_constant__ CUtensorMap v_tile_map,
                    const bf16* __restrict__ q, long long q_stride, Cache8 cache, const int* __restrict__ block_table, int table_width,
-                   const int* __restrict__ positions, int heads, float scale_log2, int window, int partition, int num_partitions,
-                   int part_slow, float* __restrict__ partial_o, float* __restrict__ partial_ml, bf16* __restrict__ out,
-                   const float* __restrict__ sinks) {
+                   const int* __restrict__ all_positions, int num_rows, int heads, float scale_log2, int window,
+                   float* __restrict__ parts, bf16* __restrict__ out, const float* __restrict__ sinks) {
+  using L = Layout<G>;
+  constexpr int kStages = L::kStages, kPart = L::kPart;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long barriers[BARRIERS];
   __shared__ uint32_t tmem_slot;
-  __shared__ float exchange[2][4][2 * G];              // [tile parity][warp]: the warps' maxima of s, then of s + f
+  __shared__ Stretch stretch;
+  __shared__ Chunk chunks[2];
+  __shared__ int held_positions[kHeldRows];
+  __shared__ __align__(16) float exchange[2][2 * G][4];        // [tile parity][maxima of s, then of s + f][warp]
   __shared__ float sums[4][G];
-  __shared__ float factors[G];                         // of a head's scores: scale, log2 e, and the power of two taken out of its queries
+  // Of a head's scores: scale, log2 e, and the power of two taken out of its queries, by n & 3: part n + 4's are written when the scores
+  // of part n + 2 are over, which were formed when the softmax was past every tile but the last two, so past part n.
+  __shared__ float factors[4][G];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
   auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
-  if (threadIdx.x == kSoftmaxThreads) {
-    for (int i = 0; i < BARRIERS; ++i) barrier_init(bar(i), (i == P_READY || i == Q_READY) ? (uint32_t)kSoftmaxThreads : 1u);
+  const int group = heads / cache.kv_heads, group_tiles = (group + kHeads - 1) / kHeads, units = cache.kv_heads * group_tiles;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < BARRIERS; ++i) {
+      const bool softmax = i == P_READY || i == P_READY + 1, chunk = i == CHUNK_FREE || i == CHUNK_FREE + 1;
+      barrier_init(bar(i), softmax ? (uint32_t)kSoftmaxThreads : (chunk ? 7u : 1u));      // (a chunk: both loaders, issuer, four warps)
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 5) {
+  if (warp == kIssuer) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemColumns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // the rows of Q and P that no head has stay zeros
-  for (int i = threadIdx.x; i < 4 * kPart / 16; i += kThreads) *reinterpret_cast<uint4*>(smem + kOffQ + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  grid_dependency_wait();                              // the cache, the queries and the positions may come from the kernel in front
+  for (int r = threadIdx.x; r < min(num_rows, kHeldRows); r += kThreads) held_positions[r] = all_positions[r];
+  __syncthreads();
+  const int* positions = num_rows <= kHeldRows ? held_positions : all_positions;
+  if (warp == 0) {
+    // this CTA's stretch: all tiles over the CTAs, then the row that the first one lies in
+    long long total = 0;
+    for (int r = lane; r < num_rows; r += 32) total += row_at(positions, r, window).tiles;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total *= units;
+    const long long each = (total + gridDim.x - 1) / gridDim.x, first = each * blockIdx.x;
+    Stretch mine;
+    mine.row = mine.unit = mine.tile = 0;
+    mine.count = min(each, total - first);
+    long long before = 0;
+    for (int r0 = 0; r0 < num_rows && mine.count > 0; r0 += 32) {
+      const int tiles = r0 + lane < num_rows ? row_at(positions, r0 + lane, window).tiles : 0;
+      long long through = (long long)tiles * units;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long left = __shfl_up_sync(0xffffffffu, through, o);
+        if (lane >= o) through += left;
+      }
+      through += before;
+      const unsigned beyond = __ballot_sync(0xffffffffu, through > first);
+      if (beyond != 0u) {
+        const int in = __ffs(beyond) - 1;
+        const int row_tiles = __shfl_sync(0xffffffffu, tiles, in);
+        const long long inside = first - (__shfl_sync(0xffffffffu, through, in) - (long long)row_tiles * units);
+        mine.row = r0 + in;
+        mine.unit = (int)(inside / row_tiles);
+        mine.tile = (int)(inside % row_tiles);
+        break;
+      }
+      before = __shfl_sync(0xffffffffu, through, 31);
+    }
+    if (lane == 0) {
+      if (*reinterpret_cast<volatile int*>(&g_error) != 0) mine.count = 0;       // an earlier wait ran out: nothing is begun
+      stretch = mine;
+    }
+  }
   tensor_fence_before_sync();
   __syncthreads();
   tensor_fence_after_sync();
-  const uint32_t tmem_s = tmem_slot, tmem_o = tmem_slot + 16u;
-  grid_dependency_wait();                              // the cache, the queries and the positions may come from the kernel in front
   grid_launch_dependents();
-
-  const int part = part_slow ? blockIdx.z : blockIdx.x, row = part_slow ? blockIdx.x : blockIdx.z;
-  const int group = heads / cache.kv_heads, group_tiles = (group + kHeads - 1) / kHeads;
-  const int kv_head = blockIdx.y / group_tiles;
-  const int head0 = kv_head * group + (blockIdx.y % group_tiles) * kHeads;
-  const int valid_heads = min(kHeads, kv_head * group + group - head0);
-  const int position = positions[row];
-  const int first_key = (window > 0 && position >= window) ? position + 1 - window : 0;
-  const int part_end = (int)min((long long)position + 1, (long long)(part + 1) * partition);
-  const int begin = max(part * partition, first_key / kKeys * kKeys);
-  const int tiles = position >= 0 && begin < part_end ? (part_end - begin + kKeys - 1) / kKeys : 0;
-  const bool go = *reinterpret_cast<volatile int*>(&g_error) == 0;
-  const int* table = block_table + (size_t)row * table_width;
+  const uint32_t tmem_s = tmem_slot, tmem_o = tmem_slot + 32u;
   const int shift = 31 - __clz(cache.page_size);       // pages are powers of two
-  if (tiles == 0 || !go) {
-    // a padding row, or a partition without keys: the merge reads a denominator of 0; without a merge the row is zeros
-    if (position >= 0 && threadIdx.x < kDim) {
-      for (int g = 0; g < valid_heads; ++g) {
-        const size_t head = (size_t)row * heads + head0 + g;
-        if (num_partitions == 1) out[head * kDim + threadIdx.x] = __float2bfloat16_rn(0.0f);
-        else if (threadIdx.x == 0) {
-          partial_ml[(head * num_partitions + part) * 2] = -INFINITY;
-          partial_ml[(head * num_partitions + part) * 2 + 1] = 0.0f;
+  const int count = (int)max(0ll, stretch.count);      // tiles of this CTA
+  Walk walk{stretch, positions, num_rows, units, window};
+  Part part;
+
+  if (warp == kScout) {
+    // ------------------------------------------------------------------ scout
+    const int pages_per_tile = kKeys >> shift, page_size = cache.page_size;
+    bool alive = true;
+    int tile = 0, parts_begun = 0;                     // the walk's next tile of `part`
+    part.last = 0;
+    for (int g0 = 0; g0 < count; g0 += kChunk) {
+      const int buffer = g0 / kChunk & 1, tiles = min(kChunk, count - g0);
+      if (alive && !wait_barrier(bar(CHUNK_FREE + buffer), (uint32_t)(g0 / kChunk >> 1 & 1) ^ 1u)) { g_error = 1; alive = false; }
+      __syncwarp();
+      Chunk& chunk = chunks[buffer];
+      Part begun[kChunk];                              // the parts that begin in this chunk
+      int beginning = 0;
+      // what this lane's two entries (tile, page slot) of the chunk are
+      const int* table[2] = {block_table, block_table};
+      int block[2] = {-1, -1}, head_of[2] = {0, 0};
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        if (j < tiles) {
+          if (tile >= part.last) {
+            walk.next(part);
+            tile = part.first;
+          }
+          if (tile == part.first) begun[j] = part;     // (an index known at compile time: registers)
+          if (lane == 0) {
+            chunk.column[j] = part.unit / group_tiles * kDim;
+            chunk.first[j] = tile == part.first;
+            chunk.last[j] = tile == part.last - 1;
+          }
+          beginning |= (tile == part.first ? 1 : 0) << j;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int entry = lane + 32 * i;
+            if (entry / pages_per_tile == j) {
+              const int key = part.of.begin + tile * kKeys + entry % pages_per_tile * page_size;
+              table[i] = block_table + (size_t)part.row * table_width;
+              head_of[i] = part.unit / group_tiles;
+              block[i] = key <= part.of.position && key + page_size > part.of.first_key && (key >> shift) < table_width ? key >> shift : -1;
+            }
+          }
+          ++tile;
         }
       }
+      int page[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) page[i] = block[i] >= 0 ? table[i][block[i]] : -1;
+      float2 scale[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (page[i] >= cache.pages) page[i] = -1;
+        const size_t at = (size_t)max(page[i], 0) * cache.kv_heads + head_of[i];
+        scale[i] = page[i] >= 0 ? make_float2(cache.k_scales[at], cache.v_scales[at]) : make_float2(1.0f, 1.0f);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int entry = lane + 32 * i;
+        if (entry < kChunk * pages_per_tile) {
+          chunk.row[entry / pages_per_tile][entry % pages_per_tile] = page[i] >= 0 ? page[i] << shift : -page_size;
+          chunk.scale[entry / pages_per_tile][entry % pages_per_tile] = scale[i];
+        }
+      }
+      __syncwarp();
+      if (lane == 0) barrier_arrive(bar(CHUNK_FULL + buffer));
+      // the queries of the parts that begin here, in their two parts, as operands: a lane has four elements of a head
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        if ((beginning >> j & 1) == 0) continue;
+        const int parity = parts_begun & 1;
+        if (alive && !wait_barrier(bar(Q_FREE + parity), (uint32_t)(parts_begun >> 1 & 1) ^ 1u)) { g_error = 1; alive = false; }
+        __syncwarp();
+        const int kv_head = begun[j].unit / group_tiles, head0 = kv_head * group + begun[j].unit % group_tiles * kHeads;
+        const int valid_heads = min(kHeads, kv_head * group + group - head0);
+        const bf16* from = q + (size_t)begun[j].row * q_stride + (size_t)head0 * kDim + lane * 4;
+        uint2 raw[G];
+#pragma unroll
+        for (int h = 0; h < G; ++h) raw[h] = *reinterpret_cast<const uint2*>(from + min(h, valid_heads - 1) * kDim);
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          float x[4] = {__uint_as_float(raw[h].x << 16), __uint_as_float(raw[h].x & 0xffff0000u), __uint_as_float(raw[h].y << 16),
+                        __uint_as_float(raw[h].y & 0xffff0000u)};
+          const float largest = warp_largest(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+          const int e = least_scale_exponent(fminf(largest, 3.38953139e38f));
+          const float inverse = power_of_two(-e);
+          uint32_t hi[2], lo[2];
+          split(x[0] * inverse, x[1] * inverse, hi[0], lo[0]);
+          split(x[2] * inverse, x[3] * inverse, hi[1], lo[1]);
+          unsigned char* to = smem + L::kOffQ + parity * 2 * kPart + swizzled(h, lane * 4);
+          *reinterpret_cast<uint32_t*>(to) = hi[0] | (hi[1] << 16);
+          *reinterpret_cast<uint32_t*>(to + kPart) = lo[0] | (lo[1] << 16);
+          if (lane == 0) factors[parts_begun & 3][h] = power_of_two(e) * scale_log2;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) barrier_arrive(bar(Q_READY + (parts_begun & 3)));
+        ++parts_begun;
+      }
     }
-  } else if (warp == 4) {
-    // ------------------------------------------------------------------ loader: lane l has page slot l of the tile
-    const int pages_per_tile = kKeys >> shift, page_size = cache.page_size;
-    const uint32_t box_bytes = (uint32_t)page_size * kDim;
-    const bool loads = lane < pages_per_tile;
-    auto row_of = [&](int t) {
-      const int key = begin + t * kKeys + lane * page_size;
-      int page = -1;
-      if (loads && t < tiles && key < part_end && key + page_size > first_key) page = page_of_block(table, table_width, key >> shift, cache.pages);
-      return page >= 0 ? page << shift : -page_size;   // a negative row lies outside the tensor: zeros
-    };
-    int cache_row = row_of(0);
+  } else if (warp == kKeyLoader || warp == kValueLoader) {
+    // ------------------------------------------------------------------ loaders: lane l has page slot l of the tile
+    const bool values = warp == kValueLoader;
+    const uint32_t box_bytes = (uint32_t)cache.page_size * kDim;
+    const bool loads = lane < (kKeys >> shift);
+    const uint32_t full0 = bar(values ? V_FULL : K_FULL), free0 = bar(values ? V_FREE : K_FREE);
+    const uint32_t base = smem_base + (uint32_t)(values ? L::kOffV : L::kOffK);
     bool alive = true;
-    for (int t = 0; t < tiles && alive; ++t) {
-      const uint32_t stage = (uint32_t)t % kStages, parity = (uint32_t)(t / kStages) & 1u;
-      const int next_row = row_of(t + 1);              // on its way while this tile's stage is awaited
+    uint32_t stage = 0, parity = 0;
+    for (int g = 0; g < count; ++g) {
+      const int buffer = g / kChunk & 1;
+      if (g % kChunk == 0 && alive && !wait_barrier(bar(CHUNK_FULL + buffer), (uint32_t)(g / kChunk >> 1 & 1))) { g_error = 1; alive = false; }
+      alive = __all_sync(0xffffffffu, alive);
+      const int cache_row = loads ? chunks[buffer].row[g % kChunk][lane] : 0, column = chunks[buffer].column[g % kChunk];
+      __syncwarp();
+      if (g % kChunk == kChunk - 1 && lane == 0) barrier_arrive(bar(CHUNK_FREE + buffer));
+      if (alive && !wait_barrier(free0 + 8u * stage, parity ^ 1u)) { g_error = 1; alive = false; }
+      alive = __all_sync(0xffffffffu, alive);
+      if (!alive) break;
+      // Where the tile's pages lie one behind the other in the pool one box takes them all (a copy instruction costs the warp about 75
+      // cycles for every lane that takes part).
       const int first_row = __shfl_sync(0xffffffffu, cache_row, 0);
       const bool in_a_row = first_row >= 0 && __all_sync(0xffffffffu, !loads || cache_row == first_row + (lane << shift));
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const uint32_t full = bar((which ? V_FULL : K_FULL) + (int)stage);
-        if (!wait_barrier(bar((which ? V_FREE : K_FREE) + (int)stage), parity ^ 1u)) { g_error = 1; alive = false; }
-        alive = __all_sync(0xffffffffu, alive);
-        if (!alive) break;
-        const uint32_t to = smem_base + (uint32_t)(which ? kOffV : kOffK) + stage * (uint32_t)kTile;
-        if (lane == 0) barrier_expect_bytes(full, (uint32_t)kTile);
-        __syncwarp();
-        if (in_a_row) {
-          if (lane == 0) tma_load_2d(to, which ? &v_tile_map : &k_tile_map, full, kv_head * kDim, first_row);
-        } else if (loads) {
-          tma_load_2d(to + (uint32_t)lane * box_bytes, which ? &v_map : &k_map, full, kv_head * kDim, cache_row);
-        }
+      const uint32_t full = full0 + 8u * stage, to = base + stage * (uint32_t)kTile;
+      if (lane == 0) barrier_expect_bytes(full, (uint32_t)kTile);
+      __syncwarp();
+      if (in_a_row) {
+        if (lane == 0) tma_load_2d(to, values ? &v_tile_map : &k_tile_map, full, column, first_row);
+      } else if (loads) {                              // (a negative row lies outside the tensor: zeros)
+        tma_load_2d(to + (uint32_t)lane * box_bytes, values ? &v_map : &k_map, full, column, cache_row);
       }
-      cache_row = next_row;
+      if (++stage == (uint32_t)kStages) { stage = 0; parity ^= 1u; }
     }
-  } else if (warp == 5) {
+  } else if (warp == kIssuer) {
     // ------------------------------------------------------------------ issuer (tcgen05.cuh: from a whole warp)
     constexpr uint32_t scores_hi = instruction_descriptor_8bit(kKeys, kHeads, E4M3, E4M3);
     constexpr uint32_t scores_lo = instruction_descriptor_8bit(kKeys, kHeads, E4M3, E5M2);
     constexpr uint32_t values_hi = instruction_descriptor_8bit(kDim, kHeads, E4M3, E4M3, true);
     constexpr uint32_t values_lo = instruction_descriptor_8bit(kDim, kHeads, E4M3, E5M2, true);
     const uint32_t elected = elect_one();
-    const uint32_t k_low = operand_low(smem_base + kOffK), q_low = operand_low(smem_base + kOffQ);
-    const uint32_t v_low = operand_low_mn_major(smem_base + kOffV, kTile), p_low = operand_low(smem_base + kOffP);
+    const uint32_t k_low = operand_low(smem_base + L::kOffK), q_low = operand_low(smem_base + L::kOffQ);
+    const uint32_t v_low = operand_low_mn_major(smem_base + L::kOffV, kTile), p_low = operand_low(smem_base + L::kOffP);
     constexpr uint32_t kPartStep = kPart >> 4, kTileStep = kTile >> 4;
     bool alive = true;
     auto check = [&](int index, uint32_t parity) {
       if (alive && !wait_barrier(bar(index), parity)) { g_error = 2; alive = false; }
     };
-    auto issue_scores = [&](int t) {
-      const uint32_t stage = (uint32_t)t % kStages;
-      check(K_FULL + (int)stage, (uint32_t)(t / kStages) & 1u);
+    uint32_t k_stage = 0, k_parity = 0, v_stage = 0, v_parity = 0, first_tiles = 0;
+    int n = 0;                                         // parts whose scores are under way
+    auto issue_scores = [&](int g) {
+      const int buffer = g / kChunk & 1;
+      if (g % kChunk == 0) check(CHUNK_FULL + buffer, (uint32_t)(g / kChunk >> 1 & 1));
+      __syncwarp();
+      const bool first = __shfl_sync(0xffffffffu, chunks[buffer].first[g % kChunk], 0) != 0;
+      const bool last = __shfl_sync(0xffffffffu, chunks[buffer].last[g % kChunk], 0) != 0;
+      __syncwarp();
+      if (g % kChunk == kChunk - 1 && lane == 0) barrier_arrive(bar(CHUNK_FREE + buffer));
+      if (first) check(Q_READY + (n & 3), (uint32_t)(n >> 2 & 1));
+      check(K_FULL + (int)k_stage, k_parity);
+      __syncwarp();
       tensor_fence_after_sync();
-      const uint32_t a = k_low + stage * kTileStep;
+      const uint32_t a = k_low + k_stage * kTileStep, b = q_low + (uint32_t)(n & 1) * 2u * kPartStep, d = tmem_s + (uint32_t)(g & 1) * 16u;
 #pragma unroll
-      for (int kk = 0; kk < kDim / 32; ++kk) mma_8bit_ss_halves(tmem_s, a + 2u * kk, q_low + 2u * kk, scores_hi, kk > 0 ? 1u : 0u, elected);
+      for (int kk = 0; kk < kDim / 32; ++kk) mma_8bit_ss_halves(d, a + 2u * kk, b + 2u * kk, scores_hi, kk > 0 ? 1u : 0u, elected);
 #pragma unroll
-      for (int kk = 0; kk < kDim / 32; ++kk) mma_8bit_ss_halves(tmem_s, a + 2u * kk, q_low + kPartStep + 2u * kk, scores_lo, 1u, elected);
-      mma_commit_elected(bar(S_FULL), elected);
-      mma_commit_elected(bar(K_FREE + (int)stage), elected);
+      for (int kk = 0; kk < kDim / 32; ++kk) mma_8bit_ss_halves(d, a + 2u * kk, b + kPartStep + 2u * kk, scores_lo, 1u, elected);
+      mma_commit_elected(bar(S_FULL + (g & 1)), elected);
+      mma_commit_elected(bar(K_FREE + (int)k_stage), elected);
+      if (last) {
+        mma_commit_elected(bar(Q_FREE + (n & 1)), elected);
+        ++n;
+      }
+      first_tiles = (first_tiles & ~(1u << (g & 3))) | ((first ? 1u : 0u) << (g & 3));
+      if (++k_stage == (uint32_t)kStages) { k_stage = 0; k_parity ^= 1u; }
     };
-    check(Q_READY, 0u);
-    issue_scores(0);
-    for (int t = 0; t < tiles; ++t) {
-      const uint32_t stage = (uint32_t)t % kStages;
-      check(V_FULL + (int)stage, (uint32_t)(t / kStages) & 1u);
-      check(P_READY, (uint32_t)t & 1u);
+    for (int g = 0; g < min(count, 2); ++g) issue_scores(g);
+    for (int g = 0; g < count; ++g) {
+      check(V_FULL + (int)v_stage, v_parity);
+      check(P_READY + (g & 1), (uint32_t)(g >> 1 & 1));
+      __syncwarp();
       tensor_fence_after_sync();
-      const uint32_t a = v_low + stage * kTileStep;
+      const uint32_t a = v_low + v_stage * kTileStep, b = p_low + (uint32_t)(g & 1) * 2u * kPartStep;
+      const uint32_t begins = first_tiles >> (g & 3) & 1u;
       // 32 keys are 32 rows of 128 bytes further down the values, 32 bytes further along the weights
 #pragma unroll
       for (int kk = 0; kk < kKeys / 32; ++kk)
-        mma_8bit_ss_halves(tmem_o, a + (uint32_t)kk * (4096u >> 4), p_low + 2u * kk, values_hi, t > 0 || kk > 0 ? 1u : 0u, elected);
+        mma_8bit_ss_halves(tmem_o, a + (uint32_t)kk * (4096u >> 4), b + 2u * kk, values_hi, kk > 0 ? 1u : begins ^ 1u, elected);
 #pragma unroll
       for (int kk = 0; kk < kKeys / 32; ++kk)
-        mma_8bit_ss_halves(tmem_o, a + (uint32_t)kk * (4096u >> 4), p_low + kPartStep + 2u * kk, values_lo, 1u, elected);
-      mma_commit_elected(bar(V_FREE + (int)stage), elected);
-      // the next scores are issued behind this product, so that their barrier also says that O^T may be rescaled
-      if (t + 1 < tiles) issue_scores(t + 1);
-      else mma_commit_elected(bar(O_DONE), elected);
+        mma_8bit_ss_halves(tmem_o, a + (uint32_t)kk * (4096u >> 4), b + kPartStep + 2u * kk, values_lo, 1u, elected);
+      mma_commit_elected(bar(V_FREE + (int)v_stage), elected);
+      mma_commit_elected(bar(PV_DONE + (g & 1)), elected);
+      if (++v_stage == (uint32_t)kStages) { v_stage = 0; v_parity ^= 1u; }
+      // The scores of the tile after next take the accumulator that the softmax has read (P_READY says so); issued behind this
+      // product, their barrier also says that the weights' buffer is free.
+      if (g + 2 < count) issue_scores(g + 2);
     }
   } else {
     // ------------------------------------------------------------------ softmax: thread = key of the tile, then element
-    const int r = threadIdx.x;
+    const int r = threadIdx.x, slot = r >> shift;
     const uint32_t lane_bits = (uint32_t)(warp * 32) << 16;
     bool alive = true;
-    // the group's queries in their two parts: a warp takes a head at a time, a lane four elements
-    for (int h = warp; h < valid_heads; h += 4) {
-      const uint2 raw = *reinterpret_cast<const uint2*>(q + (size_t)row * q_stride + (size_t)(head0 + h) * kDim + lane * 4);
-      float x[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
-                    __uint_as_float(raw.y & 0xffff0000u)};
-      const float largest = warp_largest(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-      const int e = least_scale_exponent(fminf(largest, 3.38953139e38f));
-      const float inverse = power_of_two(-e);
-      uint32_t hi[2], lo[2];
-      split(x[0] * inverse, x[1] * inverse, hi[0], lo[0]);
-      split(x[2] * inverse, x[3] * inverse, hi[1], lo[1]);
-      unsigned char* to = smem + kOffQ + swizzled(h, lane * 4);
-      *reinterpret_cast<uint32_t*>(to) = hi[0] | (hi[1] << 16);
-      *reinterpret_cast<uint32_t*>(to + kPart) = lo[0] | (lo[1] << 16);
-      if (lane == 0 && h < G) factors[h] = power_of_two(e) * scale_log2;
-    }
-    if (r < G && r >= valid_heads) factors[r] = 0.0f;
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    barrier_arrive(bar(Q_READY));
-    asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");
-    float factor_of[G], top[G], top_weight[G], denominator[G];
+    uint32_t stage = 0, stage_parity = 0;
+    int g = 0;
+    for (int n = 0; walk.next(part); ++n) {
+      const Row& of = part.of;
+      const int kv_head = part.unit / group_tiles;
+      const int head0 = kv_head * group + part.unit % group_tiles * kHeads;
+      const int valid_heads = min(kHeads, kv_head * group + group - head0);
+      float top[G], top_weight[G], denominator[G];
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      factor_of[g] = factors[g];
-      top[g] = top_weight[g] = -INFINITY;
-      denominator[g] = 0.0f;
-    }
-    unsigned char* p_smem = smem + kOffP;
-    // a key's page two tiles ahead of its use, its page's scales one
-    auto page_at = [&](int t) {
-      const int key = begin + t * kKeys + r;
-      return t < tiles && key <= position && key >= first_key ? page_of_block(table, table_width, key >> shift, cache.pages) : -1;
-    };
-    auto scale_at = [&](const float* scales, int page) { return page >= 0 ? scales[(size_t)page * cache.kv_heads + kv_head] : 1.0f; };
-    int page = page_at(0), page_next = page_at(1);
-    float k_scale = scale_at(cache.k_scales, page), v_scale = scale_at(cache.v_scales, page);
-    for (int t = 0; t < tiles; ++t) {
-      const uint32_t stage = (uint32_t)t % kStages;
-      const int page_after = page_at(t + 2);
-      const float k_next = scale_at(cache.k_scales, page_next), v_next = scale_at(cache.v_scales, page_next);
-      const bool visible = page >= 0 && begin + t * kKeys + r < part_end;
-      const float shift_v = (float)(((__float_as_int(v_scale) >> 23) & 0xff) - 127);      // the exponent of a power of two
-      if (!visible) {
-        // what the product with this key's weight of 0 reads is zeros, not whatever lies there
-        if (alive && !wait_barrier(bar(V_FULL + (int)stage), (uint32_t)(t / kStages) & 1u)) { g_error = 3; alive = false; }
-        uint4* mine = reinterpret_cast<uint4*>(smem + kOffV + stage * kTile + r * kDim);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mine[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int h = 0; h < G; ++h) {
+        top[h] = top_weight[h] = -INFINITY;
+        denominator[h] = 0.0f;
       }
-      __syncwarp();
-      if (alive && !wait_barrier(bar(S_FULL), (uint32_t)t & 1u)) { g_error = 3; alive = false; }
-      __syncwarp();
-      tensor_fence_after_sync();
-      float s[G];
-      tmem_load<G>(tmem_s + lane_bits, s);
-      float* mine = &exchange[t & 1][warp][0];
+      const float* factor_of = factors[n & 3];
+      if (alive && !wait_barrier(bar(Q_READY + (n & 3)), (uint32_t)(n >> 2 & 1))) { g_error = 3; alive = false; }
+      for (int t = part.first; t < part.last; ++t, ++g) {
+        const int buffer = g / kChunk & 1, key = of.begin + t * kKeys + r;
+        if (g % kChunk == 0 && alive && !wait_barrier(bar(CHUNK_FULL + buffer), (uint32_t)(g / kChunk >> 1 & 1))) { g_error = 3; alive = false; }
+        const bool visible = chunks[buffer].row[g % kChunk][slot] >= 0 && key <= of.position && key >= of.first_key;
+        const float2 scale = chunks[buffer].scale[g % kChunk][slot];
+        __syncwarp();
+        if (g % kChunk == kChunk - 1 && lane == 0) barrier_arrive(bar(CHUNK_FREE + buffer));
+        const float shift_v = (float)(((__float_as_int(scale.y) >> 23) & 0xff) - 127);    // the exponent of a power of two
+        if (!visible) {
+          // what the product with this key's weight of 0 reads is zeros, not whatever lies there
+          if (alive && !wait_barrier(bar(V_FULL + (int)stage), stage_parity)) { g_error = 3; alive = false; }
+          uint4* mine = reinterpret_cast<uint4*>(smem + L::kOffV + stage * kTile + r * kDim);
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        s[g] = visible ? s[g] * (k_scale * factor_of[g]) : -INFINITY;
-        const float a = warp_largest(s[g]), b = warp_largest(s[g] + shift_v);
-        if (lane == 0) { mine[g] = a; mine[G + g] = b; }
+          for (int i = 0; i < 8; ++i) mine[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+        if (alive && !wait_barrier(bar(S_FULL + (g & 1)), (uint32_t)(g >> 1 & 1))) { g_error = 3; alive = false; }
+        __syncwarp();
+        tensor_fence_after_sync();
+        float s[G];
+        tmem_load<G>(tmem_s + (uint32_t)(g & 1) * 16u + lane_bits, s);
+        float(*seen)[4] = exchange[g & 1];
+        float mine = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          s[h] = visible ? s[h] * (scale.x * factor_of[h]) : -INFINITY;
+          const float a = warp_largest(s[h]), b = warp_largest(s[h] + shift_v);
+          mine = lane == h ? a : (lane == G + h ? b : mine);
+        }
+        if (lane < 2 * G) seen[lane][warp] = mine;
+        asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");
+        float rescale[G];
+        bool grow = false;
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          const float4 four = *reinterpret_cast<const float4*>(seen[h]), more = *reinterpret_cast<const float4*>(seen[G + h]);
+          const float a = fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)), b = fmaxf(fmaxf(more.x, more.y), fmaxf(more.z, more.w));
+          if (a > top[h] + kRises) {
+            denominator[h] *= approximate_exp2(top[h] - a);    // 0 when nothing was seen before
+            top[h] = a;
+          }
+          const bool rises = b > top_weight[h] + kRises;
+          rescale[h] = rises ? approximate_exp2(top_weight[h] - (b - kHeadroom)) : 1.0f;
+          top_weight[h] = rises ? b - kHeadroom : top_weight[h];
+          grow = grow || rises;
+        }
+        // O^T may be rescaled when the product with the last tile's weights is over: this thread's lane is an element of the head, its
+        // columns are the heads (all threads agree: the maxima are the same for all).
+        if (t > part.first && grow) {
+          if (alive && !wait_barrier(bar(PV_DONE + ((g - 1) & 1)), (uint32_t)(g - 1 >> 1 & 1))) { g_error = 3; alive = false; }
+          __syncwarp();
+          tensor_fence_after_sync();
+          float o[G];
+          tmem_load<G>(tmem_o + lane_bits, o);
+#pragma unroll
+          for (int h = 0; h < G; ++h) o[h] *= rescale[h];
+          tmem_store<G>(tmem_o + lane_bits, o);
+          tmem_store_wait();
+        }
+        unsigned char* p_smem = smem + L::kOffP + (g & 1) * 2 * kPart;
+#pragma unroll
+        for (int h = 0; h < G; h += 2) {
+          float w[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            denominator[h + i] += visible ? approximate_exp2(s[h + i] - top[h + i]) : 0.0f;
+            w[i] = visible ? approximate_exp2(s[h + i] + shift_v - top_weight[h + i]) : 0.0f;
+          }
+          uint32_t hi, lo;
+          split(w[0], w[1], hi, lo);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            unsigned char* to = p_smem + swizzled(h + i, r);
+            to[0] = (unsigned char)(hi >> (8 * i));
+            to[kPart] = (unsigned char)(lo >> (8 * i));
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tensor_fence_before_sync();
+        barrier_arrive(bar(P_READY + (g & 1)));
+        if (++stage == (uint32_t)kStages) { stage = 0; stage_parity ^= 1u; }
+      }
+#pragma unroll
+      for (int h = 0; h < G; ++h) {
+        const float total = warp_sum(denominator[h]);  // every thread holds its keys' share
+        if (lane == 0) sums[warp][h] = total;
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");
-      float rescale[G];
-      bool grow = false;
+      if (alive && !wait_barrier(bar(PV_DONE + ((g - 1) & 1)), (uint32_t)(g - 1 >> 1 & 1))) { g_error = 3; alive = false; }
+      __syncwarp();
+      tensor_fence_after_sync();
+      float o[G];
+      tmem_load<G>(tmem_o + lane_bits, o);
+      // (the next part's first product waits for its weights, which these threads write behind this)
+      if (alive) {
+        // a part that is not the whole: in its CTA's second place if it begins here, in the first if it goes on from the CTA before
+        const int heads_of_unit = min(group, kHeads);
+        float* to = parts + ((size_t)blockIdx.x * 2 + (part.first == 0 ? 1 : 0)) * heads_of_unit * (kDim + 2);
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const float a = fmaxf(fmaxf(exchange[t & 1][0][g], exchange[t & 1][1][g]), fmaxf(exchange[t & 1][2][g], exchange[t & 1][3][g]));
-        const float b = fmaxf(fmaxf(exchange[t & 1][0][G + g], exchange[t & 1][1][G + g]),
-                              fmaxf(exchange[t & 1][2][G + g], exchange[t & 1][3][G + g]));
-        if (a > top[g] + kRises) {
-          denominator[g] *= approximate_exp2(top[g] - a);      // 0 when nothing was seen before
-          top[g] = a;
-        }
-        const bool rises = b > top_weight[g] + kRises;
-        rescale[g] = rises ? approximate_exp2(top_weight[g] - (b - kHeadroom)) : 1.0f;
-        top_weight[g] = rises ? b - kHeadroom : top_weight[g];
-        grow = grow || rises;
-      }
-      // The product with the last tile's weights is over (these scores were issued behind it), so O^T may be rescaled: this thread's
-      // lane is an element of the head, its columns are the heads.
-      if (t > 0 && grow) {
-        float o[G];
-        tmem_load<G>(tmem_o + lane_bits, o);
-#pragma unroll
-        for (int g = 0; g < G; ++g) o[g] *= rescale[g];
-        tmem_store<G>(tmem_o + lane_bits, o);
-        tmem_store_wait();
-      }
-#pragma unroll
-      for (int g = 0; g < G; g += 2) {
-        float w[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          denominator[g + i] += visible ? approximate_exp2(s[g + i] - top[g + i]) : 0.0f;
-          w[i] = visible ? approximate_exp2(s[g + i] + shift_v - top_weight[g + i]) : 0.0f;
-        }
-        uint32_t hi, lo;
-        split(w[0], w[1], hi, lo);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          unsigned char* to = p_smem + swizzled(g + i, r);
-          to[0] = (unsigned char)(hi >> (8 * i));
-          to[kPart] = (unsigned char)(lo >> (8 * i));
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tensor_fence_before_sync();
-      barrier_arrive(bar(P_READY));
-      page = page_next;
-      page_next = page_after;
-      k_scale = k_next;
-      v_scale = v_next;
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float total = warp_sum(denominator[g]);    // every thread holds its keys' share
-      if (lane == 0) sums[warp][g] = total;
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");
-    if (alive && !wait_barrier(bar(O_DONE), 0u)) { g_error = 3; alive = false; }
-    __syncwarp();
-    tensor_fence_after_sync();
-    float o[G];
-    tmem_load<G>(tmem_o + lane_bits, o);
-    if (alive) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        if (g >= valid_heads) break;
-        float total = (sums[0][g] + sums[1][g]) + (sums[2][g] + sums[3][g]);
-        const size_t head = (size_t)row * heads + head0 + g;
-        // the products are relative to 2^top_weight, the sum to 2^top
-        const float value = total == 0.0f ? 0.0f : o[g] * exp2f(top_weight[g] - top[g]);    // (NaN stays NaN)
-        if (num_partitions == 1) {
-          if (total != 0.0f && sinks != nullptr) total += exp2f(sinks[head0 + g] * kLog2e - top[g]);
-          out[head * kDim + r] = __float2bfloat16_rn(total == 0.0f ? 0.0f : value / total);
-        } else {
-          partial_o[(head * num_partitions + part) * kDim + r] = value;
-          if (r == 0) {
-            partial_ml[(head * num_partitions + part) * 2] = top[g];
-            partial_ml[(head * num_partitions + part) * 2 + 1] = total;
+        for (int h = 0; h < G; ++h) {
+          if (h >= valid_heads) break;
+          float total = (sums[0][h] + sums[1][h]) + (sums[2][h] + sums[3][h]);
+          // the products are relative to 2^top_weight, the sum to 2^top
+          const float value = total == 0.0f ? 0.0f : o[h] * exp2f(top_weight[h] - top[h]);    // (NaN stays NaN)
+          if (part.whole()) {
+            if (total != 0.0f && sinks != nullptr) total += exp2f(sinks[head0 + h] * kLog2e - top[h]);
+            out[((size_t)part.row * heads + head0 + h) * kDim + r] = __float2bfloat16_rn(total == 0.0f ? 0.0f : value / total);
+          } else {
+            to[h * (kDim + 2) + r] = value;
+            if (r == 0) {
+              to[h * (kDim + 2) + kDim] = top[h];
+              to[h * (kDim + 2) + kDim + 1] = total;
+            }
           }
         }
       }
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");     // (the sums have been read)
     }
     tensor_fence_before_sync();
   }
   __syncthreads();
-  if (warp == 5) {
+  if (warp == kIssuer) {
     tensor_fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(kTmemColumns) : "memory");
   }
 }
 
+// Joins the parts of what was cut: a warp for each row and head.
+constexpr int kJoinWarps = 4;
+__global__ void __launch_bounds__(kJoinWarps * 32)
+join_8bit_kernel(const float* __restrict__ parts, const int* __restrict__ positions, int num_rows, int heads, int kv_heads, int window,
+                 int ctas, bf16* __restrict__ out, const float* __restrict__ sinks) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int row = blockIdx.y, head = blockIdx.x * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (head >= heads) return;
+  // all tiles, and those of the rows before this one
+  long long total = 0, before = 0;
+  for (int r = lane; r < num_rows; r += 32) {
+    const int tiles = row_at(positions, r, window).tiles;
+    total += tiles;
+    before += r < row ? tiles : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  const int group = heads / kv_heads, group_tiles = (group + kHeads - 1) / kHeads, units = kv_heads * group_tiles;
+  const int tiles = row_at(positions, row, window).tiles;
+  if (tiles == 0) return;
+  const long long each = (total * units + ctas - 1) / ctas;
+  const int heads_of_unit = min(group, kHeads);
+  const int in_group = head % group, unit = head / group * group_tiles + in_group / kHeads, h = in_group % kHeads;
+  const long long first = before * units + (long long)unit * tiles;
+  const int from = (int)(first / each), to = (int)((first + tiles - 1) / each);
+  if (from == to) return;                              // one CTA had all of it
+  auto place = [&](int cta) { return parts + (((size_t)cta * 2 + (cta == from ? 1 : 0)) * heads_of_unit + h) * (kDim + 2); };
+  float top = -INFINITY;
+  for (int c = from + lane; c <= to; c += 32) {
+    const float2 ml = *reinterpret_cast<const float2*>(place(c) + kDim);
+    if (ml.y != 0.0f) top = fmaxf(top, ml.x);
+  }
+  top = warp_max(top);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int c = from; c <= to; ++c) {
+    const float* p = place(c);
+    const float2 ml = *reinterpret_cast<const float2*>(p + kDim);
+    const float2 a = *reinterpret_cast<const float2*>(p + lane * 4), b = *reinterpret_cast<const float2*>(p + lane * 4 + 2);
+    const float factor = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top);            // 0: no visible key (its values are zeros)
+    sum += ml.y * factor;
+    o.x += a.x * factor; o.y += a.y * factor; o.z += b.x * factor; o.w += b.y * factor;
+  }
+  if (sum != 0.0f && sinks != nullptr) sum += exp2f(sinks[head] * kLog2e - top);
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  __nv_bfloat162 both[2] = {__floats2bfloat162_rn(o.x * inverse, o.y * inverse), __floats2bfloat162_rn(o.z * inverse, o.w * inverse)};
+  *reinterpret_cast<uint2*>(out + ((size_t)row * heads + head) * kDim + lane * 4) = *reinterpret_cast<const uint2*>(both);
+}
+
 template <int G>
 int launch(const Attention8& a, const CUtensorMap (&maps)[4]) {
-  const cudaError_t err = cudaFuncSetAttribute(decode_8bit_kernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (err != cudaSuccess) {
-    mir_set_error("%s: cannot reserve %d bytes of shared memory: %s", a.what, kSmemBytes, cudaGetErrorString(err));
-    return MIR_CUDA_ERROR;
-  }
-  const int group = a.heads / a.cache.kv_heads, units = a.cache.kv_heads * ((group + kHeads - 1) / kHeads);
-  // a request's CTAs start together; with a handful of rows partitions beyond the contexts come last
-  const dim3 grid = a.num_rows <= 4 ? dim3(a.num_rows, units, a.num_partitions) : dim3(a.num_partitions, units, a.num_rows);
-  return mir_launch("decode_attention_8bit", decode_8bit_kernel<G>, grid, dim3(kThreads), (size_t)kSmemBytes, a.stream, 0, maps[0], maps[1],
-                    maps[2], maps[3], (const bf16*)a.q, a.q_stride, a.cache, a.block_table, a.table_width, a.positions, a.heads,
-                    a.scale * kLog2e, a.window, a.partition, a.num_partitions, a.num_rows <= 4 ? 1 : 0, a.partial_o(a.num_rows),
-                    a.partial_ml(a.num_rows), (bf16*)a.out, a.sinks);
+  const int status = reserve_shared(decode_8bit_kernel<G>, Layout<G>::kSmemBytes, a.what);
+  if (status != MIR_OK) return status;
+  return mir_launch("decode_attention_8bit", decode_8bit_kernel<G>, dim3(a.num_partitions), dim3(kThreads), (size_t)Layout<G>::kSmemBytes, a.stream, 0,
+                    maps[0], maps[1], maps[2], maps[3], (const bf16*)a.q, a.q_stride, a.cache, a.block_table, a.table_width, a.positions,
+                    a.num_rows, a.heads, a.scale * kLog2e, a.window, a.scratch, (bf16*)a.out, a.sinks);
 }
 
 }  // namespace
@@ -421,11 +678,16 @@ bool mir_decode_8bit_takes(int head_dim, int page_size) {
   return head_dim == kDim && page_size >= 8 && page_size <= kKeys && kKeys % page_size == 0;
 }
 
+// CTAs over which it shares a call's tiles, and the floats of scratch for two parts of each.
+int mir_decode_8bit_ctas(long long most_tiles) { return (int)std::max(1ll, std::min(most_tiles, 2ll * mir_sm_count())); }
+long long mir_decode_8bit_floats(int ctas, int group) { return 2ll * ctas * std::min(group, kHeads) * (kDim + 2); }
+
 int mir_attention_8bit_decode(const Attention8& a) {
   if (a.num_rows > 65535) {
     mir_set_error("%s: %d rows are more than one launch takes", a.what, a.num_rows);
     return MIR_BAD_ARGUMENT;
   }
+  const int group = a.heads / a.cache.kv_heads;
   const long long rows = (long long)a.cache.pages * a.cache.page_size, width = (long long)a.cache.kv_heads * kDim;
   CUtensorMap maps[4];
   const void* tensors[2] = {a.cache.k, a.cache.v};
@@ -433,8 +695,9 @@ int mir_attention_8bit_decode(const Attention8& a) {
     const int status = tensor_map_of_bytes(tensors[i & 1], rows, width, width, i < 2 ? a.cache.page_size : kKeys, &maps[i]);
     if (status != MIR_OK) return status;
   }
-  const int columns = std::min(a.heads / a.cache.kv_heads, kHeads);
+  const int columns = std::min(group, kHeads);
   const int status = columns <= 4 ? launch<4>(a, maps) : (columns <= 8 ? launch<8>(a, maps) : launch<16>(a, maps));
-  if (status != MIR_OK || a.num_partitions == 1) return status;
-  return mir_merge_8bit(a, a.num_rows);
+  if (status != MIR_OK) return status;
+  return mir_launch("join_8bit", join_8bit_kernel, dim3((a.heads + kJoinWarps - 1) / kJoinWarps, a.num_rows), dim3(kJoinWarps * 32), 0, a.stream, 0, (const float*)a.scratch, a.positions,
+                    a.num_rows, a.heads, a.cache.kv_heads, a.window, a.num_partitions, (bf16*)a.out, a.sinks);
 }

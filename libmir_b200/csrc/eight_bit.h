@@ -16,7 +16,8 @@ struct Attention8 {
   int num_rows = 0, heads = 0, head_dim = 0;
   float scale = 0.0f;
   int window = 0;
-  int partition = 0, num_partitions = 1;   // keys split over this many partitions, joined by mir_merge_8bit
+  // keys split over this many partitions, joined by mir_merge_8bit; partition 0: all requests' keys shared out over that many CTAs
+  int partition = 0, num_partitions = 1;
   float* scratch = nullptr;
   long long scratch_floats = 0;
   const float* sinks = nullptr;        // [heads] or null
@@ -32,6 +33,8 @@ int mir_attention_8bit_general(const Attention8& a, int tokens);
 int mir_merge_8bit(const Attention8& a, int tokens);
 // Single tokens on the 5th-generation tensor cores (attention_8bit_decode.cu), where it takes the sizes.
 bool mir_decode_8bit_takes(int head_dim, int page_size);
+int mir_decode_8bit_ctas(long long most_tiles);
+long long mir_decode_8bit_floats(int ctas, int group);
 int mir_attention_8bit_decode(const Attention8& a);
 
 // The product of rounded rows (codes [m, k], scales [blocks of 128 columns, scale_stride], scale_stride m

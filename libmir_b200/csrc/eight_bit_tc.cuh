@@ -85,6 +85,27 @@ inline int tensor_map_of_results(const void* base, bool is_float, long long rows
                        ld, 32, 64, map);
 }
 
+// Lets a kernel have this much shared memory, once for each device.
+template <typename Kernel>
+inline int reserve_shared(Kernel kernel, int bytes, const char* what) {
+  static std::mutex g_mutex;
+  static std::map<std::pair<const void*, int>, int> g_done;
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err == cudaSuccess) {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    int& done = g_done[std::make_pair(reinterpret_cast<const void*>(kernel), device)];
+    if (done >= bytes) return MIR_OK;
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err == cudaSuccess) done = bytes;
+  }
+  if (err != cudaSuccess) {
+    mir_set_error("%s: cannot reserve %d bytes of shared memory: %s", what, bytes, cudaGetErrorString(err));
+    return MIR_CUDA_ERROR;
+  }
+  return MIR_OK;
+}
+
 // a * b + c of two numbers side by side.
 __device__ __forceinline__ float2 fma_two(float2 a, float2 b, float2 c) {
   unsigned long long x, y, z, d;

@@ -316,11 +316,8 @@ int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, int scale_s
     return MIR_BAD_ARGUMENT;
   }
   auto kernel = out_float ? linear_8bit_tiles_kernel<true> : linear_8bit_tiles_kernel<false>;
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (err != cudaSuccess) {
-    mir_set_error("linear_8bit: cannot reserve %d bytes of shared memory: %s", kSmemBytes, cudaGetErrorString(err));
-    return MIR_CUDA_ERROR;
-  }
+  status = reserve_shared(kernel, kSmemBytes, "linear_8bit");
+  if (status != MIR_OK) return status;
   // results by way of shared memory where their rows begin and lie on 16-byte boundaries
   const int width = out_float ? 4 : 2;
   const bool boxes = ((uintptr_t)out & 15) == 0 && (out_stride * width) % 16 == 0;

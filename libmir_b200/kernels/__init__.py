@@ -239,6 +239,8 @@ _SIGNATURES = {
         "mir_prefill_attention_8bit": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
                                        c_void_p, c_longlong, c_void_p, c_void_p],
+        "mir_decode_attention_8bit_error": [],
+        "mir_linear_8bit_tiles_error": [],
         "mir_linear_8bit_workspace": [c_int, c_int],
         "mir_quantize_weight_8bit": [c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
         "mir_linear_8bit": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int,
@@ -2383,5 +2385,5 @@ def repetition_penalty(logits: torch.Tensor, ids: torch.Tensor, id_rows: torch.T
                                            id_rows.data_ptr(), penalties.data_ptr(), ids.numel(), _stream()))
 
 
-from .eight_bit import (decode_attention_8bit, decode_attention_8bit_plan, linear_8bit,  # noqa: E402,F401
+from .eight_bit import (decode_attention_8bit, decode_attention_8bit_plan, eight_bit_error, linear_8bit,  # noqa: E402,F401
                         prefill_attention_8bit, quantize_weight_8bit, store_kv_8bit)

@@ -85,8 +85,10 @@ def store_kv_8bit(qkv: torch.Tensor, slot_mapping: torch.Tensor, k_pages: torch.
 
 
 def decode_attention_8bit_plan(rows: int, heads: int, kv_heads: int, head_dim: int, page_size: int, max_context: int) -> tuple:
-    """(keys per partition, partitions, floats of scratch) for decode_attention_8bit of `rows` single tokens whose longest
-    context is max_context keys."""
+    """(partition, num_partitions, floats of scratch) for decode_attention_8bit of `rows` single tokens whose longest context is
+    max_context keys.  Sizes that the tcgen05 kernel takes (head_dim 128, pages of 8 to 128 keys that divide 128): partition 0,
+    and the CTAs over which it shares all requests' keys out evenly, by the positions it finds on the device, however long
+    the contexts are by then.  Others: keys per partition, and as many partitions as cover the longest context."""
     keys, count, floats = ctypes.c_int(), ctypes.c_int(), ctypes.c_longlong()
     lib = library("eight_bit")
     _check(lib, lib.mir_decode_attention_8bit_plan(rows, heads, kv_heads, head_dim, page_size, max_context, ctypes.byref(keys),
@@ -102,7 +104,7 @@ def decode_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.T
     """decode_attention over an 8-bit cache: row r of qkv is one token of request r at positions[r], and sees the keys up to
     its own (inside the window).  A position below 0 is a padding row: its row of `out` is left as it is.  Keys whose page the
     block table does not have (an entry below 0 or beyond the pool, or a block behind its last column) are not seen; a row
-    that sees none gets zeros.  The partitions (decode_attention_8bit_plan) cover the longest context: keys behind
+    that sees none gets zeros.  `partition`, `num_partitions`: decode_attention_8bit_plan's; where partition is not 0, keys behind
     partition * num_partitions are not seen either.  `scratch`: float32, the plan's size; calls that may run at the same
     time, or graphs, take one each.  `sinks`: one number per query head in the softmax's denominator."""
     what = "decode_attention_8bit"
@@ -147,6 +149,13 @@ def prefill_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.
         v_scales.data_ptr(), pages, block_table.data_ptr(), block_table.shape[1], query_starts.data_ptr(), context_lens.data_ptr(),
         rows, tokens, page_size, heads, kv_heads, head_dim, scale, int(window or 0), partition, count, _ptr(scratch),
         0 if scratch is None else scratch.numel(), _ptr(sinks), _stream()))
+
+
+def eight_bit_error() -> int:
+    """0 unless a bounded wait of one of the tcgen05 kernels ran out (synchronises the device); such a kernel does no work from
+    then on."""
+    lib = library("eight_bit")
+    return int(lib.mir_decode_attention_8bit_error() or lib.mir_linear_8bit_tiles_error())
 
 
 def quantize_weight_8bit(weight: torch.Tensor) -> tuple:

@@ -287,6 +287,25 @@ def test_decode_attention_hides_missing_pages_and_what_lies_there(dim):
         close(out, want, attention_bound(want, size))
 
 
+@pytest.mark.parametrize("heads, kv_heads, rows, longest", [(32, 8, 90, 300), (16, 16, 70, 130), (20, 1, 600, 260), (8, 8, 150, 500)])
+def test_decode_attention_of_many_short_contexts(heads, kv_heads, rows, longest):
+    """More requests and kv heads than CTAs, each of one to four tiles of keys: every CTA takes several, and parts of some.
+    More rows than a CTA keeps positions of; padding rows anywhere."""
+    from libmir_b200 import kernels
+    g = seeded(rows)
+    lengths = torch.randint(1, longest + 1, (rows,), generator=g).tolist()
+    batch = Batch(19, lengths, heads, kv_heads, 128, 16)
+    positions = [n - 1 if i % 7 else -1 for i, n in enumerate(lengths)]
+    out = run_decode(batch, batch.on_gpu(), positions, 0.09)
+    picked = [i for i in range(rows) if i % (rows // 30) == 0 and positions[i] >= 0]
+    some = [positions[i] if i in picked else -1 for i in range(rows)]
+    want, size = batch.decode(some, 0.09)
+    close(out[picked], want[picked], attention_bound(want, size)[picked])
+    padding = [i for i in range(rows) if positions[i] < 0]
+    assert (out[padding] == 7.0).all()
+    assert kernels.eight_bit_error() == 0
+
+
 def test_decode_attention_of_a_context_longer_than_its_table_reads_what_is_there():
     batch = Batch(17, [64], 8, 2, 128, 16)
     out = run_decode(batch, batch.on_gpu(), [1000], 0.1)
