@@ -363,9 +363,8 @@ MIR_EXPORT int mir_decode_attention_8bit_plan(int rows, int heads, int kv_heads,
   const int group = heads / kv_heads;
   if (mir_decode_8bit_takes(head_dim, page_size)) {
     // the tcgen05 kernel shares all requests' keys out over its CTAs by the positions that it finds
-    const long long units = (long long)kv_heads * ((group + 15) / 16);
     *keys = 0;
-    *count = mir_decode_8bit_ctas(rows * units * std::max(1ll, (max_context + 127ll) / 128));
+    *count = mir_decode_8bit_ctas(rows * std::max(1ll, (max_context + 127ll) / 128), heads, kv_heads);
     *floats = mir_decode_8bit_floats(*count, group);
     return MIR_OK;
   }

@@ -1,11 +1,12 @@
 // Attention of single tokens over the 8-bit cache on the 5th-generation tensor cores, head_dim 128, pages of 8 to 128 keys:
 // the bytes of the cache go from memory into the products as they are, nothing is widened.
 //
-// The work is all requests' tiles of 128 keys, times their kv heads (16 query heads of a group at most), one behind the other; every
-// CTA takes the same number of tiles of that row, so that requests of any lengths load all SMs alike (a CTA for each request and
-// kv head left the SMs idle for 29% of the time with 64 contexts of 1,024 to 2,048 keys).  A stretch of one request and kv head that
-// lies within a CTA is finished there; the parts of one that is cut are joined by a second kernel.  What is cut where
-// follows from the positions alone, on the device: a captured launch fits contexts that have grown.
+// The work is all requests' tiles of 128 keys, one behind the other, for every unit (a kv head and up to 16 query heads of its
+// group).  It is shared out evenly over teams of CTAs, a CTA for each unit, by the positions alone and on the device, so that requests
+// of any lengths load all SMs alike and a captured launch fits contexts that have grown.  The CTAs of a team read the same rows of the
+// cache at the same time, 128 bytes beside each other: a CTA that took one unit's tiles after another's read those pieces by
+// themselves and got 4.5 TB/s.  Stretches of a request that lie within a team are finished there; the parts of one that is cut
+// are joined by a second kernel.
 // The products are transposed, so that the keys (then the elements of the head) are the 128 rows of the tensor
 // cores and the query heads the 16 columns:
 //
@@ -57,8 +58,8 @@ template <int G> struct Layout {
 static_assert(Layout<16>::kSmemBytes >= kLeastSharedBeside, "never beside a kernel that takes all tensor memory");
 
 enum { K_FULL = 0, K_FREE = K_FULL + 3, V_FULL = K_FREE + 3, V_FREE = V_FULL + 3, S_FULL = V_FREE + 3, P_READY = S_FULL + 2,
-       Q_READY = P_READY + 2, Q_FREE = Q_READY + 4, CHUNK_FULL = Q_FREE + 2, CHUNK_FREE = CHUNK_FULL + 2, PV_DONE = CHUNK_FREE + 2,
-       BARRIERS = PV_DONE + 2 };
+       Q_READY = P_READY + 2, Q_FREE = Q_READY + 4, CHUNK_FULL = Q_FREE + 2, CHUNK_FREE = CHUNK_FULL + 2, ROWS_FULL = CHUNK_FREE + 2,
+       PV_DONE = ROWS_FULL + 2, BARRIERS = PV_DONE + 2 };
 // Tiles are counted over the CTA's whole stretch (g): stage g % kStages of the rings, g & 1 of S_FULL, P_READY and PV_DONE (who waits for
 // tile g of one of them knows that tile g - 2 is over, so the parity says which), chunk g / kChunk.
 // Parts are counted too (n): the queries' buffers and Q_FREE go by n & 1, Q_READY by n & 3: the softmax may begin part n when the
@@ -122,16 +123,21 @@ __device__ __forceinline__ Row row_at(const int* __restrict__ positions, int row
   return r;
 }
 
-// Where a CTA's stretch begins, and how long it is.  Stretches are `each` tiles; tile index = units * (tiles of the rows before) +
-// unit * (the row's tiles) + tile.
+// The least share with which `ctas` of them hold `total`.
+__device__ __forceinline__ long long shares_of(long long total, int ctas) {
+  if (total <= 0x7fffffffll - ctas) return ((unsigned)total + (unsigned)ctas - 1u) / (unsigned)ctas;
+  return (total + ctas - 1) / ctas;
+}
+
+// Where a team's stretch of tiles begins, and how long it is.
 struct Stretch {
-  int row, unit, tile;
+  int row, tile;
   long long count;
 };
 
-// One part of a stretch: tiles [first, last) of a row and unit.
+// One part of a stretch: tiles [first, last) of a row.
 struct Part {
-  int row, unit, first, last;
+  int row, first, last;
   Row of;
   __device__ __forceinline__ bool whole() const { return first == 0 && last == of.tiles; }
 };
@@ -140,20 +146,16 @@ struct Part {
 struct Walk {
   Stretch at;
   const int* positions;
-  int num_rows, units, window;
+  int num_rows, window;
   __device__ __forceinline__ bool next(Part& part) {
     if (at.count <= 0) return false;
     Row r = row_at(positions, at.row, window);
-    while (at.tile >= r.tiles) {                         // the row's next unit, or the next row that has tiles
+    while (at.tile >= r.tiles) {                         // the next row that has tiles
       at.tile = 0;
-      if (r.tiles == 0 || ++at.unit >= units) {
-        at.unit = 0;
-        if (++at.row >= num_rows) return false;
-        r = row_at(positions, at.row, window);
-      }
+      if (++at.row >= num_rows) return false;
+      r = row_at(positions, at.row, window);
     }
     part.row = at.row;
-    part.unit = at.unit;
     part.first = at.tile;
     part.last = (int)min((long long)r.tiles, at.tile + at.count);
     part.of = r;
@@ -167,7 +169,7 @@ struct Walk {
 struct Chunk {
   int row[kChunk][kSlots];                             // a page's first row of the cache; below 0 where it is not there or not wanted
   float2 scale[kChunk][kSlots];                        // its scales, of keys and of values
-  int column[kChunk], first[kChunk], last[kChunk];     // the kv head's bytes within a row; whether the tile is its part's first, its last
+  int first[kChunk], last[kChunk];                     // whether the tile is its part's first, its last
 };
 
 // G: heads that the softmax threads handle (a unit's heads rounded up to 4, 8 or 16).
@@ -196,6 +198,9 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
   auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
   const int group = heads / cache.kv_heads, group_tiles = (group + kHeads - 1) / kHeads, units = cache.kv_heads * group_tiles;
+  const int unit = blockIdx.x % units, team = blockIdx.x / units, teams = gridDim.x / units;
+  const int kv_head = unit / group_tiles, head0 = kv_head * group + unit % group_tiles * kHeads;
+  const int valid_heads = min(kHeads, kv_head * group + group - head0);
   if (threadIdx.x == 0) {
     for (int i = 0; i < BARRIERS; ++i) {
       const bool softmax = i == P_READY || i == P_READY + 1, chunk = i == CHUNK_FREE || i == CHUNK_FREE + 1;
@@ -213,20 +218,19 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   __syncthreads();
   const int* positions = num_rows <= kHeldRows ? held_positions : all_positions;
   if (warp == 0) {
-    // this CTA's stretch: all tiles over the CTAs, then the row that the first one lies in
+    // this team's stretch: all tiles over the teams, then the row that the first one lies in
     long long total = 0;
     for (int r = lane; r < num_rows; r += 32) total += row_at(positions, r, window).tiles;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= units;
-    const long long each = (total + gridDim.x - 1) / gridDim.x, first = each * blockIdx.x;
+    const long long each = shares_of(total, teams), first = each * team;
     Stretch mine;
-    mine.row = mine.unit = mine.tile = 0;
+    mine.row = mine.tile = 0;
     mine.count = min(each, total - first);
     long long before = 0;
     for (int r0 = 0; r0 < num_rows && mine.count > 0; r0 += 32) {
       const int tiles = r0 + lane < num_rows ? row_at(positions, r0 + lane, window).tiles : 0;
-      long long through = (long long)tiles * units;
+      long long through = tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long left = __shfl_up_sync(0xffffffffu, through, o);
@@ -236,11 +240,8 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
       const unsigned beyond = __ballot_sync(0xffffffffu, through > first);
       if (beyond != 0u) {
         const int in = __ffs(beyond) - 1;
-        const int row_tiles = __shfl_sync(0xffffffffu, tiles, in);
-        const long long inside = first - (__shfl_sync(0xffffffffu, through, in) - (long long)row_tiles * units);
         mine.row = r0 + in;
-        mine.unit = (int)(inside / row_tiles);
-        mine.tile = (int)(inside % row_tiles);
+        mine.tile = (int)(first - (__shfl_sync(0xffffffffu, through, in) - __shfl_sync(0xffffffffu, tiles, in)));
         break;
       }
       before = __shfl_sync(0xffffffffu, through, 31);
@@ -257,25 +258,60 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   const uint32_t tmem_s = tmem_slot, tmem_o = tmem_slot + 32u;
   const int shift = 31 - __clz(cache.page_size);       // pages are powers of two
   const int count = (int)max(0ll, stretch.count);      // tiles of this CTA
-  Walk walk{stretch, positions, num_rows, units, window};
+  Walk walk{stretch, positions, num_rows, window};
   Part part;
 
   if (warp == kScout) {
-    // ------------------------------------------------------------------ scout
+    // ------------------------------------------------------------------ scout: the table's entries are on their way a chunk ahead of
+    // the scales that they lead to (the memory is busy: a load takes 2 us and more)
     const int pages_per_tile = kKeys >> shift, page_size = cache.page_size;
     bool alive = true;
+    // this lane's two entries (tile, page slot) of the next chunk of `ahead`: the raw numbers of the table, -1 where none is wanted
+    Walk ahead = walk;
+    Part ahead_part;
+    ahead_part.last = 0;
+    int ahead_tile = 0;
+    auto look_up = [&](int tiles, int (&page)[2]) {
+      const int* from[2] = {block_table, block_table};
+      bool wanted[2] = {false, false};
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        if (j >= tiles) break;
+        if (ahead_tile >= ahead_part.last) {
+          ahead.next(ahead_part);
+          ahead_tile = ahead_part.first;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int entry = lane + 32 * i;
+          if (entry / pages_per_tile == j) {
+            const int key = ahead_part.of.begin + ahead_tile * kKeys + entry % pages_per_tile * page_size;
+            from[i] = block_table + (size_t)ahead_part.row * table_width + (key >> shift);
+            wanted[i] = key <= ahead_part.of.position && key + page_size > ahead_part.of.first_key && (key >> shift) < table_width;
+          }
+        }
+        ++ahead_tile;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        page[i] = -1;
+        if (wanted[i]) page[i] = *from[i];
+      }
+    };
+    auto load_queries = [&](const Part& of, uint2 (&raw)[G]) {
+      const bf16* from = q + (size_t)of.row * q_stride + (size_t)head0 * kDim + lane * 4;
+#pragma unroll
+      for (int h = 0; h < G; ++h) raw[h] = *reinterpret_cast<const uint2*>(from + min(h, valid_heads - 1) * kDim);
+    };
     int tile = 0, parts_begun = 0;                     // the walk's next tile of `part`
     part.last = 0;
+    int page[2], page_next[2] = {-1, -1};
+    look_up(min(kChunk, count), page);
     for (int g0 = 0; g0 < count; g0 += kChunk) {
       const int buffer = g0 / kChunk & 1, tiles = min(kChunk, count - g0);
-      if (alive && !wait_barrier(bar(CHUNK_FREE + buffer), (uint32_t)(g0 / kChunk >> 1 & 1) ^ 1u)) { g_error = 1; alive = false; }
-      __syncwarp();
-      Chunk& chunk = chunks[buffer];
+      if (g0 + kChunk < count) look_up(min(kChunk, count - g0 - kChunk), page_next);
       Part begun[kChunk];                              // the parts that begin in this chunk
-      int beginning = 0;
-      // what this lane's two entries (tile, page slot) of the chunk are
-      const int* table[2] = {block_table, block_table};
-      int block[2] = {-1, -1}, head_of[2] = {0, 0};
+      int beginning = 0, last_tiles = 0;
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) {
         if (j < tiles) {
@@ -284,42 +320,41 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
             tile = part.first;
           }
           if (tile == part.first) begun[j] = part;     // (an index known at compile time: registers)
-          if (lane == 0) {
-            chunk.column[j] = part.unit / group_tiles * kDim;
-            chunk.first[j] = tile == part.first;
-            chunk.last[j] = tile == part.last - 1;
-          }
           beginning |= (tile == part.first ? 1 : 0) << j;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int entry = lane + 32 * i;
-            if (entry / pages_per_tile == j) {
-              const int key = part.of.begin + tile * kKeys + entry % pages_per_tile * page_size;
-              table[i] = block_table + (size_t)part.row * table_width;
-              head_of[i] = part.unit / group_tiles;
-              block[i] = key <= part.of.position && key + page_size > part.of.first_key && (key >> shift) < table_width ? key >> shift : -1;
-            }
-          }
+          last_tiles |= (tile == part.last - 1 ? 1 : 0) << j;
           ++tile;
         }
       }
-      int page[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) page[i] = block[i] >= 0 ? table[i][block[i]] : -1;
+      uint2 raw[G];                                    // of the CTA's first part: beside the first table entries
+      if (g0 == 0) load_queries(begun[0], raw);
       float2 scale[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (page[i] >= cache.pages) page[i] = -1;
-        const size_t at = (size_t)max(page[i], 0) * cache.kv_heads + head_of[i];
-        scale[i] = page[i] >= 0 ? make_float2(cache.k_scales[at], cache.v_scales[at]) : make_float2(1.0f, 1.0f);
+        const size_t at = (size_t)max(page[i], 0) * cache.kv_heads + kv_head;
+        scale[i] = make_float2(1.0f, 1.0f);
+        if (page[i] >= 0) scale[i] = make_float2(cache.k_scales[at], cache.v_scales[at]);
       }
+      if (alive && !wait_barrier(bar(CHUNK_FREE + buffer), (uint32_t)(g0 / kChunk >> 1 & 1) ^ 1u)) { g_error = 1; alive = false; }
+      __syncwarp();
+      Chunk& chunk = chunks[buffer];
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j)
+        if (lane == j) {
+          chunk.first[j] = beginning >> j & 1;
+          chunk.last[j] = last_tiles >> j & 1;
+        }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int entry = lane + 32 * i;
-        if (entry < kChunk * pages_per_tile) {
-          chunk.row[entry / pages_per_tile][entry % pages_per_tile] = page[i] >= 0 ? page[i] << shift : -page_size;
-          chunk.scale[entry / pages_per_tile][entry % pages_per_tile] = scale[i];
-        }
+        if (entry < kChunk * pages_per_tile) chunk.row[entry / pages_per_tile][entry % pages_per_tile] = page[i] >= 0 ? page[i] << shift : -page_size;
+      }
+      __syncwarp();
+      if (lane == 0) barrier_arrive(bar(ROWS_FULL + buffer));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int entry = lane + 32 * i;
+        if (entry < kChunk * pages_per_tile) chunk.scale[entry / pages_per_tile][entry % pages_per_tile] = scale[i];
       }
       __syncwarp();
       if (lane == 0) barrier_arrive(bar(CHUNK_FULL + buffer));
@@ -328,14 +363,9 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
       for (int j = 0; j < kChunk; ++j) {
         if ((beginning >> j & 1) == 0) continue;
         const int parity = parts_begun & 1;
+        if (g0 + j > 0) load_queries(begun[j], raw);
         if (alive && !wait_barrier(bar(Q_FREE + parity), (uint32_t)(parts_begun >> 1 & 1) ^ 1u)) { g_error = 1; alive = false; }
         __syncwarp();
-        const int kv_head = begun[j].unit / group_tiles, head0 = kv_head * group + begun[j].unit % group_tiles * kHeads;
-        const int valid_heads = min(kHeads, kv_head * group + group - head0);
-        const bf16* from = q + (size_t)begun[j].row * q_stride + (size_t)head0 * kDim + lane * 4;
-        uint2 raw[G];
-#pragma unroll
-        for (int h = 0; h < G; ++h) raw[h] = *reinterpret_cast<const uint2*>(from + min(h, valid_heads - 1) * kDim);
 #pragma unroll
         for (int h = 0; h < G; ++h) {
           float x[4] = {__uint_as_float(raw[h].x << 16), __uint_as_float(raw[h].x & 0xffff0000u), __uint_as_float(raw[h].y << 16),
@@ -356,6 +386,8 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
         if (lane == 0) barrier_arrive(bar(Q_READY + (parts_begun & 3)));
         ++parts_begun;
       }
+      page[0] = page_next[0];
+      page[1] = page_next[1];
     }
   } else if (warp == kKeyLoader || warp == kValueLoader) {
     // ------------------------------------------------------------------ loaders: lane l has page slot l of the tile
@@ -368,9 +400,9 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
     uint32_t stage = 0, parity = 0;
     for (int g = 0; g < count; ++g) {
       const int buffer = g / kChunk & 1;
-      if (g % kChunk == 0 && alive && !wait_barrier(bar(CHUNK_FULL + buffer), (uint32_t)(g / kChunk >> 1 & 1))) { g_error = 1; alive = false; }
+      if (g % kChunk == 0 && alive && !wait_barrier(bar(ROWS_FULL + buffer), (uint32_t)(g / kChunk >> 1 & 1))) { g_error = 1; alive = false; }
       alive = __all_sync(0xffffffffu, alive);
-      const int cache_row = loads ? chunks[buffer].row[g % kChunk][lane] : 0, column = chunks[buffer].column[g % kChunk];
+      const int cache_row = loads ? chunks[buffer].row[g % kChunk][lane] : 0;
       __syncwarp();
       if (g % kChunk == kChunk - 1 && lane == 0) barrier_arrive(bar(CHUNK_FREE + buffer));
       if (alive && !wait_barrier(free0 + 8u * stage, parity ^ 1u)) { g_error = 1; alive = false; }
@@ -384,9 +416,9 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
       if (lane == 0) barrier_expect_bytes(full, (uint32_t)kTile);
       __syncwarp();
       if (in_a_row) {
-        if (lane == 0) tma_load_2d(to, values ? &v_tile_map : &k_tile_map, full, column, first_row);
+        if (lane == 0) tma_load_2d(to, values ? &v_tile_map : &k_tile_map, full, kv_head * kDim, first_row);
       } else if (loads) {                              // (a negative row lies outside the tensor: zeros)
-        tma_load_2d(to + (uint32_t)lane * box_bytes, values ? &v_map : &k_map, full, column, cache_row);
+        tma_load_2d(to + (uint32_t)lane * box_bytes, values ? &v_map : &k_map, full, kv_head * kDim, cache_row);
       }
       if (++stage == (uint32_t)kStages) { stage = 0; parity ^= 1u; }
     }
@@ -408,7 +440,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
     int n = 0;                                         // parts whose scores are under way
     auto issue_scores = [&](int g) {
       const int buffer = g / kChunk & 1;
-      if (g % kChunk == 0) check(CHUNK_FULL + buffer, (uint32_t)(g / kChunk >> 1 & 1));
+      if (g % kChunk == 0) check(ROWS_FULL + buffer, (uint32_t)(g / kChunk >> 1 & 1));
       __syncwarp();
       const bool first = __shfl_sync(0xffffffffu, chunks[buffer].first[g % kChunk], 0) != 0;
       const bool last = __shfl_sync(0xffffffffu, chunks[buffer].last[g % kChunk], 0) != 0;
@@ -432,10 +464,27 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
       first_tiles = (first_tiles & ~(1u << (g & 3))) | ((first ? 1u : 0u) << (g & 3));
       if (++k_stage == (uint32_t)kStages) { k_stage = 0; k_parity ^= 1u; }
     };
-    for (int g = 0; g < min(count, 2); ++g) issue_scores(g);
+    // Whether all lanes see the phase with this parity complete, without waiting for it.
+    auto complete = [&](int index, uint32_t parity) {
+      uint32_t done;
+      asm volatile("{\n\t.reg .pred P1;\n\tmbarrier.test_wait.parity.shared::cta.b64 P1, [%1], %2;\n\tselp.b32 %0, 1, 0, P1;\n\t}"
+                   : "=r"(done) : "r"(bar(index)), "r"(parity) : "memory");
+      return __all_sync(0xffffffffu, done != 0u) != 0;
+    };
+    // Scores are issued up to two tiles ahead of the product with the values, but a product whose values and weights are there does
+    // not wait behind scores whose keys are not.
+    int issued = 0;
     for (int g = 0; g < count; ++g) {
-      check(V_FULL + (int)v_stage, v_parity);
-      check(P_READY + (g & 1), (uint32_t)(g >> 1 & 1));
+      unsigned long long start = 0;
+      for (unsigned poll = 1; alive; ++poll) {
+        if (issued < min(count, g + 2) && (issued == 0 || complete(K_FULL + (int)k_stage, k_parity))) issue_scores(issued++);
+        else if (complete(V_FULL + (int)v_stage, v_parity) && complete(P_READY + (g & 1), (uint32_t)(g >> 1 & 1))) break;
+        if ((poll & 63u) == 0u) {
+          const unsigned long long now = global_nanoseconds();
+          if (start == 0) start = now;
+          else if (__any_sync(0xffffffffu, now - start > kWaitNanoseconds)) { g_error = 2; alive = false; }
+        }
+      }
       __syncwarp();
       tensor_fence_after_sync();
       const uint32_t a = v_low + v_stage * kTileStep, b = p_low + (uint32_t)(g & 1) * 2u * kPartStep;
@@ -450,9 +499,8 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
       mma_commit_elected(bar(V_FREE + (int)v_stage), elected);
       mma_commit_elected(bar(PV_DONE + (g & 1)), elected);
       if (++v_stage == (uint32_t)kStages) { v_stage = 0; v_parity ^= 1u; }
-      // The scores of the tile after next take the accumulator that the softmax has read (P_READY says so); issued behind this
-      // product, their barrier also says that the weights' buffer is free.
-      if (g + 2 < count) issue_scores(g + 2);
+      // (The scores of the tile after next take the accumulator that the softmax has read: P_READY says so.  Issued behind this
+      // product, their barrier also says that the weights' buffer is free.)
     }
   } else {
     // ------------------------------------------------------------------ softmax: thread = key of the tile, then element
@@ -463,9 +511,6 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
     int g = 0;
     for (int n = 0; walk.next(part); ++n) {
       const Row& of = part.of;
-      const int kv_head = part.unit / group_tiles;
-      const int head0 = kv_head * group + part.unit % group_tiles * kHeads;
-      const int valid_heads = min(kHeads, kv_head * group + group - head0);
       float top[G], top_weight[G], denominator[G];
 #pragma unroll
       for (int h = 0; h < G; ++h) {
@@ -569,7 +614,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
       tmem_load<G>(tmem_o + lane_bits, o);
       // (the next part's first product waits for its weights, which these threads write behind this)
       if (alive) {
-        // a part that is not the whole: in its CTA's second place if it begins here, in the first if it goes on from the CTA before
+        // a part that is not the whole: in its CTA's second place if it begins here, in the first if it goes on from the team before
         const int heads_of_unit = min(group, kHeads);
         float* to = parts + ((size_t)blockIdx.x * 2 + (part.first == 0 ? 1 : 0)) * heads_of_unit * (kDim + 2);
 #pragma unroll
@@ -605,7 +650,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
 constexpr int kJoinWarps = 4;
 __global__ void __launch_bounds__(kJoinWarps * 32)
 join_8bit_kernel(const float* __restrict__ parts, const int* __restrict__ positions, int num_rows, int heads, int kv_heads, int window,
-                 int ctas, bf16* __restrict__ out, const float* __restrict__ sinks) {
+                 int teams, bf16* __restrict__ out, const float* __restrict__ sinks) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int row = blockIdx.y, head = blockIdx.x * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -625,13 +670,15 @@ join_8bit_kernel(const float* __restrict__ parts, const int* __restrict__ positi
   const int group = heads / kv_heads, group_tiles = (group + kHeads - 1) / kHeads, units = kv_heads * group_tiles;
   const int tiles = row_at(positions, row, window).tiles;
   if (tiles == 0) return;
-  const long long each = (total * units + ctas - 1) / ctas;
+  const long long each = shares_of(total, teams);
   const int heads_of_unit = min(group, kHeads);
   const int in_group = head % group, unit = head / group * group_tiles + in_group / kHeads, h = in_group % kHeads;
-  const long long first = before * units + (long long)unit * tiles;
-  const int from = (int)(first / each), to = (int)((first + tiles - 1) / each);
-  if (from == to) return;                              // one CTA had all of it
-  auto place = [&](int cta) { return parts + (((size_t)cta * 2 + (cta == from ? 1 : 0)) * heads_of_unit + h) * (kDim + 2); };
+  const long long first = before;
+  const bool small = total <= 0x7fffffffll;      // (a division of 64 bits takes far longer)
+  const int from = small ? (int)((unsigned)first / (unsigned)each) : (int)(first / each);
+  const int to = small ? (int)((unsigned)(first + tiles - 1) / (unsigned)each) : (int)((first + tiles - 1) / each);
+  if (from == to) return;                              // one team had all of it
+  auto place = [&](int team) { return parts + ((((size_t)team * units + unit) * 2 + (team == from ? 1 : 0)) * heads_of_unit + h) * (kDim + 2); };
   float top = -INFINITY;
   for (int c = from + lane; c <= to; c += 32) {
     const float2 ml = *reinterpret_cast<const float2*>(place(c) + kDim);
@@ -678,8 +725,11 @@ bool mir_decode_8bit_takes(int head_dim, int page_size) {
   return head_dim == kDim && page_size >= 8 && page_size <= kKeys && kKeys % page_size == 0;
 }
 
-// CTAs over which it shares a call's tiles, and the floats of scratch for two parts of each.
-int mir_decode_8bit_ctas(long long most_tiles) { return (int)std::max(1ll, std::min(most_tiles, 2ll * mir_sm_count())); }
+// The CTAs of a call whose rows have at most `most_tiles` tiles together, and the floats of scratch for two parts of each.
+int mir_decode_8bit_ctas(long long most_tiles, int heads, int kv_heads) {
+  const long long units = (long long)kv_heads * ((heads / kv_heads + kHeads - 1) / kHeads);
+  return (int)(units * std::max(1ll, std::min(most_tiles, 2ll * mir_sm_count() / units)));
+}
 long long mir_decode_8bit_floats(int ctas, int group) { return 2ll * ctas * std::min(group, kHeads) * (kDim + 2); }
 
 int mir_attention_8bit_decode(const Attention8& a) {
@@ -687,7 +737,11 @@ int mir_attention_8bit_decode(const Attention8& a) {
     mir_set_error("%s: %d rows are more than one launch takes", a.what, a.num_rows);
     return MIR_BAD_ARGUMENT;
   }
-  const int group = a.heads / a.cache.kv_heads;
+  const int group = a.heads / a.cache.kv_heads, units = a.cache.kv_heads * ((group + kHeads - 1) / kHeads);
+  if (a.num_partitions % units != 0) {
+    mir_set_error("%s: %d partitions are not a plan's for %d heads and %d kv heads", a.what, a.num_partitions, a.heads, a.cache.kv_heads);
+    return MIR_BAD_ARGUMENT;
+  }
   const long long rows = (long long)a.cache.pages * a.cache.page_size, width = (long long)a.cache.kv_heads * kDim;
   CUtensorMap maps[4];
   const void* tensors[2] = {a.cache.k, a.cache.v};
@@ -699,5 +753,5 @@ int mir_attention_8bit_decode(const Attention8& a) {
   const int status = columns <= 4 ? launch<4>(a, maps) : (columns <= 8 ? launch<8>(a, maps) : launch<16>(a, maps));
   if (status != MIR_OK) return status;
   return mir_launch("join_8bit", join_8bit_kernel, dim3((a.heads + kJoinWarps - 1) / kJoinWarps, a.num_rows), dim3(kJoinWarps * 32), 0, a.stream, 0, (const float*)a.scratch, a.positions,
-                    a.num_rows, a.heads, a.cache.kv_heads, a.window, a.num_partitions, (bf16*)a.out, a.sinks);
+                    a.num_rows, a.heads, a.cache.kv_heads, a.window, a.num_partitions / units, (bf16*)a.out, a.sinks);
 }

@@ -33,7 +33,7 @@ int mir_attention_8bit_general(const Attention8& a, int tokens);
 int mir_merge_8bit(const Attention8& a, int tokens);
 // Single tokens on the 5th-generation tensor cores (attention_8bit_decode.cu), where it takes the sizes.
 bool mir_decode_8bit_takes(int head_dim, int page_size);
-int mir_decode_8bit_ctas(long long most_tiles);
+int mir_decode_8bit_ctas(long long most_tiles, int heads, int kv_heads);
 long long mir_decode_8bit_floats(int ctas, int group);
 int mir_attention_8bit_decode(const Attention8& a);
 

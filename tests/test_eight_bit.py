@@ -65,7 +65,7 @@ def native_decode(**change):
     a = dict(q=AT, stride=48 * 128, out=AT, k=AT, v=AT, ks=AT, vs=AT, pages=100, table=AT, width=10, positions=AT, rows=3, page=16,
              heads=32, kv_heads=8, dim=128, scale=0.1, window=0, partition=256, parts=1, scratch=None, floats=0, sinks=None, stream=None)
     if "partition" not in change and change.get("dim", 128) != 64:
-        a.update(partition=0, scratch=AT, floats=1 << 20)               # (what the plan says for these sizes)
+        a.update(partition=0, parts=8, scratch=AT, floats=1 << 20)               # (what the plan says for these sizes)
     a.update(change)
     return kernels.library("eight_bit").mir_decode_attention_8bit(*a.values())
 
@@ -86,7 +86,7 @@ BAD_ATTENTION = [dict(dim=96), dict(dim=256), dict(heads=33), dict(heads=0), dic
 
 
 @pytest.mark.parametrize("change", [c for c in BAD_ATTENTION if c.get("parts") != 2]
-                         + [dict(scratch=None), dict(floats=2 * 4 * 130 - 1), dict(partition=128), dict(dim=64, partition=0), dict(page=24, partition=0),
+                         + [dict(scratch=None), dict(floats=8 * 2 * 4 * 130 - 1), dict(parts=9), dict(partition=128), dict(dim=64, partition=0), dict(page=24, partition=0),
                             dict(parts=2, dim=64, scratch=None), dict(parts=2, dim=64, scratch=AT, floats=3 * 32 * 2 * 66 - 1)])
 def test_decode_attention_refuses(change):
     assert native_decode(**change) == BAD_ARGUMENT
@@ -119,7 +119,8 @@ def test_a_plan_covers_the_context_with_whole_tiles(rows, heads, kv_heads, conte
     assert keys % 128 == 0 and keys * count >= context and (count == 1 or keys * (count - 1) < context) and count <= 65535
     assert floats == (0 if count == 1 else rows * heads * count * 66)
     keys, count, floats = kernels.decode_attention_8bit_plan(rows, heads, kv_heads, 128, 16, context)      # shared out
-    assert keys == 0 and 1 <= count <= min(2 * 148, max(1, rows * heads * max(1, -(-context // 128))))
+    units = kv_heads * -(-(heads // kv_heads) // 16)
+    assert keys == 0 and count % units == 0 and 1 <= count // units <= max(1, min(2 * 148 // units, rows * max(1, -(-context // 128))))
     assert floats == 2 * count * min(heads // kv_heads, 16) * 130
     with pytest.raises(KernelError):
         kernels.decode_attention_8bit_plan(rows, heads, kv_heads + heads, 128, 16, context)
