@@ -110,29 +110,26 @@ __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& 
   lo = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a - taken.x, b - taken.y), __NV_SATFINITE, __NV_E5M2);
 }
 
-// A row's share of the work: its tiles of keys, from the tile that holds its first visible key.
+// A row's share of the work: its tiles of keys, from the tile that holds its first visible key to the last that the table can have
+// (one at least: a row that sees nothing gets zeros).  All rows' tiles together are below 2^31: the launcher checks.
 struct Row {
   int position, first_key, begin, tiles;
 };
-__device__ __forceinline__ Row row_at(const int* __restrict__ positions, int row, int window) {
+__device__ __forceinline__ Row row_at(const int* __restrict__ positions, int row, int window, int table_keys) {
   Row r;
   r.position = positions[row];
   r.first_key = (window > 0 && r.position >= window) ? r.position + 1 - window : 0;
   r.begin = r.first_key / kKeys * kKeys;
-  r.tiles = r.position >= 0 ? (int)(((long long)r.position + kKeys - r.begin) / kKeys) : 0;     // (a padding row: none)
+  r.tiles = r.position < 0 ? 0 : max(1, (min(r.position, table_keys - 1) - r.begin) / kKeys + 1);       // (a padding row: none)
   return r;
 }
 
-// The least share with which `ctas` of them hold `total`.
-__device__ __forceinline__ long long shares_of(long long total, int ctas) {
-  if (total <= 0x7fffffffll - ctas) return ((unsigned)total + (unsigned)ctas - 1u) / (unsigned)ctas;
-  return (total + ctas - 1) / ctas;
-}
+// The least share with which `teams` of them hold `total`.
+__device__ __forceinline__ unsigned shares_of(unsigned total, int teams) { return (total + (unsigned)teams - 1u) / (unsigned)teams; }
 
 // Where a team's stretch of tiles begins, and how long it is.
 struct Stretch {
-  int row, tile;
-  long long count;
+  int row, tile, count;
 };
 
 // One part of a stretch: tiles [first, last) of a row.
@@ -146,18 +143,18 @@ struct Part {
 struct Walk {
   Stretch at;
   const int* positions;
-  int num_rows, window;
+  int num_rows, window, table_keys;
   __device__ __forceinline__ bool next(Part& part) {
     if (at.count <= 0) return false;
-    Row r = row_at(positions, at.row, window);
+    Row r = row_at(positions, at.row, window, table_keys);
     while (at.tile >= r.tiles) {                         // the next row that has tiles
       at.tile = 0;
       if (++at.row >= num_rows) return false;
-      r = row_at(positions, at.row, window);
+      r = row_at(positions, at.row, window, table_keys);
     }
     part.row = at.row;
     part.first = at.tile;
-    part.last = (int)min((long long)r.tiles, at.tile + at.count);
+    part.last = min(r.tiles, at.tile + at.count);
     part.of = r;
     at.count -= part.last - part.first;
     at.tile = part.last;
@@ -201,6 +198,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   const int unit = blockIdx.x % units, team = blockIdx.x / units, teams = gridDim.x / units;
   const int kv_head = unit / group_tiles, head0 = kv_head * group + unit % group_tiles * kHeads;
   const int valid_heads = min(kHeads, kv_head * group + group - head0);
+  const int table_keys = (int)min(0x7fffffffll, (long long)table_width * cache.page_size);
   if (threadIdx.x == 0) {
     for (int i = 0; i < BARRIERS; ++i) {
       const bool softmax = i == P_READY || i == P_READY + 1, chunk = i == CHUNK_FREE || i == CHUNK_FREE + 1;
@@ -219,32 +217,31 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   const int* positions = num_rows <= kHeldRows ? held_positions : all_positions;
   if (warp == 0) {
     // this team's stretch: all tiles over the teams, then the row that the first one lies in
-    long long total = 0;
-    for (int r = lane; r < num_rows; r += 32) total += row_at(positions, r, window).tiles;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const long long each = shares_of(total, teams), first = each * team;
+    unsigned total = 0;
+    for (int r = lane; r < num_rows; r += 32) total += (unsigned)row_at(positions, r, window, table_keys).tiles;
+    total = __reduce_add_sync(0xffffffffu, total);
+    const unsigned each = shares_of(total, teams), first = min(total, each * (unsigned)team);
     Stretch mine;
     mine.row = mine.tile = 0;
-    mine.count = min(each, total - first);
-    long long before = 0;
+    mine.count = (int)min(each, total - first);
+    unsigned before = 0;
     for (int r0 = 0; r0 < num_rows && mine.count > 0; r0 += 32) {
-      const int tiles = r0 + lane < num_rows ? row_at(positions, r0 + lane, window).tiles : 0;
-      long long through = tiles;
+      const unsigned tiles = r0 + lane < num_rows ? (unsigned)row_at(positions, r0 + lane, window, table_keys).tiles : 0u;
+      const unsigned all = __reduce_add_sync(0xffffffffu, tiles);
+      if (before + all > first) {
+        unsigned through = tiles;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long left = __shfl_up_sync(0xffffffffu, through, o);
-        if (lane >= o) through += left;
-      }
-      through += before;
-      const unsigned beyond = __ballot_sync(0xffffffffu, through > first);
-      if (beyond != 0u) {
-        const int in = __ffs(beyond) - 1;
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned left = __shfl_up_sync(0xffffffffu, through, o);
+          if (lane >= o) through += left;
+        }
+        through += before;
+        const int in = __ffs(__ballot_sync(0xffffffffu, through > first)) - 1;
         mine.row = r0 + in;
-        mine.tile = (int)(first - (__shfl_sync(0xffffffffu, through, in) - __shfl_sync(0xffffffffu, tiles, in)));
+        mine.tile = (int)(first - __shfl_sync(0xffffffffu, through - tiles, in));
         break;
       }
-      before = __shfl_sync(0xffffffffu, through, 31);
+      before += all;
     }
     if (lane == 0) {
       if (*reinterpret_cast<volatile int*>(&g_error) != 0) mine.count = 0;       // an earlier wait ran out: nothing is begun
@@ -257,14 +254,15 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   grid_launch_dependents();
   const uint32_t tmem_s = tmem_slot, tmem_o = tmem_slot + 32u;
   const int shift = 31 - __clz(cache.page_size);       // pages are powers of two
-  const int count = (int)max(0ll, stretch.count);      // tiles of this CTA
-  Walk walk{stretch, positions, num_rows, window};
+  const int count = stretch.count;                     // tiles of this CTA
+  Walk walk{stretch, positions, num_rows, window, table_keys};
   Part part;
 
   if (warp == kScout) {
     // ------------------------------------------------------------------ scout: the table's entries are on their way a chunk ahead of
     // the scales that they lead to (the memory is busy: a load takes 2 us and more)
-    const int pages_per_tile = kKeys >> shift, page_size = cache.page_size;
+    const int slot_shift = 7 - shift, page_size = cache.page_size;     // (128 >> shift pages a tile)
+    const int entries = kChunk << slot_shift, slot = lane & ((1 << slot_shift) - 1);
     bool alive = true;
     // this lane's two entries (tile, page slot) of the next chunk of `ahead`: the raw numbers of the table, -1 where none is wanted
     Walk ahead = walk;
@@ -284,8 +282,8 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int entry = lane + 32 * i;
-          if (entry / pages_per_tile == j) {
-            const int key = ahead_part.of.begin + ahead_tile * kKeys + entry % pages_per_tile * page_size;
+          if (entry >> slot_shift == j) {
+            const int key = ahead_part.of.begin + ahead_tile * kKeys + (slot << shift);
             from[i] = block_table + (size_t)ahead_part.row * table_width + (key >> shift);
             wanted[i] = key <= ahead_part.of.position && key + page_size > ahead_part.of.first_key && (key >> shift) < table_width;
           }
@@ -347,14 +345,14 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int entry = lane + 32 * i;
-        if (entry < kChunk * pages_per_tile) chunk.row[entry / pages_per_tile][entry % pages_per_tile] = page[i] >= 0 ? page[i] << shift : -page_size;
+        if (entry < entries) chunk.row[entry >> slot_shift][slot] = page[i] >= 0 ? page[i] << shift : -page_size;
       }
       __syncwarp();
       if (lane == 0) barrier_arrive(bar(ROWS_FULL + buffer));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int entry = lane + 32 * i;
-        if (entry < kChunk * pages_per_tile) chunk.scale[entry / pages_per_tile][entry % pages_per_tile] = scale[i];
+        if (entry < entries) chunk.scale[entry >> slot_shift][slot] = scale[i];
       }
       __syncwarp();
       if (lane == 0) barrier_arrive(bar(CHUNK_FULL + buffer));
@@ -646,37 +644,32 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   }
 }
 
-// Joins the parts of what was cut: a warp for each row and head.
+// Joins the parts of what was cut: a block for each row and head, whose warps take the parts in turn.
 constexpr int kJoinWarps = 4;
 __global__ void __launch_bounds__(kJoinWarps * 32)
 join_8bit_kernel(const float* __restrict__ parts, const int* __restrict__ positions, int num_rows, int heads, int kv_heads, int window,
-                 int teams, bf16* __restrict__ out, const float* __restrict__ sinks) {
+                 int table_keys, int teams, bf16* __restrict__ out, const float* __restrict__ sinks) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int row = blockIdx.y, head = blockIdx.x * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (head >= heads) return;
+  __shared__ float4 sums_of[kJoinWarps][32];
+  __shared__ float denominators[kJoinWarps];
+  const int row = blockIdx.y, head = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // all tiles, and those of the rows before this one
-  long long total = 0, before = 0;
+  unsigned total = 0, before = 0;
   for (int r = lane; r < num_rows; r += 32) {
-    const int tiles = row_at(positions, r, window).tiles;
+    const unsigned tiles = (unsigned)row_at(positions, r, window, table_keys).tiles;
     total += tiles;
-    before += r < row ? tiles : 0;
+    before += r < row ? tiles : 0u;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
+  total = __reduce_add_sync(0xffffffffu, total);
+  before = __reduce_add_sync(0xffffffffu, before);
   const int group = heads / kv_heads, group_tiles = (group + kHeads - 1) / kHeads, units = kv_heads * group_tiles;
-  const int tiles = row_at(positions, row, window).tiles;
-  if (tiles == 0) return;
-  const long long each = shares_of(total, teams);
+  const unsigned tiles = (unsigned)row_at(positions, row, window, table_keys).tiles;
+  if (tiles == 0u) return;
+  const unsigned each = shares_of(total, teams);
   const int heads_of_unit = min(group, kHeads);
   const int in_group = head % group, unit = head / group * group_tiles + in_group / kHeads, h = in_group % kHeads;
-  const long long first = before;
-  const bool small = total <= 0x7fffffffll;      // (a division of 64 bits takes far longer)
-  const int from = small ? (int)((unsigned)first / (unsigned)each) : (int)(first / each);
-  const int to = small ? (int)((unsigned)(first + tiles - 1) / (unsigned)each) : (int)((first + tiles - 1) / each);
+  const int from = (int)(before / each), to = (int)((before + tiles - 1u) / each);
   if (from == to) return;                              // one team had all of it
   auto place = [&](int team) { return parts + ((((size_t)team * units + unit) * 2 + (team == from ? 1 : 0)) * heads_of_unit + h) * (kDim + 2); };
   float top = -INFINITY;
@@ -687,14 +680,24 @@ join_8bit_kernel(const float* __restrict__ parts, const int* __restrict__ positi
   top = warp_max(top);
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
-#pragma unroll 8
-  for (int c = from; c <= to; ++c) {
+#pragma unroll 4
+  for (int c = from + warp; c <= to; c += kJoinWarps) {
     const float* p = place(c);
     const float2 ml = *reinterpret_cast<const float2*>(p + kDim);
     const float2 a = *reinterpret_cast<const float2*>(p + lane * 4), b = *reinterpret_cast<const float2*>(p + lane * 4 + 2);
     const float factor = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top);            // 0: no visible key (its values are zeros)
     sum += ml.y * factor;
     o.x += a.x * factor; o.y += a.y * factor; o.z += b.x * factor; o.w += b.y * factor;
+  }
+  sums_of[warp][lane] = o;
+  if (lane == 0) denominators[warp] = sum;
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWarps; ++w) {
+    const float4 theirs = sums_of[w][lane];
+    o.x += theirs.x; o.y += theirs.y; o.z += theirs.z; o.w += theirs.w;
+    sum += denominators[w];
   }
   if (sum != 0.0f && sinks != nullptr) sum += exp2f(sinks[head] * kLog2e - top);
   const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -742,6 +745,11 @@ int mir_attention_8bit_decode(const Attention8& a) {
     mir_set_error("%s: %d partitions are not a plan's for %d heads and %d kv heads", a.what, a.num_partitions, a.heads, a.cache.kv_heads);
     return MIR_BAD_ARGUMENT;
   }
+  const long long table_keys = std::min(0x7fffffffll, (long long)a.table_width * a.cache.page_size);
+  if ((long long)a.num_rows * (table_keys / kKeys + 1) > 0x7fffffffll) {
+    mir_set_error("%s: %d rows of up to %lld keys are more than one launch takes", a.what, a.num_rows, table_keys);
+    return MIR_BAD_ARGUMENT;
+  }
   const long long rows = (long long)a.cache.pages * a.cache.page_size, width = (long long)a.cache.kv_heads * kDim;
   CUtensorMap maps[4];
   const void* tensors[2] = {a.cache.k, a.cache.v};
@@ -752,6 +760,6 @@ int mir_attention_8bit_decode(const Attention8& a) {
   const int columns = std::min(group, kHeads);
   const int status = columns <= 4 ? launch<4>(a, maps) : (columns <= 8 ? launch<8>(a, maps) : launch<16>(a, maps));
   if (status != MIR_OK) return status;
-  return mir_launch("join_8bit", join_8bit_kernel, dim3((a.heads + kJoinWarps - 1) / kJoinWarps, a.num_rows), dim3(kJoinWarps * 32), 0, a.stream, 0, (const float*)a.scratch, a.positions,
-                    a.num_rows, a.heads, a.cache.kv_heads, a.window, a.num_partitions / units, (bf16*)a.out, a.sinks);
+  return mir_launch("join_8bit", join_8bit_kernel, dim3(a.heads, a.num_rows), dim3(kJoinWarps * 32), 0, a.stream, 0, (const float*)a.scratch, a.positions,
+                    a.num_rows, a.heads, a.cache.kv_heads, a.window, (int)table_keys, a.num_partitions / units, (bf16*)a.out, a.sinks);
 }
