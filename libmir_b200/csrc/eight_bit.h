@@ -42,3 +42,10 @@ int mir_attention_8bit_decode(const Attention8& a);
 // on the tensor cores (linear_8bit_tc.cu).
 int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, int scale_stride, const uint8_t* weight, const float* w_scales,
                           const void* bias, void* out, long long out_stride, int m, int n, int k, bool out_float, bool accumulate, cudaStream_t stream);
+// The same for up to 128 rows, bound by the weight's bytes (linear_8bit_few.cu): codes and scales as above, or, where `rounds` says so,
+// bf16 rows.
+bool mir_linear_8bit_few_takes(int m, int k);
+bool mir_linear_8bit_few_rounds(int m);
+int mir_linear_8bit_few(const uint8_t* codes, const float* scales, int scale_stride, const void* x, long long x_stride,
+                        const uint8_t* weight, const float* w_scales, const void* bias, void* out, long long out_stride, int m, int n, int k,
+                        bool out_float, bool accumulate, cudaStream_t stream);

@@ -80,86 +80,6 @@ quantize_weight_kernel(const T* __restrict__ weight, uint8_t* __restrict__ codes
   if (threadIdx.x == 0) scales[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = scale;
 }
 
-constexpr int kTile = 64, kStride = kBlock + 8;
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-// A tile of 64 rows and 64 columns of the result; codes are taken to float16 (exact) on their way into shared memory.
-__global__ void __launch_bounds__(128)
-linear_8bit_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_scales, int scale_stride, const uint8_t* __restrict__ weight,
-                   const float* __restrict__ w_scales, const void* __restrict__ bias, void* __restrict__ out, long long out_stride,
-                   int m, int n, int k, bool out_float, bool accumulate) {
-  __shared__ __align__(16) __half a_tile[kTile * kStride];
-  __shared__ __align__(16) __half b_tile[kTile * kStride];
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const int row0 = blockIdx.y * kTile, column0 = blockIdx.x * kTile;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int blocks = (k + kBlock - 1) / kBlock;
-  float total[kTile / 8][4] = {};
-  auto put = [&](__half* tile, const uint8_t* codes, int first, int limit, int block) {
-    for (int i = threadIdx.x; i < kTile * 8; i += 128) {
-      const int row = first + i / 8, column = block * kBlock + i % 8 * 16;
-      uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-      if (row < limit && column < k) raw = *reinterpret_cast<const uint4*>(codes + (size_t)row * k + column);
-      __half2* to = reinterpret_cast<__half2*>(tile + i / 8 * kStride + i % 8 * 16);
-      const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        to[2 * w] = e4m3_low(words[w]);
-        to[2 * w + 1] = e4m3_high(words[w]);
-      }
-    }
-  };
-  const int rows[2] = {row0 + warp * 16 + lane / 4, row0 + warp * 16 + lane / 4 + 8};
-  for (int block = 0; block < blocks; ++block) {
-    __syncthreads();
-    put(a_tile, x, row0, m, block);
-    put(b_tile, weight, column0, n, block);
-    __syncthreads();
-    float part[kTile / 8][4] = {};
-#pragma unroll
-    for (int kk = 0; kk < kBlock / 16; ++kk) {
-      uint32_t a[4];
-      const uint32_t at = smem_u32(a_tile + (warp * 16 + (lane & 15)) * kStride + kk * 16 + (lane >> 4) * 8);
-      asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(at));
-#pragma unroll
-      for (int c = 0; c < kTile / 8; ++c) {
-        const uint32_t* b = reinterpret_cast<const uint32_t*>(b_tile + (c * 8 + lane / 4) * kStride + kk * 16 + (lane & 3) * 2);
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(part[c][0]), "+f"(part[c][1]), "+f"(part[c][2]), "+f"(part[c][3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[4]));
-      }
-    }
-    const float w_scale = w_scales[(size_t)(column0 / kBlock) * blocks + block];
-    float scale[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) scale[i] = rows[i] < m ? x_scales[(size_t)block * scale_stride + rows[i]] * w_scale : 0.0f;
-#pragma unroll
-    for (int c = 0; c < kTile / 8; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) total[c][i] = fmaf(part[c][i], scale[i >> 1], total[c][i]);
-  }
-#pragma unroll
-  for (int c = 0; c < kTile / 8; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = rows[i >> 1], column = column0 + c * 8 + (lane & 3) * 2 + (i & 1);
-      if (row >= m || column >= n) continue;
-      float value = total[c][i];
-      const size_t at = (size_t)row * out_stride + column;
-      if (out_float) {
-        if (bias != nullptr) value += static_cast<const float*>(bias)[column];
-        float* to = static_cast<float*>(out) + at;
-        *to = accumulate ? *to + value : value;
-      } else {
-        if (bias != nullptr) value += __bfloat162float(static_cast<const bf16*>(bias)[column]);
-        static_cast<bf16*>(out)[at] = __float2bfloat16_rn(value);
-      }
-    }
-}
-
 }  // namespace
 
 // Scales of a block: one for each row, filled up to whole tiles of 128 rows.
@@ -191,7 +111,7 @@ MIR_EXPORT int mir_linear_8bit(const void* x, long long x_stride, const void* we
                                long long workspace_bytes, cudaStream_t stream) {
   if (m == 0 || n == 0) return MIR_OK;
   if (m < 0 || n < 0 || k <= 0 || (k % 16) || x_stride < k || (x_stride % 4) || out_stride < n || ((uintptr_t)x & 7) ||
-      ((uintptr_t)weight & 15) || (accumulate && !out_float) || (m + kTile - 1) / kTile > 65535) {
+      ((uintptr_t)weight & 15) || (accumulate && !out_float)) {
     mir_set_error("linear_8bit: takes columns in multiples of 16, rows of x on 8-byte boundaries and weights on 16-byte ones, "
                   "and accumulates into float32 (m %d, n %d, k %d, row strides %lld and %lld)", m, n, k, x_stride, out_stride);
     return MIR_BAD_ARGUMENT;
@@ -204,18 +124,21 @@ MIR_EXPORT int mir_linear_8bit(const void* x, long long x_stride, const void* we
   const int blocks = (k + kBlock - 1) / kBlock;
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   float* scales = reinterpret_cast<float*>(codes + ((size_t)m * k + 255) / 256 * 256);
-  const long long units = (long long)m * blocks;
-  if ((units + 7) / 8 > 0x7fffffffll) {
-    mir_set_error("linear_8bit: %d rows of %d columns are more than one launch takes", m, k);
-    return MIR_BAD_ARGUMENT;
+  // Up to 128 rows the weight's bytes are what takes the time, from there on the products.
+  const bool few = mir_linear_8bit_few_takes(m, k);
+  if (!few || !mir_linear_8bit_few_rounds(m)) {
+    const long long units = (long long)m * blocks;
+    if ((units + 7) / 8 > 0x7fffffffll) {
+      mir_set_error("linear_8bit: %d rows of %d columns are more than one launch takes", m, k);
+      return MIR_BAD_ARGUMENT;
+    }
+    const int status = mir_launch("quantize_rows_8bit", quantize_rows_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream, 0,
+                                  (const bf16*)x, x_stride, codes, scales, m, k, blocks, scale_stride_of(m));
+    if (status != MIR_OK) return status;
   }
-  const int status = mir_launch("quantize_rows_8bit", quantize_rows_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream, 0,
-                                (const bf16*)x, x_stride, codes, scales, m, k, blocks, scale_stride_of(m));
-  if (status != MIR_OK) return status;
-  if (m > 128)
-    return mir_linear_8bit_tiles(codes, scales, scale_stride_of(m), static_cast<const uint8_t*>(weight), w_scales, bias, out, out_stride, m, n, k,
-                                 out_float != 0, accumulate != 0, stream);
-  const dim3 grid((n + kTile - 1) / kTile, (m + kTile - 1) / kTile);
-  return mir_launch("linear_8bit", linear_8bit_kernel, grid, dim3(128), 0, stream, 0, codes, scales, scale_stride_of(m),
-                    (const uint8_t*)weight, w_scales, bias, out, out_stride, m, n, k, out_float != 0, accumulate != 0);
+  if (few)
+    return mir_linear_8bit_few(codes, scales, scale_stride_of(m), x, x_stride, static_cast<const uint8_t*>(weight), w_scales, bias, out,
+                               out_stride, m, n, k, out_float != 0, accumulate != 0, stream);
+  return mir_linear_8bit_tiles(codes, scales, scale_stride_of(m), static_cast<const uint8_t*>(weight), w_scales, bias, out, out_stride, m, n,
+                               k, out_float != 0, accumulate != 0, stream);
 }

@@ -155,7 +155,7 @@ def eight_bit_error() -> int:
     """0 unless a bounded wait of one of the tcgen05 kernels ran out (synchronises the device); such a kernel does no work from
     then on."""
     lib = library("eight_bit")
-    return int(lib.mir_decode_attention_8bit_error() or lib.mir_linear_8bit_tiles_error())
+    return int(lib.mir_decode_attention_8bit_error() or lib.mir_linear_8bit_tiles_error() or lib.mir_linear_8bit_few_error())
 
 
 def quantize_weight_8bit(weight: torch.Tensor) -> tuple:
@@ -171,6 +171,12 @@ def quantize_weight_8bit(weight: torch.Tensor) -> tuple:
     _check(lib, lib.mir_quantize_weight_8bit(int(weight.dtype == torch.bfloat16), weight.data_ptr(), values.data_ptr(),
                                              scales.data_ptr(), rows, columns, _stream()))
     return values, scales
+
+
+def set_linear_8bit_splits(splits: int) -> None:
+    """For measurements: over how many CTAs a product of up to 128 rows cuts K (1, 2, 4 or 8; 0: the launcher's rule)."""
+    lib = library("eight_bit")
+    _check(lib, lib.mir_linear_8bit_few_set_splits(int(splits)))
 
 
 def linear_8bit(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, out: torch.Tensor,
