@@ -24,19 +24,12 @@ constexpr int kRows = 128, kBlock = 128;
 constexpr int kWorkers = 128, kThreads = kWorkers + 64;     // four warps that round, scale and add; loader; issuer
 constexpr int kLoader = 4, kIssuer = 5;                     // warps
 constexpr int kMostStages = 6, kMostBlocks = 40;
-constexpr int kOwnRows = 16;                                // rows that the CTAs round themselves
+constexpr int kOwnRows = 16;                                // rows that the CTAs round themselves, a quarter of their blocks after the other
+constexpr int kQuarters = 4;
 
-enum { FULL = 0, EMPTY = FULL + kMostStages, SUM_FULL = EMPTY + kMostStages, SUM_FREE = SUM_FULL + 4, X_READY = SUM_FREE + 4, BARRIERS };
+enum { FULL = 0, EMPTY = FULL + kMostStages, SUM_FULL = EMPTY + kMostStages, SUM_FREE = SUM_FULL + 4, X_READY = SUM_FREE + 4, BARRIERS = X_READY + kQuarters };
 
 __device__ int g_error = 0;
-
-template <int N> __device__ __forceinline__ void tmem_columns(uint32_t address, float* v);
-template <> __device__ __forceinline__ void tmem_columns<16>(uint32_t address, float* v) {
-  float got[16];
-  tmem_load_16(address, got);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = got[i];
-}
 
 // N: columns of the products (rows of x, filled up).  OWN: x is bf16 and rounded here (N is 16 then), else it comes rounded.
 template <int N, bool OWN>
@@ -44,7 +37,7 @@ __global__ void __launch_bounds__(kThreads)
 linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const bf16* __restrict__ x,
                        long long x_stride, const float* __restrict__ x_scales, int scale_stride, const float* __restrict__ w_scales,
                        const void* __restrict__ bias, void* __restrict__ out, long long out_stride, int m, int n, int k, int splits,
-                       int per_split, int stages, int ring_bytes, bool out_float, bool accumulate) {
+                       int per_split, int stages, int ring_bytes, int x_block_bytes, bool out_float, bool accumulate) {
   constexpr int kBuffers = N <= 32 ? 4 : 2;
   constexpr uint32_t kColumns = (uint32_t)(kBuffers * N);
   constexpr int kChunk = 16;
@@ -52,21 +45,23 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
   __shared__ __align__(8) unsigned long long barriers[BARRIERS];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = blockIdx.x / splits, rank = blockIdx.x % splits;
-  const int blocks = (k + kBlock - 1) / kBlock, first = rank * per_split;
+  // without a cluster the CTAs walk over the tiles of 128 weight rows
+  const int first_tile = blockIdx.x / splits, tile_step = gridDim.x / splits, rank = blockIdx.x % splits;
+  const int tiles = (n + kRows - 1) / kRows, blocks = (k + kBlock - 1) / kBlock, first = rank * per_split;
   const int mine = max(0, min(blocks, first + per_split) - first);      // blocks of this CTA
   // shared memory: the ring (a block of weights, and of x where it comes rounded; in its place, when the products are over, the sums for
-  // the other ranks, [row of x][128]), x's own blocks, the scales
+  // the other ranks, [row of x][128]), x's own blocks (8 or 16 rows of 128 bytes; with 8 the products read what follows as the
+  // other columns, which nobody looks at), the rows' scales [block][N]
   const int stage_bytes = kRows * kBlock + (OWN ? 0 : N * kBlock);
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* own_x = smem + ring_bytes;
-  float* scales = reinterpret_cast<float*>(own_x + (OWN ? (size_t)per_split * N * kBlock : 0));       // [block][N], times the weight's
+  float* scales = reinterpret_cast<float*>(own_x + (OWN ? (size_t)per_split * x_block_bytes + 1024 : 0));
   float* sums = reinterpret_cast<float*>(smem);
   const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
   auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
   if (threadIdx.x == 0) {
     for (int i = 0; i < BARRIERS; ++i)
-      barrier_init(bar(i), i >= SUM_FREE && i < SUM_FREE + 4 ? 4u : (i == X_READY ? (uint32_t)kWorkers : 1u));
+      barrier_init(bar(i), i >= SUM_FREE && i < SUM_FREE + 4 ? 4u : (i >= X_READY ? (uint32_t)kWorkers : 1u));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kIssuer) {
@@ -84,8 +79,10 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
   if (warp == kLoader) {
     if (lane == 0 && go) {
       uint32_t stage = 0, parity = 0;
+      bool alive = true;
+      for (int tile = first_tile; tile < tiles && alive; tile += tile_step)
       for (int b = 0; b < mine; ++b) {
-        if (!wait_barrier(bar(EMPTY + (int)stage), parity ^ 1u)) { g_error = 1; break; }
+        if (!wait_barrier(bar(EMPTY + (int)stage), parity ^ 1u)) { g_error = 1; alive = false; break; }
         const uint32_t full = bar(FULL + (int)stage), to = smem_base + stage * (uint32_t)stage_bytes;
         barrier_expect_bytes(full, (uint32_t)stage_bytes);
         tma_load_2d(to, &w_map, full, (first + b) * kBlock, tile * kRows);
@@ -103,14 +100,16 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
         if (alive && !wait_barrier(bar(index), phase)) { g_error = 2; alive = false; }
       };
       uint32_t stage = 0, parity = 0, buffer = 0, buffer_parity = 0;
-      if (OWN) check(X_READY, 0u);
+      const int quarter = (mine + kQuarters - 1) / kQuarters;
+      for (int tile = first_tile; tile < tiles; tile += tile_step)
       for (int b = 0; b < mine; ++b) {
+        if (OWN && tile == first_tile && b % quarter == 0) check(X_READY + b / quarter, 0u);
         check(SUM_FREE + (int)buffer, buffer_parity ^ 1u);
         check(FULL + (int)stage, parity);
         __syncwarp();
         tensor_fence_after_sync();
         const uint32_t a = a0 + stage * (uint32_t)(stage_bytes >> 4);
-        const uint32_t c = OWN ? x0 + (uint32_t)b * (uint32_t)(N * kBlock >> 4) : a + (uint32_t)(kRows * kBlock >> 4);
+        const uint32_t c = OWN ? x0 + (uint32_t)b * (uint32_t)(x_block_bytes >> 4) : a + (uint32_t)(kRows * kBlock >> 4);
 #pragma unroll
         for (int kk = 0; kk < kBlock / 32; ++kk)
           mma_8bit_ss_halves(tmem + buffer * (uint32_t)N, a + 2u * kk, c + 2u * kk, idesc, kk > 0 ? 1u : 0u, elected);
@@ -122,97 +121,113 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
     }
   } else {
     // ------------------------------------------------------------------ workers
-    float total[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) total[i] = 0.0f;
-    const float* theirs = w_scales + (size_t)tile * blocks + first;
     if (OWN) {
-      // a warp rounds a row's block at a time, a lane four columns of it; rows that are not there are zeros
-      constexpr int kAhead = 4;
-      const int units = mine * kOwnRows;
-      for (int u0 = warp * kAhead; u0 < units; u0 += 4 * kAhead) {
-        uint2 raw[kAhead];
-        float w[kAhead];
+      // a warp rounds a row's block at a time, a lane four columns of it
+      constexpr int kAhead = 8;
+      const int quarter = (mine + kQuarters - 1) / kQuarters;
+      for (int q = 0; q < kQuarters; ++q) {
+        const int begin = min(mine, q * quarter) * m, end = min(mine, (q + 1) * quarter) * m;      // units: (block, row)
+        for (int u0 = begin + warp; u0 < end; u0 += 4 * kAhead) {
+          uint2 raw[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {               // (units is a multiple of kAhead)
-          const int block = (u0 + i) / kOwnRows, row = (u0 + i) % kOwnRows, column = (first + block) * kBlock + lane * 4;
-          raw[i] = make_uint2(0u, 0u);
-          if (row < m && column < k) raw[i] = *reinterpret_cast<const uint2*>(x + (size_t)row * x_stride + column);
-          w[i] = theirs[block];
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int block = (u0 + i) / kOwnRows, row = (u0 + i) % kOwnRows;
-          const float v[4] = {__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xffff0000u), __uint_as_float(raw[i].y << 16),
-                              __uint_as_float(raw[i].y & 0xffff0000u)};
-          uint32_t bits = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t magnitude = __float_as_uint(v[j]) & 0x7fffffffu;
-            if (magnitude < 0x7f800000u) bits = max(bits, magnitude);
+          for (int i = 0; i < kAhead; ++i) {
+            const int unit = u0 + 4 * i, block = unit / m, row = unit - block * m, column = (first + block) * kBlock + lane * 4;
+            raw[i] = make_uint2(0u, 0u);
+            if (unit < end && column < k) raw[i] = *reinterpret_cast<const uint2*>(x + (size_t)row * x_stride + column);
           }
-          bits = __reduce_max_sync(0xffffffffu, bits);
-          const int exponent = least_scale_exponent(__uint_as_float(bits));
-          const float inverse = power_of_two(-exponent);
-          *reinterpret_cast<uint32_t*>(own_x + (size_t)block * N * kBlock + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) =
-              to_e4m3x2(v[0] * inverse, v[1] * inverse) | (to_e4m3x2(v[2] * inverse, v[3] * inverse) << 16);
-          if (lane == 0) scales[block * N + row] = power_of_two(exponent) * w[i];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            const int unit = u0 + 4 * i, block = unit / m, row = unit - block * m;
+            if (unit >= end) break;
+            const float v[4] = {__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xffff0000u), __uint_as_float(raw[i].y << 16),
+                                __uint_as_float(raw[i].y & 0xffff0000u)};
+            uint32_t bits = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t magnitude = __float_as_uint(v[j]) & 0x7fffffffu;
+              if (magnitude < 0x7f800000u) bits = max(bits, magnitude);
+            }
+            bits = __reduce_max_sync(0xffffffffu, bits);
+            const int exponent = least_scale_exponent(__uint_as_float(bits));
+            const float inverse = power_of_two(-exponent);
+            *reinterpret_cast<uint32_t*>(own_x + (size_t)block * x_block_bytes + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) =
+                to_e4m3x2(v[0] * inverse, v[1] * inverse) | (to_e4m3x2(v[2] * inverse, v[3] * inverse) << 16);
+            if (lane == 0) scales[block * N + row] = power_of_two(exponent);
+          }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        barrier_arrive(bar(X_READY + q));
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      barrier_arrive(bar(X_READY));
     } else {
       for (int i = threadIdx.x; i < mine * N; i += kWorkers) {
         const int block = i / N, row = i % N;
-        scales[i] = row < m ? x_scales[(size_t)(first + block) * scale_stride + row] * theirs[block] : 0.0f;
+        scales[i] = row < m ? x_scales[(size_t)(first + block) * scale_stride + row] : 0.0f;
       }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory");
+    // a tile's scales, a block to a lane (40 at most), the next tile's ahead of their use
+    auto weight_scales = [&](int tile, float (&held)[2]) {
+      const float* theirs = w_scales + (size_t)min(tile, tiles - 1) * blocks;
+      held[0] = theirs[min(first + lane, blocks - 1)];
+      held[1] = theirs[min(first + 32 + lane, blocks - 1)];
+    };
+    float held[2], next[2];
+    weight_scales(first_tile, held);
     bool alive = go;
     uint32_t buffer = 0, buffer_parity = 0;
     const uint32_t lane_bits = (uint32_t)(warp * 32) << 16;
-    for (int b = 0; b < mine; ++b) {
-      if (alive && !wait_barrier(bar(SUM_FULL + (int)buffer), buffer_parity)) { g_error = 3; alive = false; }
-      __syncwarp();
-      tensor_fence_after_sync();
-      const uint32_t from = tmem + buffer * (uint32_t)N + lane_bits;
+    for (int tile = first_tile; tile < tiles; tile += tile_step) {
+      weight_scales(tile + tile_step, next);
+      float total[N];
 #pragma unroll
-      for (int c = 0; c < N; c += kChunk) {
-        float v[kChunk];
-        tmem_columns<kChunk>(from + (uint32_t)c, v);
-        if (c + kChunk == N) {                                // all of this warp's columns are in registers
-          tensor_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) barrier_arrive(bar(SUM_FREE + (int)buffer));
-        }
+      for (int i = 0; i < N; ++i) total[i] = 0.0f;
+      for (int b = 0; b < mine; ++b) {
+        const float w_scale = __shfl_sync(0xffffffffu, b < 32 ? held[0] : held[1], b & 31);
+        if (alive && !wait_barrier(bar(SUM_FULL + (int)buffer), buffer_parity)) { g_error = 3; alive = false; }
+        __syncwarp();
+        tensor_fence_after_sync();
+        const uint32_t from = tmem + buffer * (uint32_t)N + lane_bits;
 #pragma unroll
-        for (int i = 0; i < kChunk; i += 4) {
-          const float4 factor = *reinterpret_cast<const float4*>(scales + b * N + c + i);
-          total[c + i] = fmaf(v[i], factor.x, total[c + i]);
-          total[c + i + 1] = fmaf(v[i + 1], factor.y, total[c + i + 1]);
-          total[c + i + 2] = fmaf(v[i + 2], factor.z, total[c + i + 2]);
-          total[c + i + 3] = fmaf(v[i + 3], factor.w, total[c + i + 3]);
+        for (int c = 0; c < N; c += kChunk) {
+          float v[kChunk];
+          tmem_load_16(from + (uint32_t)c, v);
+          if (c + kChunk == N) {                              // all of this warp's columns are in registers
+            tensor_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(bar(SUM_FREE + (int)buffer));
+          }
+#pragma unroll
+          for (int i = 0; i < kChunk; i += 4) {
+            // (a row's scale is a power of two: only the addition rounds, and the product with the weight's scale)
+            const float4 x_scale = *reinterpret_cast<const float4*>(scales + b * N + c + i);
+            total[c + i] = fmaf(v[i] * x_scale.x, w_scale, total[c + i]);
+            total[c + i + 1] = fmaf(v[i + 1] * x_scale.y, w_scale, total[c + i + 1]);
+            total[c + i + 2] = fmaf(v[i + 2] * x_scale.z, w_scale, total[c + i + 2]);
+            total[c + i + 3] = fmaf(v[i + 3] * x_scale.w, w_scale, total[c + i + 3]);
+          }
         }
+        if (++buffer == (uint32_t)kBuffers) { buffer = 0; buffer_parity ^= 1u; }
       }
-      if (++buffer == (uint32_t)kBuffers) { buffer = 0; buffer_parity ^= 1u; }
-    }
-    const int column = tile * kRows + threadIdx.x;
-    if (splits > 1) {
+      held[0] = next[0];
+      held[1] = next[1];
+      const int column = tile * kRows + threadIdx.x;
+      if (splits > 1) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i < m) sums[i * kRows + threadIdx.x] = total[i];
-    } else if (column < n && alive) {
-      const float extra = bias == nullptr ? 0.0f : (out_float ? static_cast<const float*>(bias)[column]
-                                                              : __bfloat162float(static_cast<const bf16*>(bias)[column]));
+        for (int i = 0; i < N; ++i)
+          if (i < m) sums[i * kRows + threadIdx.x] = total[i];
+      } else if (column < n && alive) {
+        const float extra = bias == nullptr ? 0.0f : (out_float ? static_cast<const float*>(bias)[column]
+                                                                : __bfloat162float(static_cast<const bf16*>(bias)[column]));
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i >= m) continue;
-        const size_t at = (size_t)i * out_stride + column;
-        if (out_float) {
-          float* to = static_cast<float*>(out) + at;
-          *to = accumulate ? *to + (total[i] + extra) : total[i] + extra;
-        } else {
-          static_cast<bf16*>(out)[at] = __float2bfloat16_rn(total[i] + extra);
+        for (int i = 0; i < N; ++i) {
+          if (i >= m) continue;
+          const size_t at = (size_t)i * out_stride + column;
+          if (out_float) {
+            float* to = static_cast<float*>(out) + at;
+            *to = accumulate ? *to + (total[i] + extra) : total[i] + extra;
+          } else {
+            static_cast<bf16*>(out)[at] = __float2bfloat16_rn(total[i] + extra);
+          }
         }
       }
     }
@@ -222,7 +237,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
     // the ranks' sums, added in rank order: rank r finishes the rows r, r + splits, ...
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    const int column = tile * kRows + threadIdx.x;
+    const int column = first_tile * kRows + threadIdx.x;
     if (threadIdx.x < kWorkers && column < n && go) {
       const float extra = bias == nullptr ? 0.0f : (out_float ? static_cast<const float*>(bias)[column]
                                                               : __bfloat162float(static_cast<const bf16*>(bias)[column]));
@@ -256,11 +271,34 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
   }
 }
 
+// How a call is cut: K over `splits` CTAs of a cluster, and `ctas` of them on an SM.
+struct Cut {
+  int splits, per_split, stages, ring_bytes, x_block_bytes, bytes, ctas;
+};
+Cut cut_for(int m, int n_columns, bool own, int blocks, int splits) {
+  Cut c;
+  c.splits = splits;
+  c.per_split = (blocks + splits - 1) / splits;
+  c.x_block_bytes = own ? (m <= 8 ? 8 : 16) * kBlock : 0;
+  const int stage_bytes = kRows * kBlock + (own ? 0 : n_columns * kBlock);
+  const int sums = splits > 1 ? (m * kRows * 4 + 1023) / 1024 * 1024 : 0;
+  const int rest = 1024 + (own ? c.per_split * c.x_block_bytes + 1024 : 0) + c.per_split * n_columns * 4;
+  // three CTAs an SM where that leaves each a ring of three stages, else two
+  for (c.ctas = n_columns <= 32 ? 3 : 2; c.ctas >= 1; --c.ctas) {          // (registers: two with more columns)
+    const int budget = kSharedOfSm / c.ctas - 1024 - 512;
+    c.stages = std::min({c.per_split, kMostStages, (budget - rest) / stage_bytes});
+    if (rest + sums <= budget && (c.stages >= std::min(3, c.per_split) || c.ctas == 1)) break;
+  }
+  c.ring_bytes = std::max(c.stages * stage_bytes, sums);
+  c.bytes = std::max(rest + c.ring_bytes, kLeastSharedBeside);      // (no less than keeps it off an SM whose tensor memory is all taken)
+  return c;
+}
+
 template <int N, bool OWN>
 int launch(const uint8_t* codes, const float* scales, int scale_stride, const void* x, long long x_stride, const uint8_t* weight,
            const float* w_scales, const void* bias, void* out, long long out_stride, int m, int n, int k, bool out_float, bool accumulate,
-           int splits, cudaStream_t stream) {
-  const int blocks = (k + kBlock - 1) / kBlock, tiles = (n + kRows - 1) / kRows, per_split = (blocks + splits - 1) / splits;
+           int forced, cudaStream_t stream) {
+  const int blocks = (k + kBlock - 1) / kBlock, tiles = (n + kRows - 1) / kRows;
   CUtensorMap w_map, x_map;
   int status = tensor_map_of_bytes(weight, n, k, k, kRows, &w_map);
   if (status != MIR_OK) return status;
@@ -269,18 +307,21 @@ int launch(const uint8_t* codes, const float* scales, int scale_stride, const vo
     status = tensor_map_of_bytes(codes, m, k, k, N, &x_map);
     if (status != MIR_OK) return status;
   }
-  const int stage_bytes = kRows * kBlock + (OWN ? 0 : N * kBlock);
-  // 96 KB of ring at most: two CTAs fit on an SM
-  const int stages = std::min(per_split, kMostStages * kRows * kBlock / stage_bytes);
-  const int ring_bytes = std::max(stages * stage_bytes, splits > 1 ? (m * kRows * 4 + 1023) / 1024 * 1024 : 0);
-  const int bytes = 1024 + ring_bytes + per_split * N * (OWN ? kBlock : 0) + per_split * N * 4;
-  // (no less than what keeps a kernel that takes all tensor memory from landing beside it)
-  const int reserved = std::max(bytes, kLeastSharedBeside);
-  status = reserve_shared(linear_8bit_few_kernel<N, OWN>, reserved, "linear_8bit");
+  // the most CTAs that are all there at once, two blocks each at least; with more tiles than that they walk over the tiles
+  Cut cut = cut_for(m, N, OWN, blocks, 1);
+  for (int splits = 8; splits >= 1; splits /= 2) {
+    if (forced > 0 && splits != forced) continue;
+    cut = cut_for(m, N, OWN, blocks, splits);
+    if (cut.per_split > kMostBlocks) { cut = cut_for(m, N, OWN, blocks, std::min(8, splits * 2)); break; }
+    if (splits == 1 || forced > 0 || ((long long)tiles * splits <= (long long)cut.ctas * mir_sm_count() && blocks >= 2 * splits)) break;
+  }
+  status = reserve_shared(linear_8bit_few_kernel<N, OWN>, cut.bytes, "linear_8bit");
   if (status != MIR_OK) return status;
-  return mir_launch_cluster(mir_pdl_enabled(), "linear_8bit_few", linear_8bit_few_kernel<N, OWN>, dim3((unsigned)tiles * splits),
-                            dim3(kThreads), (size_t)reserved, stream, dim3(splits, 1, 1), w_map, x_map, (const bf16*)x, x_stride, scales,
-                            scale_stride, w_scales, bias, out, out_stride, m, n, k, splits, per_split, stages, ring_bytes, out_float, accumulate);
+  const int walkers = cut.splits > 1 ? tiles : std::min(tiles, cut.ctas * mir_sm_count());
+  return mir_launch_cluster(mir_pdl_enabled(), "linear_8bit_few", linear_8bit_few_kernel<N, OWN>, dim3((unsigned)walkers * cut.splits),
+                            dim3(kThreads), (size_t)cut.bytes, stream, dim3(cut.splits, 1, 1), w_map, x_map, (const bf16*)x, x_stride, scales,
+                            scale_stride, w_scales, bias, out, out_stride, m, n, k, cut.splits, cut.per_split, cut.stages, cut.ring_bytes,
+                            cut.x_block_bytes, out_float, accumulate);
 }
 
 int g_forced_splits = 0;          // for measurements (0: the launcher chooses)
@@ -302,13 +343,8 @@ bool mir_linear_8bit_few_rounds(int m) { return m <= kOwnRows; }
 int mir_linear_8bit_few(const uint8_t* codes, const float* scales, int scale_stride, const void* x, long long x_stride,
                         const uint8_t* weight, const float* w_scales, const void* bias, void* out, long long out_stride, int m, int n, int k,
                         bool out_float, bool accumulate, cudaStream_t stream) {
-  const int blocks = (k + kBlock - 1) / kBlock, tiles = (n + kRows - 1) / kRows;
-  int splits = 1;
-  while (splits < 8 && tiles * splits < 2 * mir_sm_count() && blocks >= 4 * splits) splits *= 2;
-  if (g_forced_splits > 0) splits = g_forced_splits;
-  while (splits < 8 && (blocks + splits - 1) / splits > kMostBlocks) splits *= 2;
 #define MIR_FEW(N, OWN) \
-  launch<N, OWN>(codes, scales, scale_stride, x, x_stride, weight, w_scales, bias, out, out_stride, m, n, k, out_float, accumulate, splits, stream)
+  launch<N, OWN>(codes, scales, scale_stride, x, x_stride, weight, w_scales, bias, out, out_stride, m, n, k, out_float, accumulate, g_forced_splits, stream)
   if (m <= kOwnRows) return MIR_FEW(16, true);
   if (m <= 32) return MIR_FEW(32, false);
   if (m <= 64) return MIR_FEW(64, false);
