@@ -416,5 +416,5 @@ MIR_EXPORT int mir_prefill_attention_8bit(const void* q, long long q_stride, voi
   a.sinks = sinks; a.stream = stream;
   if (attention_8bit_refused(a, tokens, false)) return MIR_BAD_ARGUMENT;
   if (num_rows == 0 || tokens == 0) return MIR_OK;
-  return mir_attention_8bit_general(a, tokens);
+  return mir_decode_8bit_takes(head_dim, page_size) ? mir_attention_8bit_prefill(a, tokens) : mir_attention_8bit_general(a, tokens);
 }

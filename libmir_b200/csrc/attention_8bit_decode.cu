@@ -103,13 +103,6 @@ template <int N> __device__ __forceinline__ void tmem_store(uint32_t address, co
 __device__ __forceinline__ uint32_t swizzled(int row, int column) {
   return (uint32_t)(row * 128 + (((column >> 4) ^ (row & 7)) << 4) + (column & 15));
 }
-// Two numbers within 448 as e4m3 and what that leaves as e5m2 (the first in the low bytes).
-__device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = to_e4m3x2(a, b);
-  const float2 taken = __half22float2(e4m3_low(hi));
-  lo = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a - taken.x, b - taken.y), __NV_SATFINITE, __NV_E5M2);
-}
-
 // A row's share of the work: its tiles of keys, from the tile that holds its first visible key to the last that the table can have
 // (one at least: a row that sees nothing gets zeros).  All rows' tiles together are below 2^31: the launcher checks.
 struct Row {
@@ -372,8 +365,8 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
           const int e = least_scale_exponent(fminf(largest, 3.38953139e38f));
           const float inverse = power_of_two(-e);
           uint32_t hi[2], lo[2];
-          split(x[0] * inverse, x[1] * inverse, hi[0], lo[0]);
-          split(x[2] * inverse, x[3] * inverse, hi[1], lo[1]);
+          split_e4m3_e5m2(x[0] * inverse, x[1] * inverse, hi[0], lo[0]);
+          split_e4m3_e5m2(x[2] * inverse, x[3] * inverse, hi[1], lo[1]);
           unsigned char* to = smem + L::kOffQ + parity * 2 * kPart + swizzled(h, lane * 4);
           *reinterpret_cast<uint32_t*>(to) = hi[0] | (hi[1] << 16);
           *reinterpret_cast<uint32_t*>(to + kPart) = lo[0] | (lo[1] << 16);
@@ -586,7 +579,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
             w[i] = visible ? approximate_exp2(s[h + i] + shift_v - top_weight[h + i]) : 0.0f;
           }
           uint32_t hi, lo;
-          split(w[0], w[1], hi, lo);
+          split_e4m3_e5m2(w[0], w[1], hi, lo);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             unsigned char* to = p_smem + swizzled(h + i, r);

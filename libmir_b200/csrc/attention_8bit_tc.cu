@@ -1,0 +1,647 @@
+// Causal attention of portions over the 8-bit cache on the 5th-generation tensor cores, head_dim 128, pages of 8 to 128 keys:
+//
+//   out = sum_j p_j S_v[page of j] V_j / sum_j p_j,   p_j = exp(scale q . (S_k[page of j] K_j) - reference)
+//
+// A row is a (token, query head of the kv head's group) pair, a work item 128 rows of one request and kv head (and one partition of
+// the keys, where few items are split): the heads of a group share the tiles of keys, and a short portion still fills a tile.
+// A CTA per SM walks over items, heaviest first; every ring and barrier runs on across them.  Per tile of 128 keys:
+//
+//   S = Q K^T     kind::f8f6f4, K as the cache holds it, Q in two parts q = hi + lo, hi = e4m3(q 2^-e), lo = e5m2 of what hi leaves (a
+//                 bf16 number's eight significant bits fit into the two; off by at most 2^-25 of the row's largest element);
+//   P = exp2(S S_k scale log2 e - reference), rounded to bf16, over the scores in tensor memory;
+//   O += P V      kind::f16, V as bf16: an e4m3 number times a power of two is exact in bf16, so the page's scale is in it.
+//
+// K needs no conversion, V four instructions for two elements: a byte's sign is spread over 16 bits (prmt), shifted by 4 and masked,
+// which is the bf16 number of the same exponent field, 2^-120 times the e4m3 one (subnormals too); a product in bf16 with 2^120
+// times the page's scale puts that right.  Both products take as long as they would in bf16; the schedulers' slots bound the kernel.
+//
+// Roles: a scout reads block table and scales ahead and leaves them in shared memory; two loaders (TMA) for keys and values; an
+// issuer; four warps that split queries and widen values; two streams of eight softmax warps that take the tiles in turn, with a
+// running reference that they hand to each other (raised when a tile's maximum exceeds it by 2^8), three score accumulators and
+// one for the output, which a stream that raises the reference rescales when the product of the tile before is over.
+// A hidden key's score becomes -inf by selection; rows of values that no query of the item sees are written as zeros.
+#include <algorithm>
+#include "eight_bit_tc.cuh"
+
+using namespace mir;
+using namespace mir::tc;
+typedef __nv_bfloat16 bf16;
+
+namespace {
+
+constexpr int kRows = 128, kKeys = 128, kDim = 128;
+constexpr int kTile8 = kKeys * kDim;                        // bytes of a tile of keys, values or query parts as they are
+constexpr int kHalf = 128 * 128, kTile16 = 2 * kHalf;       // bytes of a tile of bf16 values: two halves of 64 elements
+constexpr int kKeyStages = 3, kRawStages = 3, kValueStages = 2, kInfos = 8, kSlots = 16;
+constexpr int kOffQ = 0, kOffK = 2 * kTile8, kOffRaw = kOffK + kKeyStages * kTile8, kOffV = kOffRaw + kRawStages * kTile8;
+constexpr int kSmemBytes = kOffV + kValueStages * kTile16 + 1024;
+static_assert(kSmemBytes + kLeastSharedBeside > kSharedOfSm, "no other kernel with tensor memory beside this one");
+constexpr int kParts = 2, kCols = kKeys / kParts;           // softmax threads of a row and stream; columns of each
+constexpr int kStreams = 2, kStreamThreads = kRows * kParts;
+enum { kKeyLoader = 0, kIssuer = 1, kValueLoader = 2, kScout = 3, kFirstConverter = 4, kFirstSoftmax = 8 };      // warps
+constexpr int kConverters = 128, kThreads = (kFirstSoftmax + 8 * kStreams) * 32;
+// launched with 80 registers a thread (6 * 80 = 480); the first eight warps give some up: 40 + 56 + 4 * 96 = 480
+constexpr int kRoleRegisters = 40, kConverterRegisters = 56, kSoftmaxRegisters = 96;
+static_assert(kRoleRegisters + kConverterRegisters + 4 * kSoftmaxRegisters <= 6 * 80, "no more registers than the launch holds");
+constexpr uint32_t kTmemColumns = 512;                      // S at 0, 128, 256; O at 384
+constexpr float kRises = 8.0f;
+
+// Tiles are counted over a CTA's items (g), items with tiles too (n).  Three stages: g % 3, phase g / 3; two: g & 1, g >> 1.
+// Q_FULL goes by n & 3: the softmax may begin item n when the queries of the items behind it are there already.
+enum { Q_FULL = 0, Q_FREE = Q_FULL + 4, K_FULL, K_FREE = K_FULL + 3, RAW_FULL = K_FREE + 3, RAW_FREE = RAW_FULL + 3, V_FULL = RAW_FREE + 3,
+       V_FREE = V_FULL + 2, S_FULL = V_FREE + 2, P_READY = S_FULL + 3, REF_READY = P_READY + 3, PV_DONE = REF_READY + 2,
+       ITEM_DONE = PV_DONE + 2, O_FREE, INFO_FULL, INFO_FREE = INFO_FULL + kInfos, BARRIERS = INFO_FREE + kInfos };
+
+__device__ int g_error = 0;
+
+__device__ __forceinline__ float warp_largest(float v) {
+  float top;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(v));
+  return top;
+}
+
+// What the scout leaves of a tile: each page's first row of the cache (below 0: not there, or no query of the item sees it), its scales.
+struct Info {
+  int row[kSlots];
+  float k_scale[kSlots], v_scale[kSlots];
+  int whole;                                                // all pages are there
+};
+
+struct Work {
+  int request, kv_head, part, first_row, rows, first_token, first_position, last_position, first_key, begin, end, tiles;
+};
+
+struct Items {
+  const int* query_starts;
+  const int* context_lens;
+  int num_rows, kv_heads, group, window, partition, num_partitions, row_tiles, count;
+  // Item `index`: the kv head is the fast index, then the partition, then the batch's tiles of rows from the last one of the last request
+  // backwards (late tiles see the most keys and come first).  False beyond the last item.
+  __device__ __forceinline__ bool at(int index, Work& w) const {
+    if (index < 0 || index >= count) return false;
+    w.kv_head = index % kv_heads;
+    const int rest = index / kv_heads;
+    w.part = rest % num_partitions;
+    int remaining = row_tiles - 1 - rest / num_partitions;
+    w.request = -1;
+    int tokens = 0;
+    for (int r = 0; r < num_rows; ++r) {
+      tokens = query_starts[r + 1] - query_starts[r];
+      const int tiles = (tokens * group + kRows - 1) / kRows;
+      if (remaining < tiles) { w.request = r; break; }
+      remaining -= tiles;
+    }
+    if (w.request < 0) return false;
+    w.first_row = remaining * kRows;
+    w.rows = min(kRows, tokens * group - w.first_row);
+    w.first_token = query_starts[w.request];
+    const int start = context_lens[w.request] - tokens;
+    w.first_position = start + w.first_row / group;
+    w.last_position = start + (w.first_row + w.rows - 1) / group;
+    w.first_key = (window > 0 && w.first_position >= window) ? w.first_position + 1 - window : 0;
+    w.begin = max(w.first_key / kKeys * kKeys, w.part * partition);
+    w.end = (int)min((long long)w.last_position + 1, (long long)(w.part + 1) * partition);
+    w.tiles = w.end > w.begin ? (w.end - w.begin + kKeys - 1) / kKeys : 0;
+    return true;
+  }
+};
+
+// The k-th item of CTA `cta`: rounds are dealt out back and forth, so that the CTA with a round's heaviest item gets the next one's lightest.
+__device__ __forceinline__ int item_of(int k, int cta, int ctas) { return k * ctas + ((k & 1) ? ctas - 1 - cta : cta); }
+
+struct Counter {                                            // stage and phase of a ring
+  uint32_t stage = 0, phase = 0;
+  __device__ __forceinline__ void step(uint32_t stages) {
+    if (++stage == stages) { stage = 0; phase ^= 1u; }
+  }
+};
+
+// Two e4m3 numbers (bytes `selector` of `word`, spread with their signs) as bf16 numbers 2^-120 times as large.
+template <uint32_t SELECTOR> __device__ __forceinline__ uint32_t lifted(uint32_t word) {
+  uint32_t spread;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(spread) : "r"(word), "n"(SELECTOR));
+  return (spread << 4) & 0x87f087f0u;
+}
+__device__ __forceinline__ uint32_t times(uint32_t pair, uint32_t factor) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(pair), "r"(factor));
+  return d;
+}
+// bf16 pair of 2^e, e from -126 to 127.
+__device__ __forceinline__ uint32_t power_pair(int e) { return (uint32_t)(e + 127) << 7 | (uint32_t)(e + 127) << 23; }
+
+struct Handoff {
+  bool has_from;
+  uint32_t from_barrier, from_phase, to_barrier;
+  const float* from;
+  float* to;
+};
+
+// One tile of the softmax for this thread's kCols columns of its row, from column `first` on: the scores, times their pages' scales; the hidden
+// ones (outside low .. high, or of pages that are not there) -inf; the row's maximum with the thread that has the other columns; the
+// reference, which comes from the tile before and goes to the next; the weights, packed to bf16.  Returns their sum.
+template <bool MASKED>
+__device__ __forceinline__ float softmax_tile(uint32_t scores, int first, int low, int high, float scale, const Info& info, int shift,
+                                              float& reference, float& factor, bool& grow, float& own_factor, uint32_t (&packed)[kCols / 2],
+                                              float* shared_max, int part, int team, const Handoff& handoff, bool& alive) {
+  uint32_t raw[2][32];
+  tmem_load_32_ahead(scores + (uint32_t)first, raw[0]);
+  tmem_load_32_ahead(scores + (uint32_t)first + 32u, raw[1]);
+  tmem_load_done(raw[0]);
+  tmem_load_done(raw[1]);
+  float v[kCols];
+#pragma unroll
+  for (int c8 = 0; c8 < kCols / 8; ++c8) {                  // (a page has eight keys or more)
+    const int slot = (first + c8 * 8) >> shift;
+    const float k_scale = info.k_scale[slot] * scale;
+    const bool there = !MASKED || info.row[slot] >= 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = c8 * 8 + i;
+      v[c] = __uint_as_float(raw[c / 32][c % 32]) * k_scale;
+      if (MASKED) v[c] = there && c >= low - first && c <= high - first ? v[c] : -INFINITY;
+    }
+  }
+  float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) best[c & 3] = fmaxf(best[c & 3], v[c]);
+  float maximum = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+  shared_max[part * kRows] = maximum;
+  asm volatile("bar.sync %0, %1;" ::"r"(team), "n"(32 * kParts) : "memory");
+#pragma unroll
+  for (int other = 0; other < kParts; ++other) maximum = fmaxf(maximum, shared_max[other * kRows]);
+  float before = -INFINITY;
+  if (handoff.has_from) {
+    if (alive && !wait_barrier(handoff.from_barrier, handoff.from_phase)) { g_error = 3; alive = false; }
+    before = *handoff.from;
+  }
+  const float now = maximum > before + kRises ? maximum : before;
+  if (part == 0) *handoff.to = now;
+  barrier_arrive(handoff.to_barrier);
+  grow = now != before;
+  factor = grow ? approximate_exp2(before - now) : 1.0f;                  // 0 when nothing was seen before
+  own_factor = reference == now ? 1.0f : approximate_exp2(reference - now);
+  reference = now;
+  const float down = (MASKED && reference == -INFINITY) ? 0.0f : -reference;       // (a row that has seen nothing yet)
+  float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < kCols; c += 2) {
+    const float p0 = approximate_exp2(v[c] + down), p1 = approximate_exp2(v[c + 1] + down);
+    sums[(c >> 1) & 3] += p0 + p1;
+    const __nv_bfloat162 both = __floats2bfloat162_rn(p0, p1);
+    packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&both);
+  }
+  return (sums[0] + sums[1]) + (sums[2] + sums[3]);
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                    const __grid_constant__ CUtensorMap k_tile_map, const __grid_constant__ CUtensorMap v_tile_map, const bf16* __restrict__ q,
+                    long long q_stride, Cache8 cache, const int* __restrict__ block_table, int table_width,
+                    const int* __restrict__ query_starts, const int* __restrict__ context_lens, int num_rows, int heads, float scale_log2,
+                    int window, int partition, int num_partitions, float* __restrict__ partial_o, float* __restrict__ partial_ml,
+                    bf16* __restrict__ out, const float* __restrict__ sinks) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) unsigned long long barriers[BARRIERS];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int row_tiles_slot;
+  __shared__ Info infos[kInfos];
+  __shared__ float row_scales[4][kRows];                    // by n & 3: a row's scale, log2 e and the power of two taken out of its queries
+  __shared__ float exchange[kStreams][2][kParts][kRows];    // [stream][its tile's parity][part]: a row's maxima
+  __shared__ float denominators[2][kStreams][kParts][kRows];
+  __shared__ float references[2][kStreams][kRows];
+  __shared__ float handed[2][kRows];                        // a row's reference after tile g, by g & 1
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
+  auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
+  const int group = heads / cache.kv_heads;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < BARRIERS; ++i) {
+      uint32_t count = 1u;
+      if ((i >= Q_FULL && i < Q_FULL + 4) || (i >= V_FULL && i < V_FULL + 2) || (i >= RAW_FREE && i < RAW_FREE + 3)) count = kConverters;
+      if ((i >= P_READY && i < P_READY + 3) || i == REF_READY || i == REF_READY + 1) count = kStreamThreads;
+      if (i == O_FREE) count = kStreamThreads * kStreams;
+      barrier_init(bar(i), count);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kIssuer) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  grid_dependency_wait();
+  if (threadIdx.x == 0) {
+    int total = 0;
+    for (int r = 0; r < num_rows; ++r) total += ((query_starts[r + 1] - query_starts[r]) * group + kRows - 1) / kRows;
+    if (*reinterpret_cast<volatile int*>(&g_error) != 0) total = 0;       // an earlier wait ran out: nothing is begun
+    row_tiles_slot = total;
+  }
+  tensor_fence_before_sync();
+  __syncthreads();
+  tensor_fence_after_sync();
+  grid_launch_dependents();
+  const uint32_t tmem = tmem_slot, tmem_o = tmem + 384u;
+  const int shift = 31 - __clz(cache.page_size);            // pages are powers of two
+  const Items items{query_starts, context_lens, num_rows, cache.kv_heads, group, window, partition, num_partitions, row_tiles_slot,
+                    row_tiles_slot * cache.kv_heads * num_partitions};
+  const int cta = blockIdx.x, ctas = gridDim.x;
+  auto more = [&](int k) { return (long long)k * ctas < items.count; };
+  Work w;
+
+  if (warp < kFirstConverter) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegisters));
+    if (warp == kScout) {
+      // ---------------------------------------------------------------- scout: two tiles at a time, half a warp each
+      const int half = lane >> 4, slot = lane & 15, slots = kKeys >> shift;
+      bool alive = true;
+      int g = 0;
+      for (int k = 0; more(k); ++k) {
+        if (!items.at(item_of(k, cta, ctas), w)) continue;
+        const int* table = block_table + (size_t)w.request * table_width;
+        for (int t = 0; t < w.tiles; t += 2) {
+          const int tile = t + half, key = w.begin + tile * kKeys + (slot << shift);
+          int page = -1;
+          if (slot < slots && tile < w.tiles && key < w.end && key + cache.page_size > w.first_key)
+            page = page_of_block(table, table_width, key >> shift, cache.pages);
+          float k_scale = 1.0f, v_scale = 1.0f;
+          if (page >= 0) {
+            k_scale = cache.k_scales[(size_t)page * cache.kv_heads + w.kv_head];
+            v_scale = cache.v_scales[(size_t)page * cache.kv_heads + w.kv_head];
+          }
+          const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+          for (int i = 0; i < 2 && t + i < w.tiles; ++i) {
+            const int info = (g + i) % kInfos;
+            if (alive && !wait_barrier(bar(INFO_FREE + info), (uint32_t)((g + i) / kInfos & 1) ^ 1u)) { g_error = 1; alive = false; }
+            __syncwarp();
+            if (half == i) {
+              infos[info].row[slot] = page >= 0 ? page << shift : -cache.page_size;
+              infos[info].k_scale[slot] = k_scale;
+              infos[info].v_scale[slot] = v_scale;
+            }
+            if (lane == 0) infos[info].whole = __popc((there >> (16 * i)) & 0xffffu) == slots;
+            __syncwarp();
+            if (lane == 0) barrier_arrive(bar(INFO_FULL + info));
+          }
+          g += min(2, w.tiles - t);
+        }
+      }
+    } else if (warp == kKeyLoader || warp == kValueLoader) {
+      // ---------------------------------------------------------------- loaders: lane l has page slot l
+      const bool values = warp == kValueLoader;
+      const bool loads = lane < (kKeys >> shift);
+      const uint32_t box_bytes = (uint32_t)cache.page_size * kDim;
+      const uint32_t base = smem_base + (uint32_t)(values ? kOffRaw : kOffK);
+      const int full0 = values ? RAW_FULL : K_FULL, free0 = values ? RAW_FREE : K_FREE;
+      bool alive = true;
+      Counter ring;
+      int g = 0;
+      for (int k = 0; more(k) && alive; ++k) {
+        if (!items.at(item_of(k, cta, ctas), w)) continue;
+        for (int t = 0; t < w.tiles; ++t, ++g) {
+          const int info = g % kInfos;
+          if (!wait_barrier(bar(INFO_FULL + info), (uint32_t)(g / kInfos & 1))) { g_error = 1; alive = false; }
+          const int cache_row = loads ? infos[info].row[lane] : 0;
+          if (alive && !wait_barrier(bar(free0 + (int)ring.stage), ring.phase ^ 1u)) { g_error = 1; alive = false; }
+          alive = __all_sync(0xffffffffu, alive);
+          if (!alive) break;
+          const int first_row = __shfl_sync(0xffffffffu, cache_row, 0);
+          const bool in_a_row = first_row >= 0 && __all_sync(0xffffffffu, !loads || cache_row == first_row + (lane << shift));
+          const uint32_t full = bar(full0 + (int)ring.stage), to = base + ring.stage * (uint32_t)kTile8;
+          if (lane == 0) barrier_expect_bytes(full, (uint32_t)kTile8);
+          __syncwarp();
+          if (in_a_row) {
+            if (lane == 0) tma_load_2d(to, values ? &v_tile_map : &k_tile_map, full, w.kv_head * kDim, first_row);
+          } else if (loads) {                               // (a negative row lies outside the tensor: zeros)
+            tma_load_2d(to + (uint32_t)lane * box_bytes, values ? &v_map : &k_map, full, w.kv_head * kDim, cache_row);
+          }
+          ring.step(3);
+        }
+      }
+    } else {
+      // ---------------------------------------------------------------- issuer (tcgen05.cuh: from a whole warp)
+      constexpr uint32_t scores_hi = instruction_descriptor_8bit(kRows, kKeys, E4M3, E4M3);
+      constexpr uint32_t scores_lo = instruction_descriptor_8bit(kRows, kKeys, E5M2, E4M3);
+      constexpr uint32_t values_of = instruction_descriptor(kRows, kDim, true);
+      const uint32_t elected = elect_one();
+      const uint32_t q_low = operand_low(smem_base + kOffQ), k_low = operand_low(smem_base + kOffK);
+      const uint32_t v_low = operand_low_mn_major(smem_base + kOffV, kHalf);
+      bool alive = true;
+      auto check = [&](int index, uint32_t phase) {
+        if (alive && !wait_barrier(bar(index), phase)) { g_error = 2; alive = false; }
+      };
+      int g0 = 0, n = 0;
+      Counter keys, scores, weights, values;
+      for (int k = 0; more(k); ++k) {
+        if (!items.at(item_of(k, cta, ctas), w)) continue;
+        const int tiles = __shfl_sync(0xffffffffu, w.tiles, 0);
+        if (tiles == 0) continue;
+        check(Q_FULL + (n & 3), (uint32_t)(n >> 2 & 1));
+        auto issue_scores = [&](int t) {
+          check(K_FULL + (int)keys.stage, keys.phase);
+          __syncwarp();
+          tensor_fence_after_sync();
+          const uint32_t b = k_low + keys.stage * (uint32_t)(kTile8 >> 4), d = tmem + scores.stage * 128u;
+#pragma unroll
+          for (int kk = 0; kk < kDim / 32; ++kk) mma_8bit_ss_halves(d, q_low + 2u * kk, b + 2u * kk, scores_hi, kk > 0 ? 1u : 0u, elected);
+#pragma unroll
+          for (int kk = 0; kk < kDim / 32; ++kk)
+            mma_8bit_ss_halves(d, q_low + (uint32_t)(kTile8 >> 4) + 2u * kk, b + 2u * kk, scores_lo, 1u, elected);
+          mma_commit_elected(bar(S_FULL + (int)scores.stage), elected);
+          mma_commit_elected(bar(K_FREE + (int)keys.stage), elected);
+          if (t == tiles - 1) mma_commit_elected(bar(Q_FREE), elected);
+          keys.step(3);
+          scores.step(3);
+        };
+        // S(t + 3) takes the accumulator that holds P(t): behind the product with it
+        for (int t = 0; t < min(3, tiles); ++t) issue_scores(t);
+        for (int t = 0; t < tiles; ++t) {
+          const int g = g0 + t;
+          check(V_FULL + (int)values.stage, values.phase);
+          check(P_READY + (int)weights.stage, weights.phase);
+          if (t == 0 && n > 0) check(O_FREE, (uint32_t)(n - 1) & 1u);       // the last item's result has been read out
+          __syncwarp();
+          tensor_fence_after_sync();
+          const uint32_t p = tmem + weights.stage * 128u, b = v_low + values.stage * (uint32_t)(kTile16 >> 4);
+          mma_bf16_ts_halves(tmem_o, p, b, values_of, t > 0 ? 1u : 0u, elected);
+#pragma unroll
+          for (int kk = 1; kk < kKeys / 16; ++kk)
+            mma_bf16_ts_halves(tmem_o, p + (uint32_t)kk * 8u, b + (uint32_t)kk * (2048u >> 4), values_of, 1u, elected);
+          mma_commit_elected(bar(V_FREE + (int)values.stage), elected);
+          mma_commit_elected(bar(PV_DONE + (g & 1)), elected);
+          mma_commit_elected(bar(INFO_FREE + g % kInfos), elected);          // everybody is done with the tile
+          if (t == tiles - 1) mma_commit_elected(bar(ITEM_DONE), elected);
+          values.step(2);
+          weights.step(3);
+          if (t + 3 < tiles) issue_scores(t + 3);
+        }
+        g0 += tiles;
+        ++n;
+      }
+    }
+  } else if (warp < kFirstSoftmax) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConverterRegisters));
+    // ------------------------------------------------------------------ converters: an item's queries, then its tiles' values
+    const int thread = threadIdx.x - kFirstConverter * 32, my_warp = warp - kFirstConverter;
+    bool alive = true;
+    Counter raw, values;
+    int g = 0, n = 0;
+    for (int k = 0; more(k); ++k) {
+      if (!items.at(item_of(k, cta, ctas), w) || w.tiles == 0) continue;
+      // the products with the last item's queries are over
+      if (n > 0 && alive && !wait_barrier(bar(Q_FREE), (uint32_t)(n - 1) & 1u)) { g_error = 4; alive = false; }
+      __syncwarp();
+      // a warp takes 32 rows, four at a time, a lane four elements of each; rows that are not there repeat the last
+#pragma unroll 1
+      for (int r0 = my_warp * 32; r0 < my_warp * 32 + 32; r0 += 4) {
+        uint2 held[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = w.first_row + min(r0 + i, w.rows - 1), token = row / group, head = w.kv_head * group + row - token * group;
+          held[i] = *reinterpret_cast<const uint2*>(q + (size_t)(w.first_token + token) * q_stride + (size_t)head * kDim + lane * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x[4] = {__uint_as_float(held[i].x << 16), __uint_as_float(held[i].x & 0xffff0000u), __uint_as_float(held[i].y << 16),
+                              __uint_as_float(held[i].y & 0xffff0000u)};
+          const float largest = warp_largest(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+          const int e = least_scale_exponent(fminf(largest, 3.38953139e38f));
+          const float inverse = power_of_two(-e);
+          uint32_t hi[2], lo[2];
+          split_e4m3_e5m2(x[0] * inverse, x[1] * inverse, hi[0], lo[0]);
+          split_e4m3_e5m2(x[2] * inverse, x[3] * inverse, hi[1], lo[1]);
+          const int r = r0 + i;
+          unsigned char* to = smem + kOffQ + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
+          *reinterpret_cast<uint32_t*>(to) = hi[0] | (hi[1] << 16);
+          *reinterpret_cast<uint32_t*>(to + kTile8) = lo[0] | (lo[1] << 16);
+          if (lane == 0) row_scales[n & 3][r] = power_of_two(e) * scale_log2;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      barrier_arrive(bar(Q_FULL + (n & 3)));
+      ++n;
+      for (int t = 0; t < w.tiles; ++t, ++g) {
+        const int info = g % kInfos;
+        if (alive && !wait_barrier(bar(INFO_FULL + info), (uint32_t)(g / kInfos & 1))) { g_error = 4; alive = false; }
+        if (alive && !wait_barrier(bar(RAW_FULL + (int)raw.stage), raw.phase)) { g_error = 4; alive = false; }
+        if (alive && !wait_barrier(bar(V_FREE + (int)values.stage), values.phase ^ 1u)) { g_error = 4; alive = false; }
+        const unsigned char* from = smem + kOffRaw + raw.stage * kTile8;
+        unsigned char* to = smem + kOffV + values.stage * kTile16;
+        const int j = thread & 7;                            // 16 bytes of a row: 16 elements
+#pragma unroll 2
+        for (int r = thread >> 3; r < kKeys; r += kConverters / 8) {
+          const int key = w.begin + t * kKeys + r, slot = r >> shift;
+          const uint4 word = *reinterpret_cast<const uint4*>(from + r * 128 + ((j ^ (r & 7)) << 4));
+          const bool seen = key < w.end && key >= w.first_key && infos[info].row[slot] >= 0;
+          const int e = ((__float_as_int(infos[info].v_scale[slot]) >> 23) & 0xff) - 127;
+          const uint32_t factor = power_pair(min(e, 7) + 120);
+          uint32_t wide[8];
+          const uint32_t words[4] = {word.x, word.y, word.z, word.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            wide[2 * i] = times(lifted<0x9180>(words[i]), factor);
+            wide[2 * i + 1] = times(lifted<0xb3a2>(words[i]), factor);
+          }
+          if (e > 7) {                                       // (beyond what one bf16 factor holds)
+            const uint32_t rest = power_pair(e - 7);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) wide[i] = times(wide[i], rest);
+          }
+          // (0x7f and 0xff are NaN in e4m3, 480 in the bf16 number: put right)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t nan = __vcmpeq4(words[i] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            if (nan != 0u) {
+              if (nan & 0xffu) wide[2 * i] |= 0x7fffu;
+              if (nan & 0xff00u) wide[2 * i] |= 0x7fff0000u;
+              if (nan & 0xff0000u) wide[2 * i + 1] |= 0x7fffu;
+              if (nan & 0xff000000u) wide[2 * i + 1] |= 0x7fff0000u;
+            }
+          }
+          if (!seen) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) wide[i] = 0u;
+          }
+          unsigned char* row = to + (j >> 2) * kHalf + r * 128;
+          *reinterpret_cast<uint4*>(row + ((((j & 3) * 2) ^ (r & 7)) << 4)) = make_uint4(wide[0], wide[1], wide[2], wide[3]);
+          *reinterpret_cast<uint4*>(row + ((((j & 3) * 2 + 1) ^ (r & 7)) << 4)) = make_uint4(wide[4], wide[5], wide[6], wide[7]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        barrier_arrive(bar(V_FULL + (int)values.stage));
+        barrier_arrive(bar(RAW_FREE + (int)raw.stage));
+        raw.step(3);
+        values.step(2);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    // ------------------------------------------------------------------ softmax
+    const int stream = (warp - kFirstSoftmax) >> 3;          // takes the tiles t = stream, stream + 2, ...
+    const int quarter = warp & 3;                            // the accumulator lanes this warp may touch
+    const int part = ((warp - kFirstSoftmax) >> 2) & 1;      // which kCols columns of the row
+    const int r = quarter * 32 + lane, first = part * kCols;
+    const uint32_t lane_bits = (uint32_t)(quarter * 32) << 16;
+    const int team = 1 + stream * 4 + quarter;
+    bool alive = true;
+    int g0 = 0, n = 0;
+    for (int k = 0; more(k); ++k) {
+      if (!items.at(item_of(k, cta, ctas), w)) continue;
+      const int row = w.first_row + min(r, w.rows - 1), token = row / group, head = w.kv_head * group + row - token * group;
+      const size_t out_row = (size_t)(w.first_token + token) * heads + head;
+      if (w.tiles == 0) {                                    // a partition without keys, or rows that see none
+        if (stream == 0 && part == 0 && r < w.rows) {
+          if (num_partitions > 1) {
+            *reinterpret_cast<float2*>(partial_ml + (out_row * num_partitions + w.part) * 2) = make_float2(-INFINITY, 0.0f);
+          } else {
+            uint4* to = reinterpret_cast<uint4*>(out + out_row * kDim);
+#pragma unroll
+            for (int i = 0; i < kDim / 8; ++i) to[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        continue;
+      }
+      const int position = w.first_position + (w.first_row % group + min(r, w.rows - 1)) / group;
+      float reference = -INFINITY, denominator = 0.0f, scale = 0.0f;
+      if (stream < w.tiles) {
+        if (alive && !wait_barrier(bar(Q_FULL + (n & 3)), (uint32_t)(n >> 2 & 1))) { g_error = 3; alive = false; }
+        scale = row_scales[n & 3][r];
+      }
+      for (int t = stream; t < w.tiles; t += kStreams) {
+        const int g = g0 + t, stage = g % 3, info = g % kInfos, key0 = w.begin + t * kKeys;
+        if (alive && !wait_barrier(bar(INFO_FULL + info), (uint32_t)(g / kInfos & 1))) { g_error = 3; alive = false; }
+        if (alive && !wait_barrier(bar(S_FULL + stage), (uint32_t)(g / 3 & 1))) { g_error = 3; alive = false; }
+        __syncwarp();
+        tensor_fence_after_sync();
+        const uint32_t scores = tmem + (uint32_t)stage * 128u + lane_bits;
+        const int high = min(position, w.end - 1) - key0, low = window > 0 ? position - window + 1 - key0 : -1;
+        const bool every = infos[info].whole && key0 + kKeys - 1 <= w.first_position && key0 + kKeys <= w.end &&
+                           (window == 0 || w.last_position - window + 1 <= key0);
+        uint32_t packed[kCols / 2];
+        bool grow;
+        float factor, own_factor;
+        Handoff handoff;
+        handoff.has_from = t > 0;
+        handoff.from_barrier = bar(REF_READY + ((g - 1) & 1));
+        handoff.from_phase = (uint32_t)((g - 1) >> 1) & 1u;
+        handoff.from = &handed[(g - 1) & 1][r];
+        handoff.to_barrier = bar(REF_READY + (g & 1));
+        handoff.to = &handed[g & 1][r];
+        float* shared_max = &exchange[stream][(t / kStreams) & 1][0][r];
+        const float sum = every ? softmax_tile<false>(scores, first, low, high, scale, infos[info], shift, reference, factor, grow, own_factor,
+                                                      packed, shared_max, part, team, handoff, alive)
+                                : softmax_tile<true>(scores, first, low, high, scale, infos[info], shift, reference, factor, grow, own_factor,
+                                                     packed, shared_max, part, team, handoff, alive);
+        denominator = denominator * own_factor + sum;
+        // the accumulator holds the products up to tile t - 1, whose end is waited for; the product with this tile's weights is not
+        // issued before this stream arrives, so nothing else touches it meanwhile
+        if (t > 0 && __any_sync(0xffffffffu, grow)) {
+          if (alive && !wait_barrier(bar(PV_DONE + ((g - 1) & 1)), (uint32_t)((g - 1) >> 1) & 1u)) { g_error = 3; alive = false; }
+          __syncwarp();
+          tensor_fence_after_sync();
+#pragma unroll 1
+          for (int c0 = 0; c0 < kDim / kParts; c0 += 32) {
+            float o[32];
+            tmem_load_32(tmem_o + lane_bits + (uint32_t)(part * (kDim / kParts) + c0), o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= factor;
+            tmem_store_32(tmem_o + lane_bits + (uint32_t)(part * (kDim / kParts) + c0), o);
+          }
+        }
+        tmem_store_32_bits(scores + (uint32_t)(first / 2), packed);
+        tmem_store_wait();
+        tensor_fence_before_sync();
+        barrier_arrive(bar(P_READY + stage));
+      }
+      // every softmax thread learns every stream's reference and denominator
+      const int slot = n & 1;
+      denominators[slot][stream][part][r] = denominator;
+      if (part == 0) references[slot][stream][r] = reference;
+      asm volatile("bar.sync 9, %0;" ::"n"(kStreamThreads * kStreams) : "memory");
+      const float top = fmaxf(references[slot][0][r], references[slot][1][r]);
+      float total = 0.0f;
+#pragma unroll
+      for (int other = 0; other < kStreams; ++other) {
+        const float theirs = references[slot][other][r];     // -inf: that stream saw no key of this row
+        if (theirs > -INFINITY)
+          total += (denominators[slot][other][0][r] + denominators[slot][other][1][r]) * approximate_exp2(theirs - top);
+      }
+      if (alive && !wait_barrier(bar(ITEM_DONE), (uint32_t)n & 1u)) { g_error = 3; alive = false; }
+      __syncwarp();
+      tensor_fence_after_sync();
+      constexpr int kOut = kDim / (kParts * kStreams);       // 32 columns of the row for each of its threads
+      const int column = (stream * kParts + part) * kOut;
+      float o[kOut];
+      tmem_load_32(tmem_o + lane_bits + (uint32_t)column, o);
+      tensor_fence_before_sync();
+      barrier_arrive(bar(O_FREE));                           // (the next item's products may overwrite it)
+      if (r < w.rows && alive) {
+        if (num_partitions == 1) {
+          if (total != 0.0f && sinks != nullptr) total += exp2f(sinks[head] * kLog2e - top);
+          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+          uint4* to = reinterpret_cast<uint4*>(out + out_row * kDim + column);
+#pragma unroll
+          for (int i = 0; i < kOut; i += 8) {
+            uint4 packed_out;
+            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&packed_out);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              h[c] = __floats2bfloat162_rn(total == 0.0f ? 0.0f : o[i + 2 * c] * inverse, total == 0.0f ? 0.0f : o[i + 2 * c + 1] * inverse);
+            to[i / 8] = packed_out;
+          }
+        } else {
+          const size_t at = out_row * num_partitions + w.part;
+          if (column == 0) *reinterpret_cast<float2*>(partial_ml + at * 2) = make_float2(top, total);
+          if (total != 0.0f) {
+            float4* to = reinterpret_cast<float4*>(partial_o + at * kDim + column);
+#pragma unroll
+            for (int i = 0; i < kOut; i += 4) to[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+      }
+      g0 += w.tiles;
+      ++n;
+    }
+    tensor_fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == kIssuer) {
+    tensor_fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
+  }
+}
+
+}  // namespace
+
+// 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 scout or loader, 2 issuer, 3 softmax, 4 converters).
+// Synchronises the device.
+MIR_EXPORT int mir_prefill_attention_8bit_error() {
+  int flag = 0;
+  if (cudaMemcpyFromSymbol(&flag, g_error, sizeof(int)) != cudaSuccess) return -1;
+  return flag;
+}
+
+int mir_attention_8bit_prefill(const Attention8& a, int tokens) {
+  const int group = a.heads / a.cache.kv_heads;
+  // an upper bound of the items (the kernel counts them); as many CTAs as there can be work for
+  const long long items = (((long long)tokens * group + kRows - 1) / kRows + a.num_rows) * a.cache.kv_heads * a.num_partitions;
+  if (items > 0x7fffffffll || (long long)tokens * group > 0x7fffffffll - kRows) {
+    mir_set_error("%s: %d tokens in %d rows are more than one launch takes", a.what, tokens, a.num_rows);
+    return MIR_BAD_ARGUMENT;
+  }
+  const long long rows = (long long)a.cache.pages * a.cache.page_size, width = (long long)a.cache.kv_heads * kDim;
+  CUtensorMap maps[4];
+  const void* tensors[2] = {a.cache.k, a.cache.v};
+  for (int i = 0; i < 4; ++i) {
+    const int status = tensor_map_of_bytes(tensors[i & 1], rows, width, width, i < 2 ? a.cache.page_size : kKeys, &maps[i]);
+    if (status != MIR_OK) return status;
+  }
+  int status = reserve_shared(prefill_8bit_kernel, kSmemBytes, a.what);
+  if (status != MIR_OK) return status;
+  status = mir_launch("prefill_attention_8bit", prefill_8bit_kernel, dim3((unsigned)std::min<long long>(items, mir_sm_count())), dim3(kThreads),
+                      (size_t)kSmemBytes, a.stream, 0, maps[0], maps[1], maps[2], maps[3], (const bf16*)a.q, a.q_stride, a.cache, a.block_table,
+                      a.table_width, a.query_starts, a.context_lens, a.num_rows, a.heads, a.scale * kLog2e, a.window, a.partition,
+                      a.num_partitions, a.partial_o(tokens), a.partial_ml(tokens), (bf16*)a.out, a.sinks);
+  if (status != MIR_OK || a.num_partitions == 1) return status;
+  return mir_merge_8bit(a, tokens);
+}

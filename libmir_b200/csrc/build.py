@@ -51,7 +51,7 @@ LIBRARIES = {
     },
     # the operators for serving in 8 bits
     "eight_bit": {
-        "sources": ["runtime.cu", "store_8bit.cu", "attention_8bit.cu", "attention_8bit_decode.cu", "linear_8bit.cu", "linear_8bit_few.cu", "linear_8bit_tc.cu"],
+        "sources": ["runtime.cu", "store_8bit.cu", "attention_8bit.cu", "attention_8bit_decode.cu", "attention_8bit_tc.cu", "linear_8bit.cu", "linear_8bit_few.cu", "linear_8bit_tc.cu"],
         "headers": ["eight_bit.h", "eight_bit.cuh", "eight_bit_tc.cuh", "tcgen05.cuh"],
         "link": [],
         "defines": [],

@@ -30,6 +30,13 @@ __device__ __forceinline__ int least_scale_exponent(float largest) {
 __device__ __forceinline__ uint32_t to_e4m3x2(float first, float second) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(first, second), __NV_SATFINITE, __NV_E4M3);
 }
+// Two numbers within 448 as e4m3 and what that leaves as e5m2 (the first in the low bytes).
+__device__ __forceinline__ __half2 e4m3_low(uint32_t word);
+__device__ __forceinline__ void split_e4m3_e5m2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = to_e4m3x2(a, b);
+  const float2 taken = __half22float2(e4m3_low(hi));
+  lo = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a - taken.x, b - taken.y), __NV_SATFINITE, __NV_E5M2);
+}
 // The two e4m3 numbers of the low (high) half of a word as float16, exact.
 __device__ __forceinline__ __half2 e4m3_low(uint32_t word) {
   return __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word & 0xffffu), __NV_E4M3));

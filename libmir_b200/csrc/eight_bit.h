@@ -36,6 +36,8 @@ bool mir_decode_8bit_takes(int head_dim, int page_size);
 int mir_decode_8bit_ctas(long long most_tiles, int heads, int kv_heads);
 long long mir_decode_8bit_floats(int ctas, int group);
 int mir_attention_8bit_decode(const Attention8& a);
+// Portions on them (attention_8bit_tc.cu), for the same sizes.
+int mir_attention_8bit_prefill(const Attention8& a, int tokens);
 
 // The product of rounded rows (codes [m, k], scales [blocks of 128 columns, scale_stride], scale_stride m
 // filled up to whole 128) with an 8-bit weight, by tiles of 128 rows

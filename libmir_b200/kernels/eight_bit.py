@@ -155,7 +155,7 @@ def eight_bit_error() -> int:
     """0 unless a bounded wait of one of the tcgen05 kernels ran out (synchronises the device); such a kernel does no work from
     then on."""
     lib = library("eight_bit")
-    return int(lib.mir_decode_attention_8bit_error() or lib.mir_linear_8bit_tiles_error() or lib.mir_linear_8bit_few_error())
+    return int(lib.mir_decode_attention_8bit_error() or lib.mir_prefill_attention_8bit_error() or lib.mir_linear_8bit_tiles_error() or lib.mir_linear_8bit_few_error())
 
 
 def quantize_weight_8bit(weight: torch.Tensor) -> tuple:
