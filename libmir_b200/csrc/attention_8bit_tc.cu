@@ -38,11 +38,12 @@ constexpr int kSmemBytes = kOffV + kValueStages * kTile16 + 1024;
 static_assert(kSmemBytes + kLeastSharedBeside > kSharedOfSm, "no other kernel with tensor memory beside this one");
 constexpr int kParts = 2, kCols = kKeys / kParts;           // softmax threads of a row and stream; columns of each
 constexpr int kStreams = 2, kStreamThreads = kRows * kParts;
-enum { kKeyLoader = 0, kIssuer = 1, kValueLoader = 2, kScout = 3, kFirstConverter = 4, kFirstSoftmax = 8 };      // warps
-constexpr int kConverters = 128, kThreads = (kFirstSoftmax + 8 * kStreams) * 32;
-// launched with 80 registers a thread (6 * 80 = 480); the first eight warps give some up: 40 + 56 + 4 * 96 = 480
-constexpr int kRoleRegisters = 40, kConverterRegisters = 56, kSoftmaxRegisters = 96;
-static_assert(kRoleRegisters + kConverterRegisters + 4 * kSoftmaxRegisters <= 6 * 80, "no more registers than the launch holds");
+enum { kKeyLoader = 0, kIssuer = 1, kValueLoader = 2, kScout = 3, kFirstConverter = 4, kFirstSoftmax = 12 };     // warps
+// (Eight converting warps: four had a quarter of their schedulers' slots each, took 3,100 cycles for a tile's values and set the pace.)
+constexpr int kConverters = 256, kThreads = (kFirstSoftmax + 8 * kStreams) * 32;
+// launched with 72 registers a thread (7 * 72 = 504); the first twelve warps give some up: 40 + 2 * 40 + 4 * 96 = 504
+constexpr int kRoleRegisters = 40, kConverterRegisters = 40, kSoftmaxRegisters = 96;
+static_assert(kRoleRegisters + 2 * kConverterRegisters + 4 * kSoftmaxRegisters <= 7 * 72, "no more registers than the launch holds");
 constexpr uint32_t kTmemColumns = 512;                      // S at 0, 128, 256; O at 384
 constexpr float kRises = 8.0f;
 
@@ -63,8 +64,9 @@ __device__ __forceinline__ float warp_largest(float v) {
 // What the scout leaves of a tile: each page's first row of the cache (below 0: not there, or no query of the item sees it), its scales.
 struct Info {
   int row[kSlots];
-  float k_scale[kSlots], v_scale[kSlots];
-  int whole;                                                // all pages are there
+  float k_scale[kSlots];
+  uint32_t v_factor[kSlots], v_rest[kSlots];               // what a lifted value is multiplied by: 2^120 times its scale, as one or two bf16 pairs
+  int whole, one_factor;                                                // all pages are there
 };
 
 struct Work {
@@ -130,6 +132,12 @@ __device__ __forceinline__ uint32_t times(uint32_t pair, uint32_t factor) {
 // bf16 pair of 2^e, e from -126 to 127.
 __device__ __forceinline__ uint32_t power_pair(int e) { return (uint32_t)(e + 127) << 7 | (uint32_t)(e + 127) << 23; }
 
+__device__ __forceinline__ float max_of_three(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 struct Handoff {
   bool has_from;
   uint32_t from_barrier, from_phase, to_barrier;
@@ -149,23 +157,29 @@ __device__ __forceinline__ float softmax_tile(uint32_t scores, int first, int lo
   tmem_load_32_ahead(scores + (uint32_t)first + 32u, raw[1]);
   tmem_load_done(raw[0]);
   tmem_load_done(raw[1]);
+  // Eight columns are of one page (a page has eight keys or more): their scores share a factor, which is positive, so that the maximum is
+  // taken first and the multiplication is part of the exponent's.
   float v[kCols];
+  float maximum = -INFINITY;
 #pragma unroll
-  for (int c8 = 0; c8 < kCols / 8; ++c8) {                  // (a page has eight keys or more)
-    const int slot = (first + c8 * 8) >> shift;
-    const float k_scale = info.k_scale[slot] * scale;
+  for (int c8 = 0; c8 < kCols; c8 += 8) {
+    const int slot = (first + c8) >> shift;
+    float best[2] = {-INFINITY, -INFINITY};
     const bool there = !MASKED || info.row[slot] >= 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = c8 * 8 + i;
-      v[c] = __uint_as_float(raw[c / 32][c % 32]) * k_scale;
-      if (MASKED) v[c] = there && c >= low - first && c <= high - first ? v[c] : -INFINITY;
+    for (int i = 0; i < 8; i += 2) {
+      const int c = c8 + i;
+      v[c] = __uint_as_float(raw[c / 32][c % 32]);
+      v[c + 1] = __uint_as_float(raw[c / 32][c % 32 + 1]);
+      if (MASKED) {
+        v[c] = there && c >= low - first && c <= high - first ? v[c] : -INFINITY;
+        v[c + 1] = there && c + 1 >= low - first && c + 1 <= high - first ? v[c + 1] : -INFINITY;
+      }
+      best[i >> 1 & 1] = max_of_three(best[i >> 1 & 1], v[c], v[c + 1]);
     }
+    maximum = fmaxf(maximum, fmaxf(best[0], best[1]) * info.k_scale[slot]);
   }
-  float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) best[c & 3] = fmaxf(best[c & 3], v[c]);
-  float maximum = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+  maximum *= scale;
   shared_max[part * kRows] = maximum;
   asm volatile("bar.sync %0, %1;" ::"r"(team), "n"(32 * kParts) : "memory");
 #pragma unroll
@@ -185,11 +199,16 @@ __device__ __forceinline__ float softmax_tile(uint32_t scores, int first, int lo
   const float down = (MASKED && reference == -INFINITY) ? 0.0f : -reference;       // (a row that has seen nothing yet)
   float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int c = 0; c < kCols; c += 2) {
-    const float p0 = approximate_exp2(v[c] + down), p1 = approximate_exp2(v[c + 1] + down);
-    sums[(c >> 1) & 3] += p0 + p1;
-    const __nv_bfloat162 both = __floats2bfloat162_rn(p0, p1);
-    packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&both);
+  for (int c8 = 0; c8 < kCols; c8 += 8) {
+    const float k_scale = info.k_scale[(first + c8) >> shift] * scale;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const int c = c8 + i;
+      const float p0 = approximate_exp2(fmaf(v[c], k_scale, down)), p1 = approximate_exp2(fmaf(v[c + 1], k_scale, down));
+      sums[(c >> 1) & 3] += p0 + p1;
+      const __nv_bfloat162 both = __floats2bfloat162_rn(p0, p1);
+      packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&both);
+    }
   }
   return (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
@@ -270,7 +289,8 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             k_scale = cache.k_scales[(size_t)page * cache.kv_heads + w.kv_head];
             v_scale = cache.v_scales[(size_t)page * cache.kv_heads + w.kv_head];
           }
-          const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+          const int v_exponent = ((__float_as_int(v_scale) >> 23) & 0xff) - 127;
+          const unsigned there = __ballot_sync(0xffffffffu, page >= 0), loud = __ballot_sync(0xffffffffu, v_exponent > 7);
           for (int i = 0; i < 2 && t + i < w.tiles; ++i) {
             const int info = (g + i) % kInfos;
             if (alive && !wait_barrier(bar(INFO_FREE + info), (uint32_t)((g + i) / kInfos & 1) ^ 1u)) { g_error = 1; alive = false; }
@@ -278,9 +298,13 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             if (half == i) {
               infos[info].row[slot] = page >= 0 ? page << shift : -cache.page_size;
               infos[info].k_scale[slot] = k_scale;
-              infos[info].v_scale[slot] = v_scale;
+              infos[info].v_factor[slot] = power_pair(min(v_exponent, 7) + 120);
+              infos[info].v_rest[slot] = power_pair(max(v_exponent - 7, 0));
             }
-            if (lane == 0) infos[info].whole = __popc((there >> (16 * i)) & 0xffffu) == slots;
+            if (lane == 0) {
+              infos[info].whole = __popc((there >> (16 * i)) & 0xffffu) == slots;
+              infos[info].one_factor = ((loud >> (16 * i)) & 0xffffu) == 0u;
+            }
             __syncwarp();
             if (lane == 0) barrier_arrive(bar(INFO_FULL + info));
           }
@@ -392,17 +416,18 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       // the products with the last item's queries are over
       if (n > 0 && alive && !wait_barrier(bar(Q_FREE), (uint32_t)(n - 1) & 1u)) { g_error = 4; alive = false; }
       __syncwarp();
-      // a warp takes 32 rows, four at a time, a lane four elements of each; rows that are not there repeat the last
+      // a warp takes 16 rows, eight at a time, a lane four elements of each; rows that are not there repeat the last
+      constexpr int kHeld = 8, kWarpRows = kRows / (kConverters / 32);
 #pragma unroll 1
-      for (int r0 = my_warp * 32; r0 < my_warp * 32 + 32; r0 += 4) {
-        uint2 held[4];
+      for (int r0 = my_warp * kWarpRows; r0 < (my_warp + 1) * kWarpRows; r0 += kHeld) {
+        uint2 held[kHeld];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kHeld; ++i) {
           const int row = w.first_row + min(r0 + i, w.rows - 1), token = row / group, head = w.kv_head * group + row - token * group;
           held[i] = *reinterpret_cast<const uint2*>(q + (size_t)(w.first_token + token) * q_stride + (size_t)head * kDim + lane * 4);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kHeld; ++i) {
           const float x[4] = {__uint_as_float(held[i].x << 16), __uint_as_float(held[i].x & 0xffff0000u), __uint_as_float(held[i].y << 16),
                               __uint_as_float(held[i].y & 0xffff0000u)};
           const float largest = warp_largest(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
@@ -428,44 +453,52 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (alive && !wait_barrier(bar(V_FREE + (int)values.stage), values.phase ^ 1u)) { g_error = 4; alive = false; }
         const unsigned char* from = smem + kOffRaw + raw.stage * kTile8;
         unsigned char* to = smem + kOffV + values.stage * kTile16;
-        const int j = thread & 7;                            // 16 bytes of a row: 16 elements
-#pragma unroll 2
-        for (int r = thread >> 3; r < kKeys; r += kConverters / 8) {
-          const int key = w.begin + t * kKeys + r, slot = r >> shift;
-          const uint4 word = *reinterpret_cast<const uint4*>(from + r * 128 + ((j ^ (r & 7)) << 4));
-          const bool seen = key < w.end && key >= w.first_key && infos[info].row[slot] >= 0;
-          const int e = ((__float_as_int(infos[info].v_scale[slot]) >> 23) & 0xff) - 127;
-          const uint32_t factor = power_pair(min(e, 7) + 120);
-          uint32_t wide[8];
-          const uint32_t words[4] = {word.x, word.y, word.z, word.w};
+        // thread: 16 bytes (j) of every 32nd row (whose place in the swizzle is the same), two at a time
+        const int j = thread & 7, r0 = thread >> 3;
+        const bool all_seen = infos[info].whole && w.begin + t * kKeys >= w.first_key && w.begin + (t + 1) * kKeys <= w.end;
+        const bool one_factor = infos[info].one_factor;
+        from += r0 * 128 + ((j ^ (r0 & 7)) << 4);
+        unsigned char* low = to + (j >> 2) * kHalf + r0 * 128 + ((((j & 3) * 2) ^ (r0 & 7)) << 4);
+        unsigned char* high = to + (j >> 2) * kHalf + r0 * 128 + ((((j & 3) * 2 + 1) ^ (r0 & 7)) << 4);
+        constexpr int kStep = kConverters / 8, kTogether = 2;
+#pragma unroll 1
+        for (int base = 0; base < kKeys; base += kStep * kTogether) {
+          uint4 word[kTogether];
+          uint32_t factor[kTogether];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            wide[2 * i] = times(lifted<0x9180>(words[i]), factor);
-            wide[2 * i + 1] = times(lifted<0xb3a2>(words[i]), factor);
+          for (int i = 0; i < kTogether; ++i) {
+            word[i] = *reinterpret_cast<const uint4*>(from + (base + i * kStep) * 128);
+            factor[i] = infos[info].v_factor[(base + i * kStep + r0) >> shift];
           }
-          if (e > 7) {                                       // (beyond what one bf16 factor holds)
-            const uint32_t rest = power_pair(e - 7);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) wide[i] = times(wide[i], rest);
-          }
-          // (0x7f and 0xff are NaN in e4m3, 480 in the bf16 number: put right)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t nan = __vcmpeq4(words[i] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            if (nan != 0u) {
-              if (nan & 0xffu) wide[2 * i] |= 0x7fffu;
-              if (nan & 0xff00u) wide[2 * i] |= 0x7fff0000u;
-              if (nan & 0xff0000u) wide[2 * i + 1] |= 0x7fffu;
-              if (nan & 0xff000000u) wide[2 * i + 1] |= 0x7fff0000u;
+          for (int i = 0; i < kTogether; ++i) {
+            const int r = base + i * kStep + r0;
+            if (!all_seen) {
+              const int key = w.begin + t * kKeys + r;
+              if (key >= w.end || key < w.first_key || infos[info].row[r >> shift] < 0) word[i] = make_uint4(0u, 0u, 0u, 0u);
             }
-          }
-          if (!seen) {
+            uint32_t wide[8];
+            const uint32_t words[4] = {word[i].x, word[i].y, word[i].z, word[i].w};
+            uint32_t last = 0u;                              // a byte's upper bit: its magnitude is e4m3's last code, NaN
 #pragma unroll
-            for (int i = 0; i < 8; ++i) wide[i] = 0u;
+            for (int c = 0; c < 4; ++c) {
+              wide[2 * c] = times(lifted<0x9180>(words[c]), factor[i]);
+              wide[2 * c + 1] = times(lifted<0xb3a2>(words[c]), factor[i]);
+              last |= (words[c] & 0x7f7f7f7fu) + 0x01010101u;
+            }
+            if ((last & 0x80808080u) != 0u || !one_factor) {       // (rare: the lifted number of a NaN is 480; a scale beyond one bf16 factor)
+              const uint32_t rest = infos[info].v_rest[r >> shift];
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                wide[c] = times(wide[c], rest);
+                const uint32_t pair = words[c / 2] >> (16 * (c & 1));
+                if ((pair & 0x7fu) == 0x7fu) wide[c] |= 0x7fffu;
+                if ((pair & 0x7f00u) == 0x7f00u) wide[c] |= 0x7fff0000u;
+              }
+            }
+            *reinterpret_cast<uint4*>(low + (base + i * kStep) * 128) = make_uint4(wide[0], wide[1], wide[2], wide[3]);
+            *reinterpret_cast<uint4*>(high + (base + i * kStep) * 128) = make_uint4(wide[4], wide[5], wide[6], wide[7]);
           }
-          unsigned char* row = to + (j >> 2) * kHalf + r * 128;
-          *reinterpret_cast<uint4*>(row + ((((j & 3) * 2) ^ (r & 7)) << 4)) = make_uint4(wide[0], wide[1], wide[2], wide[3]);
-          *reinterpret_cast<uint4*>(row + ((((j & 3) * 2 + 1) ^ (r & 7)) << 4)) = make_uint4(wide[4], wide[5], wide[6], wide[7]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         barrier_arrive(bar(V_FULL + (int)values.stage));
