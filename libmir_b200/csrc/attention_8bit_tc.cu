@@ -413,24 +413,31 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     int g = 0, n = 0;
     for (int k = 0; more(k); ++k) {
       if (!items.at(item_of(k, cta, ctas), w) || w.tiles == 0) continue;
-      // the products with the last item's queries are over
-      if (n > 0 && alive && !wait_barrier(bar(Q_FREE), (uint32_t)(n - 1) & 1u)) { g_error = 4; alive = false; }
-      __syncwarp();
-      // a warp takes 16 rows, eight at a time, a lane four elements of each; rows that are not there repeat the last
+      // a warp takes 16 rows, eight at a time, a lane four elements of each; rows that are not there repeat the last.  Where a row's
+      // queries lie a lane each works out once (a division a row in every lane took longer than the rounding).
       constexpr int kHeld = 8, kWarpRows = kRows / (kConverters / 32);
+      long long offset;
+      {
+        const int row = w.first_row + min(my_warp * kWarpRows + (lane & (kWarpRows - 1)), w.rows - 1), token = row / group;
+        offset = (long long)(w.first_token + token) * q_stride + (long long)(w.kv_head * group + row - token * group) * kDim;
+      }
 #pragma unroll 1
-      for (int r0 = my_warp * kWarpRows; r0 < (my_warp + 1) * kWarpRows; r0 += kHeld) {
+      for (int half = 0; half < kWarpRows; half += kHeld) {
         uint2 held[kHeld];
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-          const int row = w.first_row + min(r0 + i, w.rows - 1), token = row / group, head = w.kv_head * group + row - token * group;
-          held[i] = *reinterpret_cast<const uint2*>(q + (size_t)(w.first_token + token) * q_stride + (size_t)head * kDim + lane * 4);
+        for (int i = 0; i < kHeld; ++i)
+          held[i] = *reinterpret_cast<const uint2*>(q + __shfl_sync(0xffffffffu, offset, half + i) + lane * 4);
+        // (asked for while the products with the last item's queries may still run)
+        if (half == 0 && n > 0) {
+          if (alive && !wait_barrier(bar(Q_FREE), (uint32_t)(n - 1) & 1u)) { g_error = 4; alive = false; }
+          __syncwarp();
         }
+        const int r0 = my_warp * kWarpRows + half;
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
           const float x[4] = {__uint_as_float(held[i].x << 16), __uint_as_float(held[i].x & 0xffff0000u), __uint_as_float(held[i].y << 16),
                               __uint_as_float(held[i].y & 0xffff0000u)};
-          const float largest = warp_largest(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+          const float largest = warp_largest(max_of_three(fmaxf(fabsf(x[0]), fabsf(x[1])), fabsf(x[2]), fabsf(x[3])));
           const int e = least_scale_exponent(fminf(largest, 3.38953139e38f));
           const float inverse = power_of_two(-e);
           uint32_t hi[2], lo[2];
