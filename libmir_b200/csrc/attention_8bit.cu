@@ -398,6 +398,27 @@ MIR_EXPORT int mir_decode_attention_8bit(const void* q, long long q_stride, void
   return shared_out ? mir_attention_8bit_decode(a) : mir_attention_8bit_general(a, rows);
 }
 
+// How portions are split over the keys: not at all where their tiles of rows and kv heads fill the SMs; a few tokens behind a long context
+// are fewer items than SMs, and each would walk over all of it (16 tokens at 16,384, 32 heads over 8: 8 items).
+MIR_EXPORT int mir_prefill_attention_8bit_plan(int rows, int tokens, int heads, int kv_heads, int head_dim, int page_size, int max_context,
+                                               int* keys, int* count, long long* floats) {
+  if (rows < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context < 0 || page_size <= 0) {
+    mir_set_error("prefill_attention_8bit: bad sizes (%d requests, %d tokens, heads %d, kv heads %d, context %d)", rows, tokens, heads,
+                  kv_heads, max_context);
+    return MIR_BAD_ARGUMENT;
+  }
+  const long long group = heads / kv_heads, tile = mir_decode_8bit_takes(head_dim, page_size) ? 128 : kRows;
+  const long long items = std::max(1ll, (tokens * group + tile - 1) / tile) * kv_heads;       // (at least as many as that)
+  const long long tiles = std::max(1ll, (max_context + 127ll) / 128);
+  // up to two partitions' items an SM, at least four tiles of keys each
+  const long long wanted = std::max(1ll, std::min(2ll * mir_sm_count() / items, tiles / 4));
+  const long long each = (tiles + wanted - 1) / wanted;
+  *keys = (int)(each * 128);
+  *count = (int)((tiles + each - 1) / each);
+  *floats = *count == 1 ? 0 : (long long)tokens * heads * *count * (head_dim + 2);
+  return MIR_OK;
+}
+
 // Portions: request r has tokens query_starts[r] .. query_starts[r + 1] - 1 of the packed rows, and its context_lens[r]
 // cached tokens include them.  Rows that no request has are left as they are.
 MIR_EXPORT int mir_prefill_attention_8bit(const void* q, long long q_stride, void* out, const void* k_pages, const void* v_pages,

@@ -142,8 +142,14 @@ def prefill_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.
     longest = block_table.shape[1] * page_size
     if max_context is not None:
         longest = min(longest, max_context)
-    partition, count, scratch = max(128, -(-longest // 128) * 128), 1, None
     lib = library("eight_bit")
+    keys, parts, floats = ctypes.c_int(), ctypes.c_int(), ctypes.c_longlong()
+    _check(lib, lib.mir_prefill_attention_8bit_plan(rows, tokens, heads, kv_heads, head_dim, page_size, longest, ctypes.byref(keys),
+                                                    ctypes.byref(parts), ctypes.byref(floats)))
+    partition, count, scratch = keys.value, parts.value, None
+    if floats.value:
+        scratch = alloc((floats.value,), torch.float32) if alloc is not None else \
+            torch.empty((floats.value,), dtype=torch.float32, device=out.device)
     _check(lib, lib.mir_prefill_attention_8bit(
         qkv.data_ptr(), qkv.stride(0), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
         v_scales.data_ptr(), pages, block_table.data_ptr(), block_table.shape[1], query_starts.data_ptr(), context_lens.data_ptr(),
