@@ -85,9 +85,9 @@ quantize_weight_kernel(const T* __restrict__ weight, uint8_t* __restrict__ codes
 // Scales of a block: one for each row, filled up to whole tiles of 128 rows.
 static int scale_stride_of(int m) { return (m + kBlock - 1) / kBlock * kBlock; }
 
-// Bytes of workspace for m rows of k columns: the rounded rows, then their scales.
+// Bytes of workspace for m rows of k columns: the rounded rows, then their scales (none where the product rounds the rows itself).
 MIR_EXPORT long long mir_linear_8bit_workspace(int m, int k) {
-  if (m <= 0 || k <= 0) return 0;
+  if (m <= 0 || k <= 0 || (mir_linear_8bit_few_takes(m, k) && mir_linear_8bit_few_rounds(m))) return 0;
   const long long codes = ((long long)m * k + 255) / 256 * 256;
   return codes + (long long)scale_stride_of(m) * ((k + kBlock - 1) / kBlock) * (long long)sizeof(float);
 }
@@ -116,9 +116,9 @@ MIR_EXPORT int mir_linear_8bit(const void* x, long long x_stride, const void* we
                   "and accumulates into float32 (m %d, n %d, k %d, row strides %lld and %lld)", m, n, k, x_stride, out_stride);
     return MIR_BAD_ARGUMENT;
   }
-  if (workspace == nullptr || workspace_bytes < mir_linear_8bit_workspace(m, k) || ((uintptr_t)workspace & 15)) {
-    mir_set_error("linear_8bit: %lld bytes of 16-byte aligned workspace are needed, got %lld", mir_linear_8bit_workspace(m, k),
-                  workspace_bytes);
+  const long long need = mir_linear_8bit_workspace(m, k);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
+    mir_set_error("linear_8bit: %lld bytes of 16-byte aligned workspace are needed, got %lld", need, workspace_bytes);
     return MIR_BAD_ARGUMENT;
   }
   const int blocks = (k + kBlock - 1) / kBlock;

@@ -14,52 +14,59 @@ from typing import Callable, Optional
 import torch
 
 from ..errors import KernelError
-from . import _check, _ptr, _require, _stream, library
+from . import _check, _ptr, _raw_device, _stream, library
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 128                 # rows and columns of a weight that share a scale, and columns of a row of activations
 
 
+# (The checks run at every call: conditions are tested in place and messages put together only where one fails.)
 def _on_this_device(what: str, *tensors) -> None:
-    here = None
+    here = _current_device()
     for tensor in tensors:
-        if tensor is None:
-            continue
-        if not tensor.is_cuda:
-            raise KernelError("kernels take CUDA tensors only: there is no CPU path")
-        if here is None:
-            here = torch.cuda.current_device()
-        if tensor.device.index != here:
+        if tensor is not None and tensor.get_device() != here:
+            if not tensor.is_cuda:
+                raise KernelError("kernels take CUDA tensors only: there is no CPU path")
             raise KernelError(f"{what}: a tensor is on {tensor.device}, the current device is cuda:{here}")
+
+
+def _current_device() -> int:
+    return _raw_device() if _raw_device is not None and torch.cuda.is_initialized() else (
+        torch.cuda.current_device() if torch.cuda.is_available() else 0)
 
 
 def _cache(what: str, k_pages, v_pages, k_scales, v_scales, page_size: int, kv_heads: int, head_dim: int) -> int:
     """Checks the four tensors of an 8-bit cache; how many pages it has."""
-    _require(page_size > 0 and kv_heads > 0 and head_dim in (64, 128), f"{what}: takes head_dim 64 or 128, got {head_dim} (page "
-             f"{page_size}, {kv_heads} kv heads)")
-    rows = k_pages.shape[0]
-    _require(k_pages.dtype == E4M3 and v_pages.dtype == E4M3 and k_pages.is_contiguous() and v_pages.is_contiguous()
-             and k_pages.shape == (rows, kv_heads, head_dim) and v_pages.shape == k_pages.shape and rows % page_size == 0 and rows > 0,
-             f"{what}: the pages are contiguous float8_e4m3fn [pages * {page_size}, {kv_heads}, {head_dim}]")
-    pages = rows // page_size
-    _require(k_scales.dtype == torch.float32 and v_scales.dtype == torch.float32 and k_scales.is_contiguous()
-             and v_scales.is_contiguous() and k_scales.shape == (pages, kv_heads) and v_scales.shape == k_scales.shape,
-             f"{what}: the scales are contiguous float32 [{pages}, {kv_heads}]")
+    if page_size <= 0 or kv_heads <= 0 or head_dim not in (64, 128):
+        raise KernelError(f"{what}: takes head_dim 64 or 128, got {head_dim} (page {page_size}, {kv_heads} kv heads)")
+    shape = k_pages.shape
+    if not (len(shape) == 3 and shape[1] == kv_heads and shape[2] == head_dim and v_pages.shape == shape and shape[0] > 0
+            and shape[0] % page_size == 0 and k_pages.dtype is E4M3 and v_pages.dtype is E4M3 and k_pages.is_contiguous()
+            and v_pages.is_contiguous()):
+        raise KernelError(f"{what}: the pages are contiguous float8_e4m3fn [pages * {page_size}, {kv_heads}, {head_dim}]")
+    pages = shape[0] // page_size
+    shape = k_scales.shape
+    if not (len(shape) == 2 and shape[0] == pages and shape[1] == kv_heads and v_scales.shape == shape and k_scales.dtype is torch.float32
+            and v_scales.dtype is torch.float32 and k_scales.is_contiguous() and v_scales.is_contiguous()):
+        raise KernelError(f"{what}: the scales are contiguous float32 [{pages}, {kv_heads}]")
     return pages
 
 
 def _attention(what: str, qkv, out, block_table, heads: int, kv_heads: int, head_dim: int, rows: int, sinks, scratch) -> None:
-    _require(heads > 0 and heads % kv_heads == 0, f"{what}: {heads} heads do not divide over {kv_heads} kv heads")
-    _require(qkv.dtype == torch.bfloat16 and out.dtype == torch.bfloat16 and out.is_contiguous() and qkv.dim() == 2
-             and qkv.stride(1) == 1 and qkv.shape[1] >= heads * head_dim and out.dim() == 2 and out.shape[1] == heads * head_dim
-             and qkv.shape[0] >= out.shape[0], f"{what}: bfloat16 rows that begin with {heads} heads of {head_dim} are needed, and out "
-             "[rows, heads * head_dim]")
-    _require(block_table.dtype == torch.int32 and block_table.is_contiguous() and block_table.dim() == 2
-             and block_table.shape[0] >= rows and (block_table.shape[1] > 0 or rows == 0), f"{what}: the block table is contiguous "
-             "int32 [rows, blocks]")
-    _require(sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == heads and sinks.is_contiguous()),
-             f"{what}: sinks are float32 [heads]")
-    _require(scratch is None or (scratch.dtype == torch.float32 and scratch.is_contiguous()), f"{what}: scratch must be float32")
+    if heads <= 0 or heads % kv_heads:
+        raise KernelError(f"{what}: {heads} heads do not divide over {kv_heads} kv heads")
+    width, given, result = heads * head_dim, qkv.shape, out.shape
+    if not (qkv.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and len(given) == 2 and len(result) == 2 and given[1] >= width
+            and result[1] == width and given[0] >= result[0] and qkv.stride(1) == 1 and out.is_contiguous()):
+        raise KernelError(f"{what}: bfloat16 rows that begin with {heads} heads of {head_dim} are needed, and out [rows, heads * head_dim]")
+    table = block_table.shape
+    if not (block_table.dtype is torch.int32 and len(table) == 2 and table[0] >= rows and (table[1] > 0 or rows == 0)
+            and block_table.is_contiguous()):
+        raise KernelError(f"{what}: the block table is contiguous int32 [rows, blocks]")
+    if sinks is not None and not (sinks.dtype is torch.float32 and sinks.numel() == heads and sinks.is_contiguous()):
+        raise KernelError(f"{what}: sinks are float32 [heads]")
+    if scratch is not None and not (scratch.dtype is torch.float32 and scratch.is_contiguous()):
+        raise KernelError(f"{what}: scratch must be float32")
 
 
 def store_kv_8bit(qkv: torch.Tensor, slot_mapping: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -74,10 +81,10 @@ def store_kv_8bit(qkv: torch.Tensor, slot_mapping: torch.Tensor, k_pages: torch.
     request's), and a slot occurs once; otherwise the page's contents are undefined."""
     _on_this_device("store_kv_8bit", qkv, slot_mapping, k_pages, v_pages, k_scales, v_scales)
     pages = _cache("store_kv_8bit", k_pages, v_pages, k_scales, v_scales, page_size, kv_heads, head_dim)
-    _require(heads >= 0 and qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1
-             and qkv.shape[1] >= (heads + 2 * kv_heads) * head_dim, "store_kv_8bit: qkv is bfloat16 [rows, (heads + 2 kv_heads) * head_dim]")
-    _require(slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous() and slot_mapping.numel() >= qkv.shape[0],
-             "store_kv_8bit: one int32 slot for each row is needed")
+    if not (heads >= 0 and qkv.dtype is torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= (heads + 2 * kv_heads) * head_dim):
+        raise KernelError("store_kv_8bit: qkv is bfloat16 [rows, (heads + 2 kv_heads) * head_dim]")
+    if not (slot_mapping.dtype is torch.int32 and slot_mapping.is_contiguous() and slot_mapping.numel() >= qkv.shape[0]):
+        raise KernelError("store_kv_8bit: one int32 slot for each row is needed")
     lib = library("eight_bit")
     _check(lib, lib.mir_store_8bit(qkv.data_ptr(), qkv.stride(0), slot_mapping.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                                    k_scales.data_ptr(), v_scales.data_ptr(), qkv.shape[0], page_size, pages, heads, kv_heads, head_dim,
@@ -112,7 +119,8 @@ def decode_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.T
     rows = out.shape[0]
     pages = _cache(what, k_pages, v_pages, k_scales, v_scales, page_size, kv_heads, head_dim)
     _attention(what, qkv, out, block_table, heads, kv_heads, head_dim, rows, sinks, scratch)
-    _require(positions.dtype == torch.int32 and positions.is_contiguous() and positions.numel() >= rows, f"{what}: bad positions")
+    if not (positions.dtype is torch.int32 and positions.is_contiguous() and positions.numel() >= rows):
+        raise KernelError(f"{what}: bad positions")
     lib = library("eight_bit")
     _check(lib, lib.mir_decode_attention_8bit(
         qkv.data_ptr(), qkv.stride(0), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
@@ -136,9 +144,9 @@ def prefill_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.
     rows, tokens = context_lens.numel(), out.shape[0]
     pages = _cache(what, k_pages, v_pages, k_scales, v_scales, page_size, kv_heads, head_dim)
     _attention(what, qkv, out, block_table, heads, kv_heads, head_dim, rows, sinks, None)
-    _require(query_starts.dtype == torch.int32 and context_lens.dtype == torch.int32 and query_starts.numel() == rows + 1
-             and query_starts.is_contiguous() and context_lens.is_contiguous(),
-             f"{what}: query_starts is int32 [requests + 1], context_lens int32 [requests]")
+    if not (query_starts.dtype is torch.int32 and context_lens.dtype is torch.int32 and query_starts.numel() == rows + 1
+            and query_starts.is_contiguous() and context_lens.is_contiguous()):
+        raise KernelError(f"{what}: query_starts is int32 [requests + 1], context_lens int32 [requests]")
     longest = block_table.shape[1] * page_size
     if max_context is not None:
         longest = min(longest, max_context)
@@ -161,20 +169,21 @@ def eight_bit_error() -> int:
     """0 unless a bounded wait of one of the tcgen05 kernels ran out (synchronises the device); such a kernel does no work from
     then on."""
     lib = library("eight_bit")
-    return int(lib.mir_decode_attention_8bit_error() or lib.mir_prefill_attention_8bit_error() or lib.mir_linear_8bit_tiles_error() or lib.mir_linear_8bit_few_error())
+    return int(lib.mir_decode_attention_8bit_error() or lib.mir_prefill_attention_8bit_error()
+               or lib.mir_linear_8bit_tiles_error() or lib.mir_linear_8bit_few_error())
 
 
 def quantize_weight_8bit(weight: torch.Tensor) -> tuple:
     """(values, scales) of a float32 or bfloat16 weight [N, K] for linear_8bit: e4m3 [N, K] and float32 [ceil(N / 128),
     ceil(K / 128)], a block's scale its largest magnitude / 448 (infinities do not count and are held as 448 times it)."""
     _on_this_device("quantize_weight_8bit", weight)
-    _require(weight.dim() == 2 and weight.is_contiguous() and weight.dtype in (torch.float32, torch.bfloat16) and weight.numel() > 0,
-             "quantize_weight_8bit: a contiguous float32 or bfloat16 [rows, columns] is needed")
+    if not (weight.dim() == 2 and weight.is_contiguous() and weight.dtype in (torch.float32, torch.bfloat16) and weight.numel() > 0):
+        raise KernelError("quantize_weight_8bit: a contiguous float32 or bfloat16 [rows, columns] is needed")
     rows, columns = weight.shape
     values = torch.empty((rows, columns), dtype=E4M3, device=weight.device)
     scales = torch.empty((-(-rows // BLOCK), -(-columns // BLOCK)), dtype=torch.float32, device=weight.device)
     lib = library("eight_bit")
-    _check(lib, lib.mir_quantize_weight_8bit(int(weight.dtype == torch.bfloat16), weight.data_ptr(), values.data_ptr(),
+    _check(lib, lib.mir_quantize_weight_8bit(int(weight.dtype is torch.bfloat16), weight.data_ptr(), values.data_ptr(),
                                              scales.data_ptr(), rows, columns, _stream()))
     return values, scales
 
@@ -195,22 +204,25 @@ def linear_8bit(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, out
     Sums are 32-bit.  `out`: bfloat16 or, the only one that accumulates, float32; `bias` has out's dtype.  x and out may be
     row-strided views.  `alloc(shape, dtype)`: where the workspace comes from (torch's caching allocator by default)."""
     _on_this_device("linear_8bit", x, weight, scales, out, bias)
-    _require(x.dim() == 2 and weight.dim() == 2 and x.dtype == torch.bfloat16 and weight.dtype == E4M3,
-             "linear_8bit: x is bfloat16 [M, K], weight float8_e4m3fn [N, K]")
+    if not (x.dim() == 2 and weight.dim() == 2 and x.dtype is torch.bfloat16 and weight.dtype is E4M3):
+        raise KernelError("linear_8bit: x is bfloat16 [M, K], weight float8_e4m3fn [N, K]")
     (m, k), n = x.shape, weight.shape[0]
-    _require(weight.shape[1] == k and out.shape == (m, n) and (x.stride(1) == 1 or m == 0) and (out.stride(1) == 1 or n <= 1 or m == 0)
-             and weight.is_contiguous(), "linear_8bit: shapes or strides do not fit")
-    _require(scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == (-(-n // BLOCK), -(-k // BLOCK)),
-             f"linear_8bit: scales are contiguous float32 [{-(-n // BLOCK)}, {-(-k // BLOCK)}]")
-    _require(out.dtype in (torch.bfloat16, torch.float32) and (out.dtype == torch.float32 or not accumulate),
-             "linear_8bit: out is bfloat16 or float32, and only float32 accumulates")
-    _require(bias is None or (bias.dtype == out.dtype and bias.numel() == n and bias.is_contiguous()),
-             "linear_8bit: bias is [N] of out's dtype")
+    if not (weight.shape[1] == k and out.shape == (m, n) and (x.stride(1) == 1 or m == 0)
+            and (out.stride(1) == 1 or n <= 1 or m == 0) and weight.is_contiguous()):
+        raise KernelError("linear_8bit: shapes or strides do not fit")
+    if not (scales.dtype is torch.float32 and scales.is_contiguous() and scales.shape == (-(-n // BLOCK), -(-k // BLOCK))):
+        raise KernelError(f"linear_8bit: scales are contiguous float32 [{-(-n // BLOCK)}, {-(-k // BLOCK)}]")
+    if not (out.dtype in (torch.bfloat16, torch.float32) and (out.dtype is torch.float32 or not accumulate)):
+        raise KernelError("linear_8bit: out is bfloat16 or float32, and only float32 accumulates")
+    if not (bias is None or (bias.dtype == out.dtype and bias.numel() == n and bias.is_contiguous())):
+        raise KernelError("linear_8bit: bias is [N] of out's dtype")
     if m == 0 or n == 0:
         return
     lib = library("eight_bit")
     size = lib.mir_linear_8bit_workspace(m, k)
-    workspace = alloc((size,), torch.uint8) if alloc is not None else torch.empty((size,), dtype=torch.uint8, device=x.device)
+    workspace = None
+    if size:                    # (up to 16 rows are rounded where they are used)
+        workspace = alloc((size,), torch.uint8) if alloc is not None else torch.empty((size,), dtype=torch.uint8, device=x.device)
     _check(lib, lib.mir_linear_8bit(x.data_ptr(), x.stride(0), weight.data_ptr(), scales.data_ptr(), _ptr(bias), out.data_ptr(),
-                                    out.stride(0), int(out.dtype == torch.float32), int(accumulate), m, n, k, workspace.data_ptr(),
+                                    out.stride(0), int(out.dtype is torch.float32), int(accumulate), m, n, k, _ptr(workspace),
                                     size, _stream()))

@@ -101,7 +101,7 @@ def test_prefill_attention_refuses(change):
                                     dict(out_stride=255), dict(accumulate=1), dict(bytes=100), dict(workspace=None),
                                     dict(workspace=AT + 4), dict(m=-1), dict(n=-1)])
 def test_linear_refuses(change):
-    a = dict(x=AT, x_stride=128, weight=AT, scales=AT, bias=None, out=AT, out_stride=256, out_float=0, accumulate=0, m=5, n=256, k=128,
+    a = dict(x=AT, x_stride=128, weight=AT, scales=AT, bias=None, out=AT, out_stride=256, out_float=0, accumulate=0, m=20, n=256, k=128,
              workspace=AT, bytes=1 << 20, stream=None)
     a.update(change)
     assert kernels.library("eight_bit").mir_linear_8bit(*a.values()) == BAD_ARGUMENT
