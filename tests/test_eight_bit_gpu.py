@@ -448,3 +448,275 @@ def test_quantize_weight(rows, columns, dtype):
             assert scales[i, j].cpu() == scale
             want = (block / scale).clamp(-448, 448).to(E4M3).float()
             assert torch.equal(codes[i * 128:(i + 1) * 128, j * 128:(j + 1) * 128].cpu().float(), want)
+
+
+# ------------------------------------------------------------------------------------------------ together, as they would be used
+def test_a_generation_over_the_8bit_cache():
+    """Two prompts in portions, then decoded tokens: norm and rotation in place, the cache's write, attention over it and the
+    output projection with 8-bit weights, every operator against the plain one on what the GPU gave it."""
+    from libmir_b200 import kernels
+    heads, kv_heads, dim, page, hidden = 8, 2, 128, 16, 512
+    g = seeded(31)
+    lengths = [150, 37]
+    steps = [[100, 37], [50, 0]] + [[1, 1]] * 20                       # tokens of each request in each step
+    batch = Batch(32, [n + 20 for n in lengths], heads, kv_heads, dim, page)
+    batch.k, batch.v = plain.Cache(batch.pool, page, kv_heads, dim), plain.Cache(batch.pool, page, kv_heads, dim)
+    cache = batch.on_gpu()
+    table = batch.table.cuda()
+    weight = torch.randn(hidden, heads * dim, generator=g) * 0.03
+    codes, scales = kernels.quantize_weight_8bit(weight.cuda())
+    values = plain.weight_values(codes.cpu(), scales.cpu())
+    inv_freq = (1e4 ** (-torch.arange(0, dim, 2).float() / dim)).cuda()
+    q_norm, k_norm = (torch.rand(2, dim, generator=g) + 0.5).cuda()
+    done = [0, 0]
+    for counts in steps:
+        positions = [p for r in range(2) for p in range(done[r], done[r] + counts[r])]
+        rows = [r for r in range(2) for _ in range(counts[r])]
+        slots = [int(batch.table[r, p // page]) * page + p % page for r, p in zip(rows, positions)]
+        qkv = (torch.randn(len(rows), (heads + 2 * kv_heads) * dim, generator=g)).bfloat16().cuda()
+        at = torch.tensor(positions, dtype=torch.int32).cuda()
+        kernels.qk_rope_store(qkv, at, None, inv_freq, q_norm, k_norm, None, None, heads, kv_heads, dim, dim, 1e-6, keys_in_place=True)
+        kernels.store_kv_8bit(qkv, torch.tensor(slots, dtype=torch.int32).cuda(), *cache, page, heads, kv_heads, dim)
+        out = torch.empty(len(rows), heads * dim, dtype=torch.bfloat16, device="cuda")
+        done = [d + c for d, c in zip(done, counts)]
+        if max(counts) == 1:
+            plan = kernels.decode_attention_8bit_plan(2, heads, kv_heads, dim, page, 200)
+            kernels.decode_attention_8bit(qkv, out, *cache, table, at, page, heads, kv_heads, dim, 0.088, None, plan[0], plan[1],
+                                          torch.empty(plan[2], device="cuda"))
+        else:
+            starts = torch.tensor([0, counts[0], sum(counts)], dtype=torch.int32).cuda()
+            kernels.prefill_attention_8bit(qkv, out, *cache, table, starts, torch.tensor(done, dtype=torch.int32).cuda(), page, heads,
+                                           kv_heads, dim, 0.088, None)
+        residual = torch.randn(len(rows), hidden, generator=g)
+        result = residual.cuda()
+        kernels.linear_8bit(out, codes, scales, result, accumulate=True)
+        # the same, plainly
+        plain_store(batch, qkv.cpu(), slots)
+        same_cache(batch, cache)
+        wants, sizes = [], []
+        for r in range(2):
+            mine = [i for i in range(len(rows)) if rows[i] == r]
+            q = qkv[mine, :heads * dim].cpu().view(len(mine), heads, dim)
+            o, s = plain.attention(q, batch.k.values(), batch.v.values(), page, batch.table[r].tolist(), [positions[i] for i in mine], 0.088)
+            wants.append(o.flatten(1))
+            sizes.append(s.flatten(1))
+        want, size = torch.cat(wants), torch.cat(sizes)
+        close(out, want, attention_bound(want, size))
+        product = plain.rounded_rows(out.cpu()) @ values.t() + residual.double()
+        close(result, product, product_bound(out.cpu(), values, torch.float32, residual.double())(product))
+    assert kernels.eight_bit_error() == 0
+
+
+def step_calls(batch, cache, qkv, slots, positions, table, codes, scales, out, result, scratch, plan):
+    from libmir_b200 import kernels
+    kernels.store_kv_8bit(qkv, slots, *cache, batch.page, batch.heads, batch.kv_heads, batch.dim)
+    kernels.decode_attention_8bit(qkv, out, *cache, table, positions, batch.page, batch.heads, batch.kv_heads, batch.dim, 0.09, None,
+                                  plan[0], plan[1], scratch)
+    kernels.linear_8bit(out, codes, scales, result)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_captured_step_replayed_for_growing_contexts(dim):
+    """Two graphs of a decode step over caches of their own, replayed in turn with new positions, slots and queries, against eager
+    calls: captured when contexts were short, replayed when they are long and a row has become padding."""
+    from libmir_b200 import kernels
+    heads, kv_heads, page, rows = 8, 2, 16, 3
+    g = seeded(41)
+    codes = (torch.randn(256, heads * dim, generator=g) * 100).clamp(-448, 448).to(E4M3).cuda()
+    scales = (torch.rand(2, -(-heads * dim // 128), generator=g) * 1e-3).cuda()
+    plan = kernels.decode_attention_8bit_plan(rows, heads, kv_heads, dim, page, 900)
+    made = []
+    for seed in (42, 43):
+        batch = Batch(seed, [900, 700, 800], heads, kv_heads, dim, page)
+        held = dict(cache=batch.on_gpu(), qkv=torch.zeros(rows, (heads + 2 * kv_heads) * dim, dtype=torch.bfloat16, device="cuda"),
+                    slots=torch.full((rows,), -1, dtype=torch.int32, device="cuda"), table=batch.table.cuda(),
+                    positions=torch.zeros(rows, dtype=torch.int32, device="cuda"), codes=codes, scales=scales,
+                    out=torch.zeros(rows, heads * dim, dtype=torch.bfloat16, device="cuda"), result=torch.zeros(rows, 256, device="cuda"),
+                    scratch=torch.empty(plan[2], device="cuda") if plan[2] else None, plan=plan)
+        eager = dict(held, cache=tuple(t.clone() for t in held["cache"]), out=held["out"].clone(), result=held["result"].clone(),
+                     scratch=torch.empty(plan[2], device="cuda") if plan[2] else None)
+        step_calls(batch, **{**held, "cache": tuple(t.clone() for t in held["cache"])})        # (warm)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step_calls(batch, **held)
+        made.append((batch, held, eager, graph))
+    for positions in ([3, 0, 17], [130, 128, 255], [899, -1, 400], [512, 699, -1]):
+        for batch, held, eager, graph in made:
+            held["qkv"].copy_(torch.randn(held["qkv"].shape, generator=g).bfloat16())
+            held["positions"].copy_(torch.tensor(positions, dtype=torch.int32))
+            held["slots"].copy_(torch.tensor([int(batch.table[r, p // page]) * page + p % page if p >= 0 else -1
+                                              for r, p in enumerate(positions)], dtype=torch.int32))
+            graph.replay()
+            step_calls(batch, **eager)
+        torch.cuda.synchronize()
+        for batch, held, eager, _ in made:
+            for name in ("out", "result"):
+                assert torch.equal(held[name], eager[name]), name
+            for a, b in zip(held["cache"], eager["cache"]):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert kernels.eight_bit_error() == 0
+
+
+def test_calls_on_two_streams_at_once():
+    """The same step on two streams, each with tensors of its own, gives what it gives alone."""
+    from libmir_b200 import kernels
+    heads, kv_heads, dim, page, rows = 8, 2, 128, 16, 3
+    g = seeded(51)
+    codes = (torch.randn(640, heads * dim, generator=g) * 100).clamp(-448, 448).to(E4M3).cuda()
+    scales = (torch.rand(5, heads, generator=g) * 1e-3).cuda()
+    plan = kernels.decode_attention_8bit_plan(rows, heads, kv_heads, dim, page, 3000)
+    held = []
+    for seed in (52, 53):
+        batch = Batch(seed, [3000, 200, 1700], heads, kv_heads, dim, page)
+        positions = [2999, 199, 1699]
+        slots = [int(batch.table[r, p // page]) * page + p % page for r, p in enumerate(positions)]
+        def state():
+            return dict(cache=batch.on_gpu(), qkv=batch.qkv[:rows].cuda(), slots=torch.tensor(slots, dtype=torch.int32).cuda(),
+                        table=batch.table.cuda(), positions=torch.tensor(positions, dtype=torch.int32).cuda(), codes=codes, scales=scales,
+                        out=torch.zeros(rows, heads * dim, dtype=torch.bfloat16, device="cuda"), result=torch.zeros(rows, 640, device="cuda"),
+                        scratch=torch.empty(plan[2], device="cuda"), plan=plan)
+        held.append((batch, state(), state()))
+    for batch, alone, _ in held:
+        step_calls(batch, **alone)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for stream, (batch, _, both) in zip(streams, held):
+            with torch.cuda.stream(stream):
+                step_calls(batch, **both)
+    torch.cuda.synchronize()
+    for batch, alone, both in held:
+        assert torch.equal(alone["out"], both["out"]) and torch.equal(alone["result"], both["result"])
+    assert kernels.eight_bit_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+@pytest.mark.parametrize("dim", [64, 128])
+def test_pages_beyond_two_gigabytes(dim):
+    """Pages at the end of a pool of more than 2^31 bytes: written and read as at its beginning."""
+    from libmir_b200 import kernels
+    heads, kv_heads, page = 16, 8, 16
+    pool = (1 << 31) // (page * kv_heads * dim) + 5000
+    batch = Batch(61, [600, 90], heads, kv_heads, dim, page)
+    small = batch.on_gpu()
+    shift = pool - batch.pool
+    large = tuple(torch.zeros((pool * page, kv_heads, dim), dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2)) \
+        + tuple(torch.zeros((pool, kv_heads), device="cuda") for _ in range(2))
+    for a, b in zip(small[:2], large[:2]):
+        b.view(torch.uint8)[shift * page:] = a.view(torch.uint8)
+    for a, b in zip(small[2:], large[2:]):
+        b[shift:] = a
+    far = torch.where(batch.table >= 0, batch.table + shift, batch.table)
+    qkv = batch.qkv[:40].cuda()
+    for r in range(2):
+        last = batch.lengths[r] - 1
+        for cache, table in ((small, batch.table), (large, far)):
+            slots = [int(table[r, p // page]) * page + p % page for p in range(last - 19, last + 1)]
+            kernels.store_kv_8bit(qkv[r * 20:r * 20 + 20], torch.tensor(slots, dtype=torch.int32).cuda(), *cache, page, heads, kv_heads, dim)
+    for a, b in zip(small[:2], large[:2]):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)[shift * page:]) and not b.view(torch.uint8)[:1000].any()
+    for a, b in zip(small[2:], large[2:]):
+        assert torch.equal(a, b[shift:])
+    positions = [599, 89]
+    near = run_decode(batch, small, positions, 0.1, table=batch.table.cuda())
+    assert torch.equal(near, run_decode(batch, large, positions, 0.1, table=far.cuda()))
+    batch.table = far
+    over = run_prefill(batch, large, [300, 50], 0.1)
+    batch.table = far - shift * (far >= 0).int()
+    assert torch.equal(over, run_prefill(batch, small, [300, 50], 0.1))
+
+
+def test_products_beyond_two_to_the_31():
+    """More than 2^31 elements of x and of the result: the last rows are right."""
+    from libmir_b200 import kernels
+    g = seeded(71)
+    m, k, n = 70000, 32768, 136
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = torch.randn(3, k, generator=g).bfloat16().cuda()
+    codes = (torch.randn(n, k, generator=g) * 100).clamp(-448, 448).to(E4M3)
+    scales = torch.rand(2, k // 128, generator=g) * 1e-3
+    weight = plain.weight_values(codes, scales)
+    out = torch.full((m, n), 3.0, device="cuda")
+    kernels.linear_8bit(x, codes.cuda(), scales.cuda(), out)
+    want = plain.rounded_rows(x[-3:].cpu()) @ weight.t()
+    close(out[-3:], want, product_bound(x[-3:].cpu(), weight, torch.float32, torch.zeros(1, dtype=torch.float64))(want))
+    assert (out[:-3] == 0).all()
+    del x, out
+    m, k, n = 40000, 128, 60000
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[-1] = torch.randn(k, generator=g).bfloat16().cuda()
+    codes = (torch.randn(n, k, generator=g) * 100).clamp(-448, 448).to(E4M3)
+    scales = torch.rand(-(-n // 128), 1, generator=g) * 1e-3
+    out = torch.full((m, n), 3.0, dtype=torch.bfloat16, device="cuda")
+    kernels.linear_8bit(x, codes.cuda(), scales.cuda(), out)
+    weight = plain.weight_values(codes, scales)
+    want = plain.rounded_rows(x[-1:].cpu()) @ weight.t()
+    close(out[-1:], want, product_bound(x[-1:].cpu(), weight, torch.bfloat16, torch.zeros(1, dtype=torch.float64))(want))
+    assert (out[-2] == 0).all() and (out[0] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_refusals_of_tensors_that_do_not_fit():
+    from libmir_b200 import kernels
+    from libmir_b200.errors import KernelError
+    batch = Batch(81, [40], 4, 2, 64, 16)
+    cache = batch.on_gpu()
+    qkv = batch.qkv[:1].cuda()
+    slots = torch.zeros(1, dtype=torch.int32).cuda()
+    k, v, ks, vs = cache
+
+    def store(**c):
+        a = dict(qkv=qkv, slots=slots, k=k, v=v, ks=ks, vs=vs, page=16, heads=4, kv_heads=2, dim=64)
+        a.update(c)
+        kernels.store_kv_8bit(*a.values())
+    store()
+    for change in (dict(k=k.view(torch.uint8)), dict(v=v[:-16]), dict(ks=ks[:-1]), dict(vs=vs.double()), dict(page=7), dict(kv_heads=1),
+                   dict(dim=32), dict(qkv=qkv.float()), dict(qkv=qkv[:, :-1]), dict(slots=slots.long()), dict(slots=slots[:0]),
+                   dict(k=k.cpu()), dict(qkv=qkv.t().contiguous().t() if qkv.shape[0] > 1 else qkv[0])):
+        with pytest.raises((KernelError, IndexError)):
+            store(**change)
+    table, positions = batch.table.cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+    out = torch.empty(1, 256, dtype=torch.bfloat16, device="cuda")
+
+    def decode(**c):
+        plan = kernels.decode_attention_8bit_plan(1, 4, 2, 64, 16, 40)
+        a = dict(qkv=qkv, out=out, k=k, v=v, ks=ks, vs=vs, table=table, positions=positions, page=16, heads=4, kv_heads=2, dim=64,
+                 scale=0.1, window=None, partition=plan[0], parts=plan[1], scratch=None, sinks=None)
+        a.update(c)
+        kernels.decode_attention_8bit(*a.values())
+    decode()
+    for change in (dict(out=out.float()), dict(out=out[:, :128]), dict(table=table.long()), dict(table=table[:0]), dict(positions=positions[:0]),
+                   dict(heads=3), dict(scale=0.0), dict(window=-3), dict(parts=2), dict(sinks=torch.zeros(3, device="cuda")),
+                   dict(sinks=torch.zeros(4)), dict(partition=0), dict(k=k[..., :32]), dict(scratch=torch.zeros(8))):
+        with pytest.raises(KernelError):
+            decode(**change)
+    starts, contexts = torch.tensor([0, 1], dtype=torch.int32).cuda(), torch.tensor([40], dtype=torch.int32).cuda()
+
+    def prefill(**c):
+        a = dict(qkv=qkv, out=out, k=k, v=v, ks=ks, vs=vs, table=table, starts=starts, contexts=contexts, page=16, heads=4, kv_heads=2,
+                 dim=64, scale=0.1, window=None)
+        a.update(c)
+        kernels.prefill_attention_8bit(*a.values())
+    prefill()
+    for change in (dict(starts=starts[:1]), dict(contexts=contexts.long()), dict(starts=starts.cpu()), dict(out=out[:, ::2]),
+                   dict(qkv=qkv[:, 1:]), dict(scale=-1.0), dict(page=3)):
+        with pytest.raises(KernelError):
+            prefill(**change)
+    codes, scales = torch.zeros(200, 128).to(E4M3).cuda(), torch.ones(2, 1).cuda()
+    x, result = torch.zeros(3, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(3, 200, device="cuda")
+
+    def linear(**c):
+        a = dict(x=x, weight=codes, scales=scales, out=result, bias=None, accumulate=False)
+        a.update(c)
+        kernels.linear_8bit(*a.values())
+    linear()
+    for change in (dict(x=x.float()), dict(x=x[:, :64]), dict(weight=codes[:, :120].contiguous(), x=x[:, :120].contiguous()),
+                   dict(scales=scales.t()), dict(scales=scales.double()), dict(out=result[:, :100]), dict(out=result.bfloat16(), accumulate=True),
+                   dict(out=result.half()), dict(bias=torch.zeros(200, dtype=torch.bfloat16, device="cuda")), dict(bias=torch.zeros(199, device="cuda")),
+                   dict(weight=codes.view(torch.uint8)), dict(x=x.cpu()), dict(weight=torch.zeros(128, 200).to(E4M3).cuda().t())):
+        with pytest.raises(KernelError):
+            linear(**change)
+    linear(x=x[:0], out=result[:0])
+    with pytest.raises(KernelError):
+        kernels.quantize_weight_8bit(torch.zeros(4, 4, dtype=torch.float16, device="cuda"))
