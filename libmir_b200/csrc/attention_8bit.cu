@@ -56,13 +56,14 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
                       const int* __restrict__ block_table, int table_width, const int* __restrict__ positions,
                       const int* __restrict__ query_starts, const int* __restrict__ context_lens, int num_rows, int group,
                       float scale_log2, int window, int partition, int num_partitions, float* __restrict__ partial_o,
-                      float* __restrict__ partial_ml, const float* __restrict__ sinks) {
+                      float* __restrict__ partial_ml, const float* __restrict__ sinks, int all_tokens) {
   constexpr int kStride = DIM + 8;              // bf16 elements of a shared row: an odd number of 16-byte pieces
   constexpr int kPieces = DIM / 16;             // 16-byte pieces of a cached row
   constexpr int kRounds = kKeys * kPieces / kThreads;
   __shared__ __align__(16) bf16 k_tile[kKeys * kStride];
   __shared__ __align__(16) bf16 v_tile[kKeys * kStride];
   __shared__ unsigned long long there_bits[2];  // [tile parity]: keys of the tile whose page the table has
+  __shared__ int hidden_nans;                   // whether NaN values were left out that some of the rows see
   grid_dependency_wait();
   grid_launch_dependents();
   const int part = blockIdx.x % num_partitions, tile = blockIdx.x / num_partitions, kv_head = blockIdx.y;
@@ -78,15 +79,15 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
   } else {
     int remaining = tile;
     for (int r = 0; r < num_rows; ++r) {
-      const int tokens = query_starts[r + 1] - query_starts[r];
-      const int tiles = (tokens * group + kRows - 1) / kRows;
+      const int tiles = (portion_of(query_starts, r, all_tokens).count * group + kRows - 1) / kRows;
       if (remaining < tiles) { request = r; break; }
       remaining -= tiles;
     }
     if (request < 0) return;
+    const Portion portion = portion_of(query_starts, request, all_tokens);
     first_row = remaining * kRows;
-    first_token = query_starts[request];
-    count = query_starts[request + 1] - first_token;
+    first_token = portion.first;
+    count = portion.count;
     first_position = context_lens[request] - count;
   }
   const int rows = min(kRows, count * group - first_row);
@@ -163,7 +164,10 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
     to[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
   };
 
-  if (threadIdx.x == 0) there_bits[0] = 0ull;
+  if (threadIdx.x == 0) {
+    there_bits[0] = 0ull;
+    hidden_nans = 0;
+  }
   if (from < end) fetch(from);
   int parity = 0;
   for (int key0 = from; key0 < end; key0 += kKeys, parity ^= 1) {
@@ -173,6 +177,14 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
     for (int i = 0; i < kRounds; ++i) {
       const int piece = threadIdx.x + i * kThreads;
       put(k_tile, k_raw[i], k_scale[i], piece);
+      if (nan_bytes(v_raw[i].x) | nan_bytes(v_raw[i].y) | nan_bytes(v_raw[i].z) | nan_bytes(v_raw[i].w)) {
+        // a weight of 0 times NaN would be NaN for the rows that do not see the key: it is left out here and put in at the end
+        const int key = key0 + piece / kPieces;
+        if (key > lowest || (window > 0 && key <= highest - window)) {
+          v_raw[i] = make_uint4(without_nans(v_raw[i].x), without_nans(v_raw[i].y), without_nans(v_raw[i].z), without_nans(v_raw[i].w));
+          hidden_nans = 1;
+        }
+      }
       put(v_tile, v_raw[i], v_scale[i], piece);
       if ((there >> i & 1u) && piece % kPieces == 0) mine |= 1ull << (piece / kPieces);
     }
@@ -241,6 +253,21 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
       }
   }
 
+  if (from < end && hidden_nans) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      for (int key = max(from, window > 0 ? position[i] - window + 1 : 0); key < end && key <= position[i]; ++key) {
+        if (key <= lowest && (window == 0 || key > highest - window)) continue;         // (every row sees it: left in)
+        const int block = key / cache.page_size, page = page_of_block(table, table_width, block, cache.pages);
+        if (page < 0) continue;
+        const uint8_t* codes = cache.v + (((size_t)page * cache.page_size + (key - block * cache.page_size)) * cache.kv_heads + kv_head) * DIM;
+#pragma unroll
+        for (int n = 0; n < DIM / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if ((codes[n * 8 + (lane & 3) * 2 + j] & 0x7f) == 0x7f) o[n][2 * i + j] = __int_as_float(0x7fffffff);
+      }
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float total = quad_sum(sum[i]);
@@ -326,7 +353,7 @@ int mir_attention_8bit_general(const Attention8& a, int tokens) {
                                 dim3(kThreads), 0, a.stream, 0, (const bf16*)a.q, a.q_stride, (bf16*)a.out, a.cache, a.block_table,
                                 a.table_width, a.positions, a.query_starts, a.context_lens, a.num_rows, group,
                                 a.scale * kLog2e, a.window, a.partition, a.num_partitions, a.partial_o(tokens), a.partial_ml(tokens),
-                                a.sinks);
+                                a.sinks, tokens);
   if (status != MIR_OK || a.num_partitions == 1) return status;
   return mir_merge_8bit(a, tokens);
 }

@@ -363,7 +363,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
                         __uint_as_float(raw[h].y & 0xffff0000u)};
           const float largest = warp_largest(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
           const int e = least_scale_exponent(fminf(largest, 3.38953139e38f));
-          const float inverse = power_of_two(-e);
+          const float inverse = query_inverse(largest, e);
           uint32_t hi[2], lo[2];
           split_e4m3_e5m2(x[0] * inverse, x[1] * inverse, hi[0], lo[0]);
           split_e4m3_e5m2(x[2] * inverse, x[3] * inverse, hi[1], lo[1]);
@@ -413,6 +413,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
       }
       if (++stage == (uint32_t)kStages) { stage = 0; parity ^= 1u; }
     }
+    wait_for_copies(full0, (uint32_t)kStages, stage, parity);
   } else if (warp == kIssuer) {
     // ------------------------------------------------------------------ issuer (tcgen05.cuh: from a whole warp)
     constexpr uint32_t scores_hi = instruction_descriptor_8bit(kKeys, kHeads, E4M3, E4M3);

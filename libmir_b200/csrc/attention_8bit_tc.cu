@@ -16,10 +16,11 @@
 // times the page's scale puts that right.  Both products take as long as they would in bf16; the schedulers' slots bound the kernel.
 //
 // Roles: a scout reads block table and scales ahead and leaves them in shared memory; two loaders (TMA) for keys and values; an
-// issuer; four warps that split queries and widen values; two streams of eight softmax warps that take the tiles in turn, with a
+// issuer; eight warps that split queries and widen values; two streams of eight softmax warps that take the tiles in turn, with a
 // running reference that they hand to each other (raised when a tile's maximum exceeds it by 2^8), three score accumulators and
 // one for the output, which a stream that raises the reference rescales when the product of the tile before is over.
-// A hidden key's score becomes -inf by selection; rows of values that no query of the item sees are written as zeros.
+// A hidden key's score becomes -inf by selection; rows of values that no query of the item sees are written as zeros, and so are NaN
+// values that only some of its queries see (0 times NaN is NaN): those queries get them when the item is over.
 #include <algorithm>
 #include "eight_bit_tc.cuh"
 
@@ -76,7 +77,7 @@ struct Work {
 struct Items {
   const int* query_starts;
   const int* context_lens;
-  int num_rows, kv_heads, group, window, partition, num_partitions, row_tiles, count;
+  int num_rows, tokens, kv_heads, group, window, partition, num_partitions, row_tiles, count;
   // Item `index`: the kv head is the fast index, then the partition, then the batch's tiles of rows from the last one of the last request
   // backwards (late tiles see the most keys and come first).  False beyond the last item.
   __device__ __forceinline__ bool at(int index, Work& w) const {
@@ -86,18 +87,18 @@ struct Items {
     w.part = rest % num_partitions;
     int remaining = row_tiles - 1 - rest / num_partitions;
     w.request = -1;
-    int tokens = 0;
+    Portion portion{0, 0};
     for (int r = 0; r < num_rows; ++r) {
-      tokens = query_starts[r + 1] - query_starts[r];
-      const int tiles = (tokens * group + kRows - 1) / kRows;
+      portion = portion_of(query_starts, r, tokens);
+      const int tiles = (portion.count * group + kRows - 1) / kRows;
       if (remaining < tiles) { w.request = r; break; }
       remaining -= tiles;
     }
     if (w.request < 0) return false;
     w.first_row = remaining * kRows;
-    w.rows = min(kRows, tokens * group - w.first_row);
-    w.first_token = query_starts[w.request];
-    const int start = context_lens[w.request] - tokens;
+    w.rows = min(kRows, portion.count * group - w.first_row);
+    w.first_token = portion.first;
+    const int start = context_lens[w.request] - portion.count;
     w.first_position = start + w.first_row / group;
     w.last_position = start + (w.first_row + w.rows - 1) / group;
     w.first_key = (window > 0 && w.first_position >= window) ? w.first_position + 1 - window : 0;
@@ -204,7 +205,11 @@ __device__ __forceinline__ float softmax_tile(uint32_t scores, int first, int lo
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       const int c = c8 + i;
-      const float p0 = approximate_exp2(fmaf(v[c], k_scale, down)), p1 = approximate_exp2(fmaf(v[c + 1], k_scale, down));
+      float p0 = approximate_exp2(fmaf(v[c], k_scale, down)), p1 = approximate_exp2(fmaf(v[c + 1], k_scale, down));
+      if (MASKED) {                                                        // (the scales' product may be 0: no -inf times that)
+        p0 = v[c] == -INFINITY ? 0.0f : p0;
+        p1 = v[c + 1] == -INFINITY ? 0.0f : p1;
+      }
       sums[(c >> 1) & 3] += p0 + p1;
       const __nv_bfloat162 both = __floats2bfloat162_rn(p0, p1);
       packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&both);
@@ -217,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                     const __grid_constant__ CUtensorMap k_tile_map, const __grid_constant__ CUtensorMap v_tile_map, const bf16* __restrict__ q,
                     long long q_stride, Cache8 cache, const int* __restrict__ block_table, int table_width,
-                    const int* __restrict__ query_starts, const int* __restrict__ context_lens, int num_rows, int heads, float scale_log2,
+                    const int* __restrict__ query_starts, const int* __restrict__ context_lens, int num_rows, int tokens, int heads, float scale_log2,
                     int window, int partition, int num_partitions, float* __restrict__ partial_o, float* __restrict__ partial_ml,
                     bf16* __restrict__ out, const float* __restrict__ sinks) {
   extern __shared__ unsigned char smem_raw[];
@@ -230,6 +235,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   __shared__ float denominators[2][kStreams][kParts][kRows];
   __shared__ float references[2][kStreams][kRows];
   __shared__ float handed[2][kRows];                        // a row's reference after tile g, by g & 1
+  __shared__ int hidden_nans[4];                            // by n & 3: n + 1 if NaN values were left out that some rows of item n see
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
@@ -253,9 +259,10 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   grid_dependency_wait();
   if (threadIdx.x == 0) {
     int total = 0;
-    for (int r = 0; r < num_rows; ++r) total += ((query_starts[r + 1] - query_starts[r]) * group + kRows - 1) / kRows;
+    for (int r = 0; r < num_rows; ++r) total += (portion_of(query_starts, r, tokens).count * group + kRows - 1) / kRows;
     if (*reinterpret_cast<volatile int*>(&g_error) != 0) total = 0;       // an earlier wait ran out: nothing is begun
     row_tiles_slot = total;
+    for (int i = 0; i < 4; ++i) hidden_nans[i] = 0;
   }
   tensor_fence_before_sync();
   __syncthreads();
@@ -263,9 +270,14 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   grid_launch_dependents();
   const uint32_t tmem = tmem_slot, tmem_o = tmem + 384u;
   const int shift = 31 - __clz(cache.page_size);            // pages are powers of two
-  const Items items{query_starts, context_lens, num_rows, cache.kv_heads, group, window, partition, num_partitions, row_tiles_slot,
+  const Items items{query_starts, context_lens, num_rows, tokens, cache.kv_heads, group, window, partition, num_partitions, row_tiles_slot,
                     row_tiles_slot * cache.kv_heads * num_partitions};
   const int cta = blockIdx.x, ctas = gridDim.x;
+  // whether all queries of an item see all keys of its tile t (that are there)
+  auto seen_by_all = [&](const Work& of, int t) {
+    const int key0 = of.begin + t * kKeys;
+    return key0 + kKeys - 1 <= of.first_position && (window == 0 || of.last_position - window + 1 <= key0);
+  };
   auto more = [&](int k) { return (long long)k * ctas < items.count; };
   Work w;
 
@@ -343,6 +355,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           ring.step(3);
         }
       }
+      wait_for_copies(bar(full0), 3u, ring.stage, ring.phase);
     } else {
       // ---------------------------------------------------------------- issuer (tcgen05.cuh: from a whole warp)
       constexpr uint32_t scores_hi = instruction_descriptor_8bit(kRows, kKeys, E4M3, E4M3);
@@ -439,7 +452,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                               __uint_as_float(held[i].y & 0xffff0000u)};
           const float largest = warp_largest(max_of_three(fmaxf(fabsf(x[0]), fabsf(x[1])), fabsf(x[2]), fabsf(x[3])));
           const int e = least_scale_exponent(fminf(largest, 3.38953139e38f));
-          const float inverse = power_of_two(-e);
+          const float inverse = query_inverse(largest, e);
           uint32_t hi[2], lo[2];
           split_e4m3_e5m2(x[0] * inverse, x[1] * inverse, hi[0], lo[0]);
           split_e4m3_e5m2(x[2] * inverse, x[3] * inverse, hi[1], lo[1]);
@@ -463,7 +476,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         // thread: 16 bytes (j) of every 32nd row (whose place in the swizzle is the same), two at a time
         const int j = thread & 7, r0 = thread >> 3;
         const bool all_seen = infos[info].whole && w.begin + t * kKeys >= w.first_key && w.begin + (t + 1) * kKeys <= w.end;
-        const bool one_factor = infos[info].one_factor;
+        const bool one_factor = infos[info].one_factor, hides = !seen_by_all(w, t);
         from += r0 * 128 + ((j ^ (r0 & 7)) << 4);
         unsigned char* low = to + (j >> 2) * kHalf + r0 * 128 + ((((j & 3) * 2) ^ (r0 & 7)) << 4);
         unsigned char* high = to + (j >> 2) * kHalf + r0 * 128 + ((((j & 3) * 2 + 1) ^ (r0 & 7)) << 4);
@@ -495,12 +508,14 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             }
             if ((last & 0x80808080u) != 0u || !one_factor) {       // (rare: the lifted number of a NaN is 480; a scale beyond one bf16 factor)
               const uint32_t rest = infos[info].v_rest[r >> shift];
+              // a weight of 0 times NaN would be NaN for the rows that do not see the key: it is left out here and put in at the end
+              if (hides && (last & 0x80808080u) != 0u) hidden_nans[(n - 1) & 3] = n;
 #pragma unroll
               for (int c = 0; c < 8; ++c) {
                 wide[c] = times(wide[c], rest);
                 const uint32_t pair = words[c / 2] >> (16 * (c & 1));
-                if ((pair & 0x7fu) == 0x7fu) wide[c] |= 0x7fffu;
-                if ((pair & 0x7f00u) == 0x7f00u) wide[c] |= 0x7fff0000u;
+                if ((pair & 0x7fu) == 0x7fu) wide[c] = hides ? wide[c] & 0xffff0000u : wide[c] | 0x7fffu;
+                if ((pair & 0x7f00u) == 0x7f00u) wide[c] = hides ? wide[c] & 0xffffu : wide[c] | 0x7fff0000u;
               }
             }
             *reinterpret_cast<uint4*>(low + (base + i * kStep) * 128) = make_uint4(wide[0], wide[1], wide[2], wide[3]);
@@ -555,8 +570,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         tensor_fence_after_sync();
         const uint32_t scores = tmem + (uint32_t)stage * 128u + lane_bits;
         const int high = min(position, w.end - 1) - key0, low = window > 0 ? position - window + 1 - key0 : -1;
-        const bool every = infos[info].whole && key0 + kKeys - 1 <= w.first_position && key0 + kKeys <= w.end &&
-                           (window == 0 || w.last_position - window + 1 <= key0);
+        const bool every = infos[info].whole && key0 + kKeys <= w.end && seen_by_all(w, t);
         uint32_t packed[kCols / 2];
         bool grow;
         float factor, own_factor;
@@ -602,9 +616,9 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       float total = 0.0f;
 #pragma unroll
       for (int other = 0; other < kStreams; ++other) {
-        const float theirs = references[slot][other][r];     // -inf: that stream saw no key of this row
-        if (theirs > -INFINITY)
-          total += (denominators[slot][other][0][r] + denominators[slot][other][1][r]) * approximate_exp2(theirs - top);
+        // (0: that stream saw no key of this row; NaN beside a reference of -inf: nothing else)
+        const float theirs = references[slot][other][r], sum = denominators[slot][other][0][r] + denominators[slot][other][1][r];
+        if (sum != 0.0f) total += sum * approximate_exp2(theirs - top);
       }
       if (alive && !wait_barrier(bar(ITEM_DONE), (uint32_t)n & 1u)) { g_error = 3; alive = false; }
       __syncwarp();
@@ -615,6 +629,25 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       tmem_load_32(tmem_o + lane_bits + (uint32_t)column, o);
       tensor_fence_before_sync();
       barrier_arrive(bar(O_FREE));                           // (the next item's products may overwrite it)
+      if (hidden_nans[n & 3] == n + 1) {
+        const int* table = block_table + (size_t)w.request * table_width;
+        const int last = min(position, w.end - 1);
+#pragma unroll 1
+        for (int key = max(w.begin, window > 0 ? position - window + 1 : 0); key <= last; ++key) {
+          if (seen_by_all(w, (key - w.begin) / kKeys)) continue;                                // (left in)
+          const int page = page_of_block(table, table_width, key >> shift, cache.pages);
+          if (page < 0) continue;
+          const uint32_t* codes = reinterpret_cast<const uint32_t*>(
+              cache.v + ((((size_t)page << shift) + (key & (cache.page_size - 1))) * cache.kv_heads + w.kv_head) * kDim + column);
+#pragma unroll
+          for (int i = 0; i < kOut; i += 4) {
+            const uint32_t nans = nan_bytes(codes[i / 4]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (nans >> (8 * j + 7) & 1u) o[i + j] = __int_as_float(0x7fffffff);
+          }
+        }
+      }
       if (r < w.rows && alive) {
         if (num_partitions == 1) {
           if (total != 0.0f && sinks != nullptr) total += exp2f(sinks[head] * kLog2e - top);
@@ -680,7 +713,7 @@ int mir_attention_8bit_prefill(const Attention8& a, int tokens) {
   if (status != MIR_OK) return status;
   status = mir_launch("prefill_attention_8bit", prefill_8bit_kernel, dim3((unsigned)std::min<long long>(items, mir_sm_count())), dim3(kThreads),
                       (size_t)kSmemBytes, a.stream, 0, maps[0], maps[1], maps[2], maps[3], (const bf16*)a.q, a.q_stride, a.cache, a.block_table,
-                      a.table_width, a.query_starts, a.context_lens, a.num_rows, a.heads, a.scale * kLog2e, a.window, a.partition,
+                      a.table_width, a.query_starts, a.context_lens, a.num_rows, tokens, a.heads, a.scale * kLog2e, a.window, a.partition,
                       a.num_partitions, a.partial_o(tokens), a.partial_ml(tokens), (bf16*)a.out, a.sinks);
   if (status != MIR_OK || a.num_partitions == 1) return status;
   return mir_merge_8bit(a, tokens);

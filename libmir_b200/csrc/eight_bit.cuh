@@ -57,6 +57,24 @@ __device__ __forceinline__ float approximate_exp2(float x) {
   return y;
 }
 
+// A word of e4m3 numbers: whether one of them is NaN; and with zeros in the places of those that are.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t word) { return ((word & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ uint32_t without_nans(uint32_t word) { return word & ~((nan_bytes(word) >> 7) * 0xffu); }
+
+// The inverse of a query row's scale 2^e for splitting it: NaN where the row holds an infinity, whose scores are no numbers.
+__device__ __forceinline__ float query_inverse(float largest, int e) {
+  return largest < INFINITY ? power_of_two(-e) : __int_as_float(0x7fffffff);
+}
+
+// The tokens of request r among `tokens` rows; what lies beyond them is cut off.
+struct Portion {
+  int first, count;
+};
+__device__ __forceinline__ Portion portion_of(const int* query_starts, int r, int tokens) {
+  const int first = min(max(query_starts[r], 0), tokens);
+  return {first, max(0, min(query_starts[r + 1], tokens) - first)};
+}
+
 // The paged 8-bit cache of one layer.
 struct Cache8 {
   const uint8_t* k;              // [pages * page_size, kv_heads, head_dim]

@@ -34,20 +34,12 @@ __device__ __forceinline__ void mma_8bit_ss_halves(uint32_t tmem_d, uint32_t a_l
 }
 
 // Tensor map of a row-major matrix [rows, columns] of bytes, bf16 or float32 with row stride `ld` bytes (a multiple of 16): boxes of
-// box_rows rows x box_bytes (64 or 128) with the swizzle of that width, out-of-range elements read as zero and not written.  A map says no more than its
-// arguments do, and is looked up by all of them.
+// box_rows rows x box_bytes (64 or 128) with the swizzle of that width, out-of-range elements read as zero and not written.
 inline int tensor_map_of(const void* base, CUtensorMapDataType type, int width, long long rows, long long columns, long long ld,
                          int box_rows, int box_bytes, CUtensorMap* map) {
   static std::mutex g_mutex;
   static EncodeTiled g_encode = nullptr;
-  static std::map<std::tuple<const void*, int, long long, long long, long long, int, int>, CUtensorMap> g_maps;
-  std::lock_guard<std::mutex> lock(g_mutex);
-  const auto key = std::make_tuple(base, (int)type, rows, columns, ld, box_rows, box_bytes);
-  const auto found = g_maps.find(key);
-  if (found != g_maps.end()) {
-    *map = found->second;
-    return MIR_OK;
-  }
+  std::unique_lock<std::mutex> lock(g_mutex);
   if (g_encode == nullptr) {
     void* entry = nullptr;
     cudaDriverEntryPointQueryResult result;
@@ -58,12 +50,13 @@ inline int tensor_map_of(const void* base, CUtensorMapDataType type, int width, 
     }
     g_encode = reinterpret_cast<EncodeTiled>(entry);
   }
+  const EncodeTiled encode = g_encode;
+  lock.unlock();
   const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)ld};
   const cuuint32_t box[2] = {(cuuint32_t)(box_bytes / width), (cuuint32_t)box_rows};
   const cuuint32_t element_strides[2] = {1, 1};
-  CUtensorMap made;
-  const CUresult status = g_encode(&made, type, 2, const_cast<void*>(base), dims, strides, box, element_strides,
+  const CUresult status = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, element_strides,
                                    CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -72,9 +65,6 @@ inline int tensor_map_of(const void* base, CUtensorMapDataType type, int width, 
                   ld, (int)status);
     return MIR_LIBRARY_ERROR;
   }
-  if (g_maps.size() > 4096) g_maps.clear();
-  g_maps.emplace(key, made);
-  *map = made;
   return MIR_OK;
 }
 inline int tensor_map_of_bytes(const void* base, long long rows, long long bytes, long long ld, int box_rows, CUtensorMap* map) {
@@ -104,6 +94,12 @@ inline int reserve_shared(Kernel kernel, int bytes, const char* what) {
     return MIR_CUDA_ERROR;
   }
   return MIR_OK;
+}
+
+// The end of a loader whose next copy would go to `stage` of a ring in `phase`: the last copies into every stage are waited for (their
+// readers did already, unless one gave up), so that none is on its way when the CTA ends.
+__device__ __forceinline__ void wait_for_copies(uint32_t full0, uint32_t stages, uint32_t stage, uint32_t phase) {
+  for (uint32_t s = 0; s < stages; ++s) (void)wait_barrier(full0 + 8u * s, s < stage ? phase : phase ^ 1u);
 }
 
 // a * b + c of two numbers side by side.

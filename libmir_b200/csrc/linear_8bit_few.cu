@@ -44,6 +44,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long barriers[BARRIERS];
   __shared__ uint32_t tmem_slot;
+  __shared__ bool go_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // without a cluster the CTAs walk over the tiles of 128 weight rows
   const int first_tile = blockIdx.x / splits, tile_step = gridDim.x / splits, rank = blockIdx.x % splits;
@@ -60,6 +61,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
   const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
   auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
   if (threadIdx.x == 0) {
+    go_slot = *reinterpret_cast<volatile int*>(&g_error) == 0;             // an earlier wait ran out: nothing is begun
     for (int i = 0; i < BARRIERS; ++i)
       barrier_init(bar(i), i >= SUM_FREE && i < SUM_FREE + 4 ? 4u : (i >= X_READY ? (uint32_t)kWorkers : 1u));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -74,7 +76,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
   const uint32_t tmem = tmem_slot;
   grid_dependency_wait();
   grid_launch_dependents();
-  const bool go = *reinterpret_cast<volatile int*>(&g_error) == 0;
+  const bool go = go_slot;
 
   if (warp == kLoader) {
     if (lane == 0 && go) {
@@ -89,6 +91,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
         if (!OWN) tma_load_2d(to + kRows * kBlock, &x_map, full, (first + b) * kBlock, 0);
         if (++stage == (uint32_t)stages) { stage = 0; parity ^= 1u; }
       }
+      wait_for_copies(bar(FULL), (uint32_t)stages, stage, parity);
     }
   } else if (warp == kIssuer) {
     if (go) {
@@ -309,11 +312,10 @@ int launch(const uint8_t* codes, const float* scales, int scale_stride, const vo
   }
   // the most CTAs that are all there at once, two blocks each at least; with more tiles than that they walk over the tiles
   Cut cut = cut_for(m, N, OWN, blocks, 1);
-  for (int splits = 8; splits >= 1; splits /= 2) {
-    if (forced > 0 && splits != forced) continue;
+  for (int splits = forced > 0 ? forced : 8; splits >= 1; splits /= 2) {
+    while ((blocks + splits - 1) / splits > kMostBlocks) splits *= 2;          // (no more than 8: mir_linear_8bit_few_takes)
     cut = cut_for(m, N, OWN, blocks, splits);
-    if (cut.per_split > kMostBlocks) { cut = cut_for(m, N, OWN, blocks, std::min(8, splits * 2)); break; }
-    if (splits == 1 || forced > 0 || ((long long)tiles * splits <= (long long)cut.ctas * mir_sm_count() && blocks >= 2 * splits)) break;
+    if (splits == 1 || forced > 0 || (blocks + splits / 2 - 1) / (splits / 2) > kMostBlocks || ((long long)tiles * splits <= (long long)cut.ctas * mir_sm_count() && blocks >= 2 * splits)) break;
   }
   status = reserve_shared(linear_8bit_few_kernel<N, OWN>, cut.bytes, "linear_8bit");
   if (status != MIR_OK) return status;

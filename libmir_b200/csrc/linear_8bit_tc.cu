@@ -56,21 +56,19 @@ template <bool OUT_FLOAT>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
                          const __grid_constant__ CUtensorMap out_map, bool boxes, const float* __restrict__ x_scales, const float* __restrict__ w_scales, const void* __restrict__ bias,
-                         void* __restrict__ out, long long out_stride, int m, int n, int k, int scale_stride, int row_tiles, int tiles, bool accumulate) {
+                         void* __restrict__ out, long long out_stride, int m, int n, int k, int scale_stride, int row_tiles, int all_tiles, bool accumulate) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long barriers[BARRIERS];
   __shared__ __align__(16) float scales_here[kScaleSlots * kRows];
   __shared__ uint32_t tmem_slot;
-  if (*reinterpret_cast<volatile int*>(&g_error) != 0) {       // an earlier wait ran out: do not queue up more
-    grid_dependency_wait();
-    return;
-  }
+  __shared__ int tiles_slot;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
   auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int blocks = (k + kBlock - 1) / kBlock;
   if (threadIdx.x == 0) {
+    tiles_slot = *reinterpret_cast<volatile int*>(&g_error) != 0 ? 0 : all_tiles;       // an earlier wait ran out: nothing is begun
     for (int i = 0; i < BARRIERS; ++i) barrier_init(bar(i), i >= SUM_FREE ? (uint32_t)kAddingWarps : 1u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -83,6 +81,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
   __syncthreads();
   tensor_fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  const int tiles = tiles_slot;
   grid_dependency_wait();
   grid_launch_dependents();
 
@@ -91,7 +90,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
   if (warp == 0) {
     // ------------------------------------------------------------------ loader
     if (lane == 0) {
-      uint32_t stage = 0, parity = 0, slot = 0;
+      uint32_t stage = 0, parity = 0, slot = 0, slot_parity = 0;
       bool alive = true;
       for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
         const int row0 = tile % row_tiles * kRows, column0 = tile / row_tiles * kColumns;
@@ -106,10 +105,12 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
                            smem_u32(scales_here + slot * kRows)), "l"(x_scales + (size_t)b * scale_stride + row0),
                        "r"((uint32_t)(kRows * sizeof(float))), "r"(bar(SCALE_FULL + (int)slot))
                        : "memory");
-          if (++slot == (uint32_t)kScaleSlots) slot = 0;
+          if (++slot == (uint32_t)kScaleSlots) { slot = 0; slot_parity ^= 1u; }
           if (++stage == (uint32_t)kStages) { stage = 0; parity ^= 1u; }
         }
       }
+      wait_for_copies(bar(FULL), kStages, stage, parity);
+      wait_for_copies(bar(SCALE_FULL), kScaleSlots, slot, slot_parity);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ issuer (tcgen05.cuh: from a whole warp)

@@ -18,6 +18,7 @@ from . import _check, _ptr, _raw_device, _stream, library
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 128                 # rows and columns of a weight that share a scale, and columns of a row of activations
+MOST_KEYS = (1 << 31) - 256      # of a context, as 32-bit positions have it
 
 
 # (The checks run at every call: conditions are tested in place and messages put together only where one fails.)
@@ -147,7 +148,7 @@ def prefill_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.
     if not (query_starts.dtype is torch.int32 and context_lens.dtype is torch.int32 and query_starts.numel() == rows + 1
             and query_starts.is_contiguous() and context_lens.is_contiguous()):
         raise KernelError(f"{what}: query_starts is int32 [requests + 1], context_lens int32 [requests]")
-    longest = block_table.shape[1] * page_size
+    longest = min(block_table.shape[1] * page_size, MOST_KEYS)
     if max_context is not None:
         longest = min(longest, max_context)
     lib = library("eight_bit")

@@ -720,3 +720,100 @@ def test_refusals_of_tensors_that_do_not_fit():
     linear(x=x[:0], out=result[:0])
     with pytest.raises(KernelError):
         kernels.quantize_weight_8bit(torch.zeros(4, 4, dtype=torch.float16, device="cuda"))
+
+
+# ------------------------------------------------------------------------------------------------ numbers that are none
+def close_with_nans(got, want, bound, what=""):
+    """NaN exactly where the plain result is, and close elsewhere."""
+    assert torch.equal(got.cpu().isnan(), want.isnan()), what
+    close(got.cpu().double().nan_to_num(0.0), want.nan_to_num(0.0), bound.nan_to_num(1e-30), what)
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, page", [(4, 2, 128, 16), (6, 2, 64, 16), (2, 2, 128, 12)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_prefill_attention_shows_nan_only_to_the_queries_that_see_it(heads, kv_heads, dim, page, window):
+    """NaN among the values and keys of the portions' own tokens, of the context before them and at the windows' edges; infinite and
+    NaN queries."""
+    new, lengths = [90, 40, 1, 150], [90, 170, 60, 150]
+    batch = Batch(91, lengths, heads, kv_heads, dim, page)
+    slot = lambda r, p: (int(batch.table[r, p // page]), p % page)
+    for r, p, head, column in ((0, 30, 0, 5), (0, 89, 1, dim - 1), (0, 0, 1, 7), (1, 120, 0, 33), (1, 169, 1, 2), (1, 95, 1, 60),
+                               (2, 59, 0, 1), (3, 128, 1, 9), (3, 127, 1, 8), (3, 3, 0, 4)):
+        at, place = slot(r, p)
+        batch.v.codes[at, place, head, column] = math.nan
+    at, place = slot(0, 60)
+    batch.k.codes[at, place, 0, 3] = math.nan                          # that head's queries from there on see it
+    batch.qkv[10, 5], batch.qkv[20, dim + 3], batch.qkv[95, 1], batch.qkv[131, 0] = math.inf, math.nan, -math.inf, math.nan
+    out = run_prefill(batch, batch.on_gpu(), new, dim ** -0.5, window)
+    want, size = batch.prefill(new, dim ** -0.5, window)
+    assert want.isnan().any() and not want.isnan().all()
+    close_with_nans(out, want, attention_bound(want, size))
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, page", [(4, 2, 128, 16), (6, 2, 64, 16), (20, 1, 128, 32)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_decode_attention_shows_nan_only_to_the_rows_that_see_it(heads, kv_heads, dim, page, window):
+    lengths = [300, 200, 500, 77, 1]
+    batch = Batch(92, lengths, heads, kv_heads, dim, page)
+    slot = lambda r, p: (int(batch.table[r, p // page]), p % page)
+    for r, p, head, column in ((0, 299, 0, 5), (0, 258, 0, 6), (0, 261, kv_heads - 1, 7), (0, 260, 0, 8), (2, 100, 0, 1)):
+        at, place = slot(r, p)
+        batch.v.codes[at, place, head, column] = math.nan
+    at, place = slot(3, 76)
+    batch.k.codes[at, place, 0, 3] = math.nan
+    batch.qkv[1, 5], batch.qkv[4, dim + 3] = math.inf, math.nan
+    positions = [n - 1 for n in lengths]
+    out = run_decode(batch, batch.on_gpu(), positions, dim ** -0.5, window)
+    want, size = batch.decode(positions, dim ** -0.5, window)
+    assert want.isnan().any() and not want.isnan().all()
+    close_with_nans(out, want, attention_bound(want, size))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_zero_queries_over_zero_keys(dim):
+    """The least scales on both sides (their product is no 32-bit number): every visible key weighs the same."""
+    batch = Batch(93, [70, 200], 4, 2, dim, 16)
+    batch.k.codes[:], batch.k.scales[:] = 0.0, 2.0 ** -118
+    batch.qkv[:, :4 * dim] = 0.0
+    cache = batch.on_gpu()
+    for scale in (0.1, 1e-12):
+        close(run_decode(batch, cache, [69, 150], scale), *with_bound(batch.decode([69, 150], scale)))
+        close(run_prefill(batch, cache, [30, 140], scale), *with_bound(batch.prefill([30, 140], scale)))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prefill_attention_ends_with_its_rows(dim):
+    """Query starts beyond the rows there are: what has a row is worked out, nothing else is written."""
+    from libmir_b200 import kernels
+    batch = Batch(94, [60, 50], 4, 2, dim, 16)
+    cache = batch.on_gpu()
+    out = torch.full((60, 4 * dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    starts, contexts = torch.tensor([0, 20, 75], dtype=torch.int32).cuda(), torch.tensor([60, 50], dtype=torch.int32).cuda()
+    kernels.prefill_attention_8bit(batch.qkv[:40].cuda(), out[:40], *cache, batch.table.cuda(), starts, contexts, 16, 4, 2, dim, 0.1, None)
+    want, bound = with_bound(batch.prefill([20, 20], 0.1))
+    close(out[:40], want, bound)
+    assert (out[40:] == 7.0).all()
+
+
+def test_linear_of_a_long_row_with_few_parts():
+    """A forced cut that would leave a CTA more blocks than it holds is made finer."""
+    from libmir_b200 import kernels
+    from libmir_b200.kernels.eight_bit import set_linear_8bit_splits
+    g = seeded(95)
+    for m in (3, 20):
+        k, n = 128 * 170, 200
+        x = torch.randn(m, k, generator=g).bfloat16()
+        codes = (torch.randn(n, k, generator=g) * 100).clamp(-448, 448).to(E4M3)
+        scales = torch.rand(2, k // 128, generator=g) * 1e-3
+        weight = plain.weight_values(codes, scales)
+        want = plain.rounded_rows(x) @ weight.t()
+        bound = product_bound(x, weight, torch.float32, torch.zeros(1, dtype=torch.float64))(want)
+        for splits in (1, 2, 4, 8, 0):
+            set_linear_8bit_splits(splits)
+            try:
+                out = torch.zeros(m, n, device="cuda")
+                kernels.linear_8bit(x.cuda(), codes.cuda(), scales.cuda(), out)
+            finally:
+                set_linear_8bit_splits(0)
+            close(out, want, bound, f"{m} rows, {splits}")
+    assert kernels.eight_bit_error() == 0
