@@ -817,3 +817,20 @@ def test_linear_of_a_long_row_with_few_parts():
                 set_linear_8bit_splits(0)
             close(out, want, bound, f"{m} rows, {splits}")
     assert kernels.eight_bit_error() == 0
+
+
+@pytest.mark.parametrize("dim, page, kv_heads, new, before", [
+    (128, 256, 3, [400, 1], [100, 200]), (64, 24, 3, [2, 290, 1], [23, 7, 40]), (128, 16, 5, [1] * 700, [3, 15, 16, 31] * 175),
+    (64, 130, 2, [1030, 5], [129, 3]), (128, 64, 2, [1] * 300, list(range(300)))])
+def test_store_of_long_pages_and_many_tokens(dim, page, kv_heads, new, before):
+    """Pages of more rows than a warp or a block holds, found and shared in each of the ways; later tokens louder than the page."""
+    lengths = [n + b for n, b in zip(new, before)]
+    batch = Batch(97, lengths, 4, kv_heads, dim, page)
+    cache = batch.on_gpu()
+    slots = [int(batch.table[r, p // page]) * page + p % page for r, (n, b) in enumerate(zip(new, before)) for p in range(b, b + n)]
+    for loud in (0, 4):
+        qkv = (torch.randn(len(slots), (4 + 2 * kv_heads) * dim, generator=batch.g)
+               * torch.exp2(torch.randint(-6, 7, (len(slots), 1), generator=batch.g).float() + loud)).bfloat16()
+        plain_store(batch, qkv, slots)
+        run_store(qkv, slots, cache, batch)
+        same_cache(batch, cache)
