@@ -156,31 +156,47 @@ __device__ __forceinline__ float softmax_tile(uint32_t scores, int first, int lo
   uint32_t raw[2][32];
   tmem_load_32_ahead(scores + (uint32_t)first, raw[0]);
   tmem_load_32_ahead(scores + (uint32_t)first + 32u, raw[1]);
+  // Eight columns are of one page (a page has eight keys or more): their scores share a factor, which is positive, so that the maximum is
+  // taken first and the multiplication is part of the exponent's.  (Where two least scales meet the factor would be 0, and a hidden
+  // key's -inf times that no number.)
+  float factors[kCols / 8];
+  uint32_t seen[kCols / 32];
+  if (MASKED) {
+#pragma unroll
+    for (int i = 0; i < kCols / 32; ++i) {
+      const int from = min(max(low - first - 32 * i, 0), 32), to = min(max(high - first - 32 * i + 1, 0), 32);
+      seen[i] = __funnelshift_lc(0xffffffffu, 0u, to) & ~__funnelshift_lc(0xffffffffu, 0u, from);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kCols / 8; ++i) {
+    const int slot = (first + 8 * i) >> shift;
+    factors[i] = info.k_scale[slot] * scale;
+    if (MASKED) {
+      factors[i] = fmaxf(factors[i], 1e-37f);
+      if (info.row[slot] < 0) seen[i / 4] &= ~(0xffu << (8 * (i & 3)));
+    }
+  }
   tmem_load_done(raw[0]);
   tmem_load_done(raw[1]);
-  // Eight columns are of one page (a page has eight keys or more): their scores share a factor, which is positive, so that the maximum is
-  // taken first and the multiplication is part of the exponent's.
   float v[kCols];
   float maximum = -INFINITY;
 #pragma unroll
   for (int c8 = 0; c8 < kCols; c8 += 8) {
-    const int slot = (first + c8) >> shift;
     float best[2] = {-INFINITY, -INFINITY};
-    const bool there = !MASKED || info.row[slot] >= 0;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       const int c = c8 + i;
       v[c] = __uint_as_float(raw[c / 32][c % 32]);
       v[c + 1] = __uint_as_float(raw[c / 32][c % 32 + 1]);
       if (MASKED) {
-        v[c] = there && c >= low - first && c <= high - first ? v[c] : -INFINITY;
-        v[c + 1] = there && c + 1 >= low - first && c + 1 <= high - first ? v[c + 1] : -INFINITY;
+        v[c] = (seen[c / 32] & (1u << (c % 32))) != 0u ? v[c] : -INFINITY;
+        v[c + 1] = (seen[c / 32] & (2u << (c % 32))) != 0u ? v[c + 1] : -INFINITY;
       }
       best[i >> 1 & 1] = max_of_three(best[i >> 1 & 1], v[c], v[c + 1]);
     }
-    maximum = fmaxf(maximum, fmaxf(best[0], best[1]) * info.k_scale[slot]);
+    maximum = fmaxf(maximum, fmaxf(best[0], best[1]) * factors[c8 / 8]);
   }
-  maximum *= scale;
   shared_max[part * kRows] = maximum;
   asm volatile("bar.sync %0, %1;" ::"r"(team), "n"(32 * kParts) : "memory");
 #pragma unroll
@@ -198,24 +214,18 @@ __device__ __forceinline__ float softmax_tile(uint32_t scores, int first, int lo
   own_factor = reference == now ? 1.0f : approximate_exp2(reference - now);
   reference = now;
   const float down = (MASKED && reference == -INFINITY) ? 0.0f : -reference;       // (a row that has seen nothing yet)
-  float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float2 downs = make_float2(down, down);
+  float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-  for (int c8 = 0; c8 < kCols; c8 += 8) {
-    const float k_scale = info.k_scale[(first + c8) >> shift] * scale;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const int c = c8 + i;
-      float p0 = approximate_exp2(fmaf(v[c], k_scale, down)), p1 = approximate_exp2(fmaf(v[c + 1], k_scale, down));
-      if (MASKED) {                                                        // (the scales' product may be 0: no -inf times that)
-        p0 = v[c] == -INFINITY ? 0.0f : p0;
-        p1 = v[c + 1] == -INFINITY ? 0.0f : p1;
-      }
-      sums[(c >> 1) & 3] += p0 + p1;
-      const __nv_bfloat162 both = __floats2bfloat162_rn(p0, p1);
-      packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&both);
-    }
+  for (int c = 0; c < kCols; c += 2) {
+    const float2 both = make_float2(factors[c / 8], factors[c / 8]);
+    float2 weight = fma_two(make_float2(v[c], v[c + 1]), both, downs);
+    weight = make_float2(approximate_exp2(weight.x), approximate_exp2(weight.y));
+    sums[(c >> 1) & 1] = add_two(sums[(c >> 1) & 1], weight);
+    const __nv_bfloat162 rounded = __floats2bfloat162_rn(weight.x, weight.y);
+    packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&rounded);
   }
-  return (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  return (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -473,32 +483,37 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (alive && !wait_barrier(bar(V_FREE + (int)values.stage), values.phase ^ 1u)) { g_error = 4; alive = false; }
         const unsigned char* from = smem + kOffRaw + raw.stage * kTile8;
         unsigned char* to = smem + kOffV + values.stage * kTile16;
-        // thread: 16 bytes (j) of every 32nd row (whose place in the swizzle is the same), two at a time
-        const int j = thread & 7, r0 = thread >> 3;
+        // thread: two pieces of 8 bytes, j and j + 8, of every 32nd row (whose place in the swizzle is the same), two rows at a time; a piece
+        // becomes 16 bytes, so that eight threads write a whole row of 128 bytes, and of two rows that are read together one begins with the
+        // first eight pieces and the other with the last, so that no two threads meet in a bank
+        const int j = thread & 7, r0 = thread >> 3, swap = r0 & 1;
         const bool all_seen = infos[info].whole && w.begin + t * kKeys >= w.first_key && w.begin + (t + 1) * kKeys <= w.end;
         const bool one_factor = infos[info].one_factor, hides = !seen_by_all(w, t);
-        from += r0 * 128 + ((j ^ (r0 & 7)) << 4);
-        unsigned char* low = to + (j >> 2) * kHalf + r0 * 128 + ((((j & 3) * 2) ^ (r0 & 7)) << 4);
-        unsigned char* high = to + (j >> 2) * kHalf + r0 * 128 + ((((j & 3) * 2 + 1) ^ (r0 & 7)) << 4);
+        from += r0 * 128;
+        const unsigned char* piece[2] = {from + ((((j >> 1) + 4 * swap) ^ (r0 & 7)) << 4) + (j & 1) * 8,
+                                         from + ((((j >> 1) + 4 - 4 * swap) ^ (r0 & 7)) << 4) + (j & 1) * 8};
+        to += r0 * 128 + ((j ^ (r0 & 7)) << 4);
+        unsigned char* wide_piece[2] = {to + swap * kHalf, to + (1 - swap) * kHalf};
         constexpr int kStep = kConverters / 8, kTogether = 2;
 #pragma unroll 1
         for (int base = 0; base < kKeys; base += kStep * kTogether) {
-          uint4 word[kTogether];
+          uint2 word[kTogether][2];
           uint32_t factor[kTogether];
 #pragma unroll
           for (int i = 0; i < kTogether; ++i) {
-            word[i] = *reinterpret_cast<const uint4*>(from + (base + i * kStep) * 128);
             factor[i] = infos[info].v_factor[(base + i * kStep + r0) >> shift];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) word[i][h] = *reinterpret_cast<const uint2*>(piece[h] + (base + i * kStep) * 128);
           }
 #pragma unroll
           for (int i = 0; i < kTogether; ++i) {
             const int r = base + i * kStep + r0;
             if (!all_seen) {
               const int key = w.begin + t * kKeys + r;
-              if (key >= w.end || key < w.first_key || infos[info].row[r >> shift] < 0) word[i] = make_uint4(0u, 0u, 0u, 0u);
+              if (key >= w.end || key < w.first_key || infos[info].row[r >> shift] < 0) word[i][0] = word[i][1] = make_uint2(0u, 0u);
             }
             uint32_t wide[8];
-            const uint32_t words[4] = {word[i].x, word[i].y, word[i].z, word[i].w};
+            const uint32_t words[4] = {word[i][0].x, word[i][0].y, word[i][1].x, word[i][1].y};
             uint32_t last = 0u;                              // a byte's upper bit: its magnitude is e4m3's last code, NaN
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -518,8 +533,10 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 if ((pair & 0x7f00u) == 0x7f00u) wide[c] = hides ? wide[c] & 0xffffu : wide[c] | 0x7fff0000u;
               }
             }
-            *reinterpret_cast<uint4*>(low + (base + i * kStep) * 128) = make_uint4(wide[0], wide[1], wide[2], wide[3]);
-            *reinterpret_cast<uint4*>(high + (base + i * kStep) * 128) = make_uint4(wide[4], wide[5], wide[6], wide[7]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              *reinterpret_cast<uint4*>(wide_piece[h] + (base + i * kStep) * 128) =
+                  make_uint4(wide[4 * h], wide[4 * h + 1], wide[4 * h + 2], wide[4 * h + 3]);
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -114,6 +114,17 @@ __device__ __forceinline__ float2 fma_two(float2 a, float2 b, float2 c) {
   return r;
 }
 
+// a + b of two numbers side by side.
+__device__ __forceinline__ float2 add_two(float2 a, float2 b) {
+  unsigned long long x, y, d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
+
 // 32 consecutive accumulator columns of this thread's lane, without waiting for them (tmem_load_done).
 __device__ __forceinline__ void tmem_load_32_ahead(uint32_t address, uint32_t (&r)[32]) {
   asm volatile(
