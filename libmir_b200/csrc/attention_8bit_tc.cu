@@ -67,7 +67,19 @@ struct Info {
   int row[kSlots];
   float k_scale[kSlots];
   uint32_t v_factor[kSlots], v_rest[kSlots];               // what a lifted value is multiplied by: 2^120 times its scale, as one or two bf16 pairs
-  int whole, one_factor;                                                // all pages are there
+  int whole, one_factor;                                   // all pages are there; v_rest is 1 throughout
+};
+
+// n / d for 0 <= n < 2^31 as (n + n m / 2^32) >> s: s the bits of d - 1, m = floor(2^32 (2^s - d) / d) + 1 (a division takes some 25
+// instructions, and every role works out its items by itself).
+struct Divider {
+  uint32_t factor;
+  int bits, by;
+  explicit Divider(int d) : bits(0), by(d) {
+    while ((1ll << bits) < d) ++bits;
+    factor = (uint32_t)((((1ull << bits) - (unsigned long long)d) << 32) / (unsigned long long)d + 1ull);
+  }
+  __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((uint32_t)n, factor) + (uint32_t)n) >> bits); }
 };
 
 struct Work {
@@ -77,30 +89,31 @@ struct Work {
 struct Items {
   const int* query_starts;
   const int* context_lens;
-  int num_rows, tokens, kv_heads, group, window, partition, num_partitions, row_tiles, count;
+  int num_rows, tokens, window, partition, row_tiles, count;
+  const Divider &kv_heads, &num_partitions, &group;
   // Item `index`: the kv head is the fast index, then the partition, then the batch's tiles of rows from the last one of the last request
   // backwards (late tiles see the most keys and come first).  False beyond the last item.
   __device__ __forceinline__ bool at(int index, Work& w) const {
     if (index < 0 || index >= count) return false;
-    w.kv_head = index % kv_heads;
-    const int rest = index / kv_heads;
-    w.part = rest % num_partitions;
-    int remaining = row_tiles - 1 - rest / num_partitions;
+    const int rest = kv_heads(index), from_last = num_partitions(rest);
+    w.kv_head = index - rest * kv_heads.by;
+    w.part = rest - from_last * num_partitions.by;
+    int remaining = row_tiles - 1 - from_last;
     w.request = -1;
     Portion portion{0, 0};
     for (int r = 0; r < num_rows; ++r) {
       portion = portion_of(query_starts, r, tokens);
-      const int tiles = (portion.count * group + kRows - 1) / kRows;
+      const int tiles = (portion.count * group.by + kRows - 1) / kRows;
       if (remaining < tiles) { w.request = r; break; }
       remaining -= tiles;
     }
     if (w.request < 0) return false;
     w.first_row = remaining * kRows;
-    w.rows = min(kRows, portion.count * group - w.first_row);
+    w.rows = min(kRows, portion.count * group.by - w.first_row);
     w.first_token = portion.first;
     const int start = context_lens[w.request] - portion.count;
-    w.first_position = start + w.first_row / group;
-    w.last_position = start + (w.first_row + w.rows - 1) / group;
+    w.first_position = start + group(w.first_row);
+    w.last_position = start + group(w.first_row + w.rows - 1);
     w.first_key = (window > 0 && w.first_position >= window) ? w.first_position + 1 - window : 0;
     w.begin = max(w.first_key / kKeys * kKeys, w.part * partition);
     w.end = (int)min((long long)w.last_position + 1, (long long)(w.part + 1) * partition);
@@ -232,8 +245,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                     const __grid_constant__ CUtensorMap k_tile_map, const __grid_constant__ CUtensorMap v_tile_map, const bf16* __restrict__ q,
                     long long q_stride, Cache8 cache, const int* __restrict__ block_table, int table_width,
-                    const int* __restrict__ query_starts, const int* __restrict__ context_lens, int num_rows, int tokens, int heads, float scale_log2,
-                    int window, int partition, int num_partitions, float* __restrict__ partial_o, float* __restrict__ partial_ml,
+                    const int* __restrict__ query_starts, const int* __restrict__ context_lens, int num_rows, int tokens,
+                    const __grid_constant__ Divider kv_heads, const __grid_constant__ Divider group, const __grid_constant__ Divider parts,
+                    float scale_log2, int window, int partition, float* __restrict__ partial_o, float* __restrict__ partial_ml,
                     bf16* __restrict__ out, const float* __restrict__ sinks) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long barriers[BARRIERS];
@@ -250,7 +264,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
   auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
-  const int group = heads / cache.kv_heads;
+  const int heads = group.by * kv_heads.by, num_partitions = parts.by;
   if (threadIdx.x == 0) {
     for (int i = 0; i < BARRIERS; ++i) {
       uint32_t count = 1u;
@@ -269,7 +283,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   grid_dependency_wait();
   if (threadIdx.x == 0) {
     int total = 0;
-    for (int r = 0; r < num_rows; ++r) total += (portion_of(query_starts, r, tokens).count * group + kRows - 1) / kRows;
+    for (int r = 0; r < num_rows; ++r) total += (portion_of(query_starts, r, tokens).count * group.by + kRows - 1) / kRows;
     if (*reinterpret_cast<volatile int*>(&g_error) != 0) total = 0;       // an earlier wait ran out: nothing is begun
     row_tiles_slot = total;
     for (int i = 0; i < 4; ++i) hidden_nans[i] = 0;
@@ -280,8 +294,8 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   grid_launch_dependents();
   const uint32_t tmem = tmem_slot, tmem_o = tmem + 384u;
   const int shift = 31 - __clz(cache.page_size);            // pages are powers of two
-  const Items items{query_starts, context_lens, num_rows, tokens, cache.kv_heads, group, window, partition, num_partitions, row_tiles_slot,
-                    row_tiles_slot * cache.kv_heads * num_partitions};
+  const Items items{query_starts, context_lens, num_rows, tokens, window, partition, row_tiles_slot,
+                    row_tiles_slot * kv_heads.by * num_partitions, kv_heads, parts, group};
   const int cta = blockIdx.x, ctas = gridDim.x;
   // whether all queries of an item see all keys of its tile t (that are there)
   auto seen_by_all = [&](const Work& of, int t) {
@@ -441,8 +455,8 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       constexpr int kHeld = 8, kWarpRows = kRows / (kConverters / 32);
       long long offset;
       {
-        const int row = w.first_row + min(my_warp * kWarpRows + (lane & (kWarpRows - 1)), w.rows - 1), token = row / group;
-        offset = (long long)(w.first_token + token) * q_stride + (long long)(w.kv_head * group + row - token * group) * kDim;
+        const int row = w.first_row + min(my_warp * kWarpRows + (lane & (kWarpRows - 1)), w.rows - 1), token = group(row);
+        offset = (long long)(w.first_token + token) * q_stride + (long long)(w.kv_head * group.by + row - token * group.by) * kDim;
       }
 #pragma unroll 1
       for (int half = 0; half < kWarpRows; half += kHeld) {
@@ -478,7 +492,6 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       ++n;
       for (int t = 0; t < w.tiles; ++t, ++g) {
         const int info = g % kInfos;
-        if (alive && !wait_barrier(bar(INFO_FULL + info), (uint32_t)(g / kInfos & 1))) { g_error = 4; alive = false; }
         if (alive && !wait_barrier(bar(RAW_FULL + (int)raw.stage), raw.phase)) { g_error = 4; alive = false; }
         if (alive && !wait_barrier(bar(V_FREE + (int)values.stage), values.phase ^ 1u)) { g_error = 4; alive = false; }
         const unsigned char* from = smem + kOffRaw + raw.stage * kTile8;
@@ -559,7 +572,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     int g0 = 0, n = 0;
     for (int k = 0; more(k); ++k) {
       if (!items.at(item_of(k, cta, ctas), w)) continue;
-      const int row = w.first_row + min(r, w.rows - 1), token = row / group, head = w.kv_head * group + row - token * group;
+      const int row = w.first_row + min(r, w.rows - 1), token = group(row), head = w.kv_head * group.by + row - token * group.by;
       const size_t out_row = (size_t)(w.first_token + token) * heads + head;
       if (w.tiles == 0) {                                    // a partition without keys, or rows that see none
         if (stream == 0 && part == 0 && r < w.rows) {
@@ -573,7 +586,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
         continue;
       }
-      const int position = w.first_position + (w.first_row % group + min(r, w.rows - 1)) / group;
+      const int position = w.first_position + token - group(w.first_row);
       float reference = -INFINITY, denominator = 0.0f, scale = 0.0f;
       if (stream < w.tiles) {
         if (alive && !wait_barrier(bar(Q_FULL + (n & 3)), (uint32_t)(n >> 2 & 1))) { g_error = 3; alive = false; }
@@ -646,25 +659,6 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       tmem_load_32(tmem_o + lane_bits + (uint32_t)column, o);
       tensor_fence_before_sync();
       barrier_arrive(bar(O_FREE));                           // (the next item's products may overwrite it)
-      if (hidden_nans[n & 3] == n + 1) {
-        const int* table = block_table + (size_t)w.request * table_width;
-        const int last = min(position, w.end - 1);
-#pragma unroll 1
-        for (int key = max(w.begin, window > 0 ? position - window + 1 : 0); key <= last; ++key) {
-          if (seen_by_all(w, (key - w.begin) / kKeys)) continue;                                // (left in)
-          const int page = page_of_block(table, table_width, key >> shift, cache.pages);
-          if (page < 0) continue;
-          const uint32_t* codes = reinterpret_cast<const uint32_t*>(
-              cache.v + ((((size_t)page << shift) + (key & (cache.page_size - 1))) * cache.kv_heads + w.kv_head) * kDim + column);
-#pragma unroll
-          for (int i = 0; i < kOut; i += 4) {
-            const uint32_t nans = nan_bytes(codes[i / 4]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (nans >> (8 * j + 7) & 1u) o[i + j] = __int_as_float(0x7fffffff);
-          }
-        }
-      }
       if (r < w.rows && alive) {
         if (num_partitions == 1) {
           if (total != 0.0f && sinks != nullptr) total += exp2f(sinks[head] * kLog2e - top);
@@ -686,6 +680,22 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             float4* to = reinterpret_cast<float4*>(partial_o + at * kDim + column);
 #pragma unroll
             for (int i = 0; i < kOut; i += 4) to[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+      }
+      if (hidden_nans[n & 3] == n + 1 && r < w.rows && total != 0.0f) {
+        // the NaN values that were left out, for the rows that see their keys
+        const int* table = block_table + (size_t)w.request * table_width;
+#pragma unroll 1
+        for (int key = max(w.begin, window > 0 ? position - window + 1 : 0); key <= min(position, w.end - 1); ++key) {
+          if (seen_by_all(w, (key - w.begin) / kKeys)) continue;                                // (left in)
+          const int page = page_of_block(table, table_width, key >> shift, cache.pages);
+          const uint8_t* codes = cache.v + ((((size_t)max(page, 0) << shift) + (key & (cache.page_size - 1))) * cache.kv_heads + w.kv_head) * kDim;
+#pragma unroll 1
+          for (int i = column; page >= 0 && i < column + kOut; ++i) {
+            if ((codes[i] & 0x7f) != 0x7f) continue;
+            if (num_partitions == 1) out[out_row * kDim + i] = __float2bfloat16_rn(__int_as_float(0x7fffffff));
+            else partial_o[(out_row * num_partitions + w.part) * kDim + i] = __int_as_float(0x7fffffff);
           }
         }
       }
@@ -730,8 +740,8 @@ int mir_attention_8bit_prefill(const Attention8& a, int tokens) {
   if (status != MIR_OK) return status;
   status = mir_launch("prefill_attention_8bit", prefill_8bit_kernel, dim3((unsigned)std::min<long long>(items, mir_sm_count())), dim3(kThreads),
                       (size_t)kSmemBytes, a.stream, 0, maps[0], maps[1], maps[2], maps[3], (const bf16*)a.q, a.q_stride, a.cache, a.block_table,
-                      a.table_width, a.query_starts, a.context_lens, a.num_rows, tokens, a.heads, a.scale * kLog2e, a.window, a.partition,
-                      a.num_partitions, a.partial_o(tokens), a.partial_ml(tokens), (bf16*)a.out, a.sinks);
+                      a.table_width, a.query_starts, a.context_lens, a.num_rows, tokens, Divider(a.cache.kv_heads), Divider(group),
+                      Divider(a.num_partitions), a.scale * kLog2e, a.window, a.partition, a.partial_o(tokens), a.partial_ml(tokens), (bf16*)a.out, a.sinks);
   if (status != MIR_OK || a.num_partitions == 1) return status;
   return mir_merge_8bit(a, tokens);
 }
