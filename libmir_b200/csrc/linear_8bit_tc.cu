@@ -35,8 +35,7 @@ static_assert(kSmemBytes + kLeastSharedBeside > kSharedOfSm, "no other kernel wi
 // scales) of block b.
 constexpr int kScaleSlots = kStages + 2;
 
-enum { FULL = 0, EMPTY = FULL + kStages, SUM_FULL = EMPTY + kStages, SCALE_FULL = SUM_FULL + 2, SUM_FREE = SCALE_FULL + kScaleSlots,
-       BARRIERS = SUM_FREE + 2 };
+enum { FULL = 0, EMPTY = FULL + kStages, SUM_FULL = EMPTY + kStages, SUM_FREE = SUM_FULL + 2, BARRIERS = SUM_FREE + 2 };
 
 __device__ int g_error = 0;
 
@@ -69,7 +68,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
   const int blocks = (k + kBlock - 1) / kBlock;
   if (threadIdx.x == 0) {
     tiles_slot = *reinterpret_cast<volatile int*>(&g_error) != 0 ? 0 : all_tiles;       // an earlier wait ran out: nothing is begun
-    for (int i = 0; i < BARRIERS; ++i) barrier_init(bar(i), i >= SUM_FREE ? (uint32_t)kAddingWarps : 1u);
+    for (int i = 0; i < BARRIERS; ++i) barrier_init(bar(i), i >= SUM_FREE ? (uint32_t)kAddingWarps : (i >= SUM_FULL ? 2u : 1u));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -90,27 +89,25 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
   if (warp == 0) {
     // ------------------------------------------------------------------ loader
     if (lane == 0) {
-      uint32_t stage = 0, parity = 0, slot = 0, slot_parity = 0;
+      uint32_t stage = 0, parity = 0, slot = 0;
       bool alive = true;
       for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
         const int row0 = tile % row_tiles * kRows, column0 = tile / row_tiles * kColumns;
         for (int b = 0; b < blocks; ++b) {
           if (!wait_barrier(bar(EMPTY + stage), parity ^ 1u)) { g_error = 1; alive = false; break; }
           const uint32_t full = bar(FULL + stage), to = smem_base + stage * (uint32_t)kStageBytes;
-          barrier_expect_bytes(full, (uint32_t)kStageBytes);
+          barrier_expect_bytes(full, (uint32_t)(kStageBytes + kRows * sizeof(float)));
           tma_load_2d(to, &x_map, full, b * kBlock, row0);
           tma_load_2d(to + kRows * kBlock, &w_map, full, b * kBlock, column0);
-          barrier_expect_bytes(bar(SCALE_FULL + (int)slot), (uint32_t)(kRows * sizeof(float)));
           asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                            smem_u32(scales_here + slot * kRows)), "l"(x_scales + (size_t)b * scale_stride + row0),
-                       "r"((uint32_t)(kRows * sizeof(float))), "r"(bar(SCALE_FULL + (int)slot))
+                       "r"((uint32_t)(kRows * sizeof(float))), "r"(full)
                        : "memory");
-          if (++slot == (uint32_t)kScaleSlots) { slot = 0; slot_parity ^= 1u; }
+          if (++slot == (uint32_t)kScaleSlots) slot = 0;
           if (++stage == (uint32_t)kStages) { stage = 0; parity ^= 1u; }
         }
       }
       wait_for_copies(bar(FULL), kStages, stage, parity);
-      wait_for_copies(bar(SCALE_FULL), kScaleSlots, slot, slot_parity);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ issuer (tcgen05.cuh: from a whole warp)
@@ -133,6 +130,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
           mma_8bit_ss_halves(d, a0 + offset + 2u * kk, b0 + offset + 2u * kk, idesc, kk > 0 ? 1u : 0u, elected);
         mma_commit_elected(bar(EMPTY + (int)stage), elected);
         mma_commit_elected(bar(SUM_FULL + (int)sum), elected);
+        if (lane == 0) barrier_arrive(bar(SUM_FULL + (int)sum));          // (the rows' scales came with the operands)
         if (++stage == (uint32_t)kStages) { stage = 0; parity ^= 1u; }
         if (++sum == 2u) { sum = 0; sum_parity ^= 1u; }
       }
@@ -142,7 +140,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
     // ------------------------------------------------------------------ adders: 128 columns of a row per thread
     const int quarter = warp & 3, half = (warp - 4) >> 2;      // a warp may read the accumulator lanes 32 quarter .. + 31
     const uint32_t lane_bits = (uint32_t)(quarter * 32) << 16;
-    uint32_t sum = 0, sum_parity = 0, slot = 0, slot_parity = 0;
+    uint32_t sum = 0, sum_parity = 0, slot = 0;
     bool alive = true;
     for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
       const int row = tile % row_tiles * kRows + quarter * 32 + lane, column0 = tile / row_tiles * kColumns + half * 128;
@@ -152,21 +150,26 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
       float2 total[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) total[i] = make_float2(0.0f, 0.0f);
-      for (int b = 0; b < blocks; ++b) {
+      // The first columns of a block are asked for before the last ones of the block in front are added.
+      uint32_t v[2][32];
+      uint32_t from = 0;
+      float next_factor = 0.0f;
+      auto begin_block = [&](int b) {
         if (b > 0 && (b & 31) == 0) {
           w_held = w_next;
           w_next = theirs[min(b + 32 + lane, blocks - 1)];
         }
-        if (alive && !wait_barrier(bar(SCALE_FULL + (int)slot), slot_parity)) { g_error = 3; alive = false; }
-        const float factor = scales_here[slot * kRows + quarter * 32 + lane] * __shfl_sync(0xffffffffu, w_held, b & 31);
-        if (++slot == (uint32_t)kScaleSlots) { slot = 0; slot_parity ^= 1u; }
         if (alive && !wait_barrier(bar(SUM_FULL + (int)sum), sum_parity)) { g_error = 3; alive = false; }
         __syncwarp();
         tensor_fence_after_sync();
-        const uint32_t from = tmem + sum * (uint32_t)kColumns + (uint32_t)(half * 128) + lane_bits;
-        const float2 both = make_float2(factor, factor);
-        uint32_t v[2][32];
+        from = tmem + sum * (uint32_t)kColumns + (uint32_t)(half * 128) + lane_bits;
         tmem_load_32_ahead(from, v[0]);
+        next_factor = scales_here[slot * kRows + quarter * 32 + lane] * __shfl_sync(0xffffffffu, w_held, b & 31);
+        if (++slot == (uint32_t)kScaleSlots) slot = 0;
+      };
+      begin_block(0);
+      for (int b = 0; b < blocks; ++b) {
+        const float2 both = make_float2(next_factor, next_factor);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           tmem_load_done(v[c & 1]);
@@ -175,13 +178,14 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
             tensor_fence_before_sync();
             __syncwarp();
             if (lane == 0) barrier_arrive(bar(SUM_FREE + (int)sum));
+            if (++sum == 2u) { sum = 0; sum_parity ^= 1u; }
+            if (b + 1 < blocks) begin_block(b + 1);
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             total[c * 16 + i] = fma_two(make_float2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), both,
                                         total[c * 16 + i]);
         }
-        if (++sum == 2u) { sum = 0; sum_parity ^= 1u; }
       }
       alive = __all_sync(0xffffffffu, alive);
       if (boxes) {
