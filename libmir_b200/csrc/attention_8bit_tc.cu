@@ -270,6 +270,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       uint32_t count = 1u;
       if ((i >= Q_FULL && i < Q_FULL + 4) || (i >= V_FULL && i < V_FULL + 2) || (i >= RAW_FREE && i < RAW_FREE + 3)) count = kConverters;
       if ((i >= P_READY && i < P_READY + 3) || i == REF_READY || i == REF_READY + 1) count = kStreamThreads;
+      if (i >= S_FULL && i < S_FULL + 3) count = 2u;
       if (i == O_FREE) count = kStreamThreads * kStreams;
       barrier_init(bar(i), count);
     }
@@ -410,6 +411,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           for (int kk = 0; kk < kDim / 32; ++kk)
             mma_8bit_ss_halves(d, q_low + (uint32_t)(kTile8 >> 4) + 2u * kk, b + 2u * kk, scores_lo, 1u, elected);
           mma_commit_elected(bar(S_FULL + (int)scores.stage), elected);
+          if (lane == 0) barrier_arrive(bar(S_FULL + (int)scores.stage));     // (what the scout left of the tile came before its keys)
           mma_commit_elected(bar(K_FREE + (int)keys.stage), elected);
           if (t == tiles - 1) mma_commit_elected(bar(Q_FREE), elected);
           keys.step(3);
@@ -594,7 +596,6 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       }
       for (int t = stream; t < w.tiles; t += kStreams) {
         const int g = g0 + t, stage = g % 3, info = g % kInfos, key0 = w.begin + t * kKeys;
-        if (alive && !wait_barrier(bar(INFO_FULL + info), (uint32_t)(g / kInfos & 1))) { g_error = 3; alive = false; }
         if (alive && !wait_barrier(bar(S_FULL + stage), (uint32_t)(g / 3 & 1))) { g_error = 3; alive = false; }
         __syncwarp();
         tensor_fence_after_sync();
