@@ -13,7 +13,12 @@
 //
 // K needs no conversion, V four instructions for two elements: a byte's sign is spread over 16 bits (prmt), shifted by 4 and masked,
 // which is the bf16 number of the same exponent field, 2^-120 times the e4m3 one (subnormals too); a product in bf16 with 2^120
-// times the page's scale puts that right.  Both products take as long as they would in bf16; the schedulers' slots bound the kernel.
+// times the page's scale puts that right.  Both products take as long as they would in bf16.
+//
+// Measured: 512 tokens at 16,384 (32 heads over 8, pages of 16): 195 us, 172 with the cache in the L2, 700 TFLOP/s; three prompts of up to
+// 2,048: 162 us.  The tensor cores are busy for a third of the time; the schedulers' slots (two thirds are taken) and the chain of
+// hand-overs of a tile, of which the widening is the longest, bound the kernel, and it is close to the instruction caches: writing a
+// loop out that is short now (the widening's, twice as long) takes 25% more.  Every wait left out was worth 1 to 3%.
 //
 // Roles: a scout reads block table and scales ahead and leaves them in shared memory; two loaders (TMA) for keys and values; an
 // issuer; eight warps that split queries and widen values; two streams of eight softmax warps that take the tiles in turn, with a

@@ -7,8 +7,11 @@
 // two accumulators in tensor memory.  The blocks' scales differ, so a block's sums cannot stay there: eight warps read them
 // (tcgen05.ld), multiply them with the block's scale and add them to 32-bit sums in registers, 128 columns of one row per thread
 // (a weight's scale is the same for 128 columns: one factor per thread and block), while the tensor cores fill the other
-// accumulator.  The tensor cores need 512 cycles for a block of a tile; a warp reads 4 x 32 columns and adds them with 64
-// two-wide FMAs, two warps a scheduler, so the adding hides behind the products.
+// accumulator.  The tensor cores need 512 cycles at their nominal rate for a block of a tile and 750 were measured without the adding; a
+// warp reads 4 x 32 columns and adds them with 64 two-wide FMAs, two warps a scheduler, 930 cycles a block with its waits, which sets
+// the pace.  4,096 x 5,120 x 25,600: 496 us, 2,160 TFLOP/s (411 us with zeros, so the power limit is part of it); 2,048 x 4,096 x 6,144:
+// 60 us, 384 tiles on 148 SMs.  A wait of its own for the rows' scales cost 8%; the first sums of a block asked for only when the block
+// before was added, 2%.
 #include <algorithm>
 #include "eight_bit_tc.cuh"
 
