@@ -78,13 +78,9 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
     if (first_position < 0) return;                               // a padding row: left as it is
   } else {
     int remaining = tile;
-    for (int r = 0; r < num_rows; ++r) {
-      const int tiles = (portion_of(query_starts, r, all_tokens).count * group + kRows - 1) / kRows;
-      if (remaining < tiles) { request = r; break; }
-      remaining -= tiles;
-    }
+    Portion portion{0, 0};
+    request = request_of_tile<kRows>(query_starts, num_rows, all_tokens, group, remaining, portion);
     if (request < 0) return;
-    const Portion portion = portion_of(query_starts, request, all_tokens);
     first_row = remaining * kRows;
     first_token = portion.first;
     count = portion.count;

@@ -104,14 +104,8 @@ struct Items {
     w.kv_head = index - rest * kv_heads.by;
     w.part = rest - from_last * num_partitions.by;
     int remaining = row_tiles - 1 - from_last;
-    w.request = -1;
     Portion portion{0, 0};
-    for (int r = 0; r < num_rows; ++r) {
-      portion = portion_of(query_starts, r, tokens);
-      const int tiles = (portion.count * group.by + kRows - 1) / kRows;
-      if (remaining < tiles) { w.request = r; break; }
-      remaining -= tiles;
-    }
+    w.request = request_of_tile<kRows>(query_starts, num_rows, tokens, group.by, remaining, portion);
     if (w.request < 0) return false;
     w.first_row = remaining * kRows;
     w.rows = min(kRows, portion.count * group.by - w.first_row);
@@ -287,12 +281,15 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   grid_dependency_wait();
-  if (threadIdx.x == 0) {
+  if (warp == 0) {
     int total = 0;
-    for (int r = 0; r < num_rows; ++r) total += (portion_of(query_starts, r, tokens).count * group.by + kRows - 1) / kRows;
-    if (*reinterpret_cast<volatile int*>(&g_error) != 0) total = 0;       // an earlier wait ran out: nothing is begun
-    row_tiles_slot = total;
-    for (int i = 0; i < 4; ++i) hidden_nans[i] = 0;
+    for (int r = lane; r < num_rows; r += 32) total += (portion_of(query_starts, r, tokens).count * group.by + kRows - 1) / kRows;
+    total = __reduce_add_sync(0xffffffffu, total);
+    if (lane == 0) {
+      if (*reinterpret_cast<volatile int*>(&g_error) != 0) total = 0;     // an earlier wait ran out: nothing is begun
+      row_tiles_slot = total;
+      for (int i = 0; i < 4; ++i) hidden_nans[i] = 0;
+    }
   }
   tensor_fence_before_sync();
   __syncthreads();
@@ -690,7 +687,8 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
       }
       if (hidden_nans[n & 3] == n + 1 && r < w.rows && total != 0.0f) {
-        // the NaN values that were left out, for the rows that see their keys
+        // the NaN values that were left out, for the rows that see their keys (over what was stored in larger words)
+        asm volatile("" ::: "memory");
         const int* table = block_table + (size_t)w.request * table_width;
 #pragma unroll 1
         for (int key = max(w.begin, window > 0 ? position - window + 1 : 0); key <= min(position, w.end - 1); ++key) {

@@ -75,6 +75,26 @@ __device__ __forceinline__ Portion portion_of(const int* query_starts, int r, in
   return {first, max(0, min(query_starts[r + 1], tokens) - first)};
 }
 
+// The request that the batch's tile `tile` (ROWS rows of one request each) belongs to, which then is the tile of that request; -1 beyond
+// the last.  Called by whole warps: 32 requests at a time are passed over together.
+template <int ROWS>
+__device__ __forceinline__ int request_of_tile(const int* query_starts, int num_rows, int tokens, int group, int& tile, Portion& portion) {
+  int r = 0;
+  for (; r + 32 < num_rows; r += 32) {
+    const int mine = portion_of(query_starts, r + (int)(threadIdx.x & 31), tokens).count;
+    const int tiles = __reduce_add_sync(0xffffffffu, (mine * group + ROWS - 1) / ROWS);
+    if (tile < tiles) break;
+    tile -= tiles;
+  }
+  for (; r < num_rows; ++r) {
+    portion = portion_of(query_starts, r, tokens);
+    const int tiles = (portion.count * group + ROWS - 1) / ROWS;
+    if (tile < tiles) return r;
+    tile -= tiles;
+  }
+  return -1;
+}
+
 // The paged 8-bit cache of one layer.
 struct Cache8 {
   const uint8_t* k;              // [pages * page_size, kv_heads, head_dim]

@@ -834,3 +834,16 @@ def test_store_of_long_pages_and_many_tokens(dim, page, kv_heads, new, before):
         plain_store(batch, qkv, slots)
         run_store(qkv, slots, cache, batch)
         same_cache(batch, cache)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prefill_attention_of_many_short_portions(dim):
+    """More requests than a warp looks at together, of no, one and a few tokens."""
+    g = seeded(98)
+    lengths = torch.randint(1, 60, (150,), generator=g).tolist()
+    new = [min(n, int(c)) for n, c in zip(lengths, torch.randint(0, 40, (150,), generator=g))]
+    batch = Batch(98, lengths, 4, 2, dim, 16)
+    out = run_prefill(batch, batch.on_gpu(), new, 0.1, extra=2)
+    want, bound = with_bound(batch.prefill(new, 0.1))
+    close(out[:sum(new)], want, bound)
+    assert (out[sum(new):] == 7.0).all()
