@@ -50,11 +50,23 @@ __device__ __forceinline__ float quad_sum(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
+// Where a partition's keys end: at the last that is seen, the partition's or the block table's.
+__device__ __forceinline__ int end_of_keys(long long seen, long long partition_end, int table_width, int page_size) {
+  return (int)min(min(seen, partition_end), min((long long)table_width * page_size, 0x7fffff00ll));
+}
+// Two elements of a query; NaN for an infinity, whose scores are no numbers.
+__device__ __forceinline__ uint32_t query_pair(const bf16* from) {
+  uint32_t pair = *reinterpret_cast<const uint32_t*>(from);
+  if ((pair & 0x7fffu) == 0x7f80u) pair |= 0x7fffu;
+  if ((pair & 0x7fff0000u) == 0x7f800000u) pair |= 0x7fff0000u;
+  return pair;
+}
+
 template <int DIM>
 __global__ void __launch_bounds__(kThreads)
 attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __restrict__ out, Cache8 cache,
-                      const int* __restrict__ block_table, int table_width, const int* __restrict__ positions,
-                      const int* __restrict__ query_starts, const int* __restrict__ context_lens, int num_rows, int group,
+                      const int* __restrict__ block_table, int table_width, const int* __restrict__ query_starts,
+                      const int* __restrict__ context_lens, int num_rows, int group,
                       float scale_log2, int window, int partition, int num_partitions, float* __restrict__ partial_o,
                       float* __restrict__ partial_ml, const float* __restrict__ sinks, int all_tokens) {
   constexpr int kStride = DIM + 8;              // bf16 elements of a shared row: an odd number of 16-byte pieces
@@ -67,25 +79,12 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
   grid_dependency_wait();
   grid_launch_dependents();
   const int part = blockIdx.x % num_partitions, tile = blockIdx.x / num_partitions, kv_head = blockIdx.y;
-  // the request and its rows: one token for each request, or portions
-  int request = -1, first_row = 0, first_token = 0, count = 1, first_position = 0;
-  if (query_starts == nullptr) {
-    const int per_request = (group + kRows - 1) / kRows;
-    request = tile / per_request;
-    first_row = tile % per_request * kRows;
-    first_token = request;
-    first_position = positions[request];
-    if (first_position < 0) return;                               // a padding row: left as it is
-  } else {
-    int remaining = tile;
-    Portion portion{0, 0};
-    request = request_of_tile<kRows>(query_starts, num_rows, all_tokens, group, remaining, portion);
-    if (request < 0) return;
-    first_row = remaining * kRows;
-    first_token = portion.first;
-    count = portion.count;
-    first_position = context_lens[request] - count;
-  }
+  // the request and its rows
+  int remaining = tile;
+  Portion portion{0, 0};
+  const int request = request_of_tile<kRows>(query_starts, num_rows, all_tokens, group, remaining, portion);
+  if (request < 0) return;
+  const int first_row = remaining * kRows, first_token = portion.first, count = portion.count, first_position = context_lens[request] - count;
   const int rows = min(kRows, count * group - first_row);
   const int lowest = first_position + first_row / group, highest = first_position + (first_row + rows - 1) / group;
   const int* table = block_table + (size_t)request * table_width;
@@ -109,11 +108,10 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
   for (int kk = 0; kk < DIM / 16; ++kk)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      query[kk][i] = *reinterpret_cast<const uint32_t*>(q + (size_t)token[i & 1] * q_stride + (size_t)head[i & 1] * DIM +
-                                                        kk * 16 + (i >> 1) * 8 + (lane & 3) * 2);
+      query[kk][i] = query_pair(q + (size_t)token[i & 1] * q_stride + (size_t)head[i & 1] * DIM + kk * 16 + (i >> 1) * 8 + (lane & 3) * 2);
 
-  const int from = max(part * partition, (window > 0 ? max(0, lowest - window + 1) : 0) / kKeys * kKeys);
-  const int end = (int)min((long long)highest + 1, (long long)(part + 1) * partition);
+  const int from = (int)min(max((long long)part * partition, (long long)((window > 0 ? max(0, lowest - window + 1) : 0) / kKeys * kKeys)), 0x7fffff00ll);
+  const int end = end_of_keys((long long)highest + 1, (long long)(part + 1) * partition, table_width, cache.page_size);
   float o[DIM / 8][4];
 #pragma unroll
   for (int n = 0; n < DIM / 8; ++n)
@@ -287,6 +285,225 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
   }
 }
 
+// Single tokens of any size: a warp by itself takes chunks of keys, up to 16 query heads of the group as the rows of the products, and needs
+// neither shared memory nor a barrier until the end.  The fragments come from the cache as they are: which element of a head is which
+// index of a product is free as long as queries and keys (values and results) agree, so a thread takes DIM / 4 neighbouring bytes of a key
+// for the scores, and DIM / 8 of each of four keys for the result.  The next chunk's bytes are on their way while this one is worked on, the
+// table's entries a chunk ahead of those.  A hidden key's values are zeros.  (64 contexts of 2,048 keys, 16 heads of 64 over 4, 67 MB: NN us.)
+template <int DIM>
+__global__ void __launch_bounds__(128)
+single_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __restrict__ out, Cache8 cache, const int* __restrict__ block_table,
+                   int table_width, const int* __restrict__ positions, int group, float scale_log2, int window, int partition,
+                   int num_partitions, float* __restrict__ partial_o, float* __restrict__ partial_ml, const float* __restrict__ sinks) {
+  constexpr int kHeads = 16, kWarps = 4, kChunk = DIM == 64 ? 32 : 16, kSteps = kChunk / 16;      // steps of 16 keys
+  constexpr int kWords = DIM / 16;              // 32-bit words of a thread's piece of a key, which are also steps of 16 elements
+  constexpr int kValueWords = DIM / 32;         // of its piece of a row of values
+  __shared__ float o_shared[kWarps][kHeads][DIM];
+  __shared__ float ml_shared[kWarps][kHeads][2];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int part = blockIdx.x % num_partitions, tile = blockIdx.x / num_partitions, kv_head = blockIdx.y;
+  const int tiles = (group + kHeads - 1) / kHeads, request = tile / tiles, first_row = tile % tiles * kHeads;
+  const int position = positions[request];
+  if (position < 0) return;                                        // a padding row: left as it is
+  const int rows = min(kHeads, group - first_row), heads = group * cache.kv_heads, first_head = kv_head * group + first_row;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int* table = block_table + (size_t)request * table_width;
+  const int first_key = (window > 0 && position >= window) ? position + 1 - window : 0;
+  const int end = end_of_keys((long long)position + 1, (long long)(part + 1) * partition, table_width, cache.page_size);
+  const int from = (int)min(max((long long)part * partition, (long long)first_key), (long long)end);
+
+  uint32_t query[kWords][4];
+#pragma unroll
+  for (int s = 0; s < kWords; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      query[s][i] = query_pair(q + (size_t)request * q_stride + (size_t)(first_head + min(g + 8 * (i & 1), rows - 1)) * DIM + t * (DIM / 4) +
+                               4 * s + 2 * (i >> 1));
+  struct Chunk {
+    uint32_t k[kSteps][2][kWords], v[kSteps][4][kValueWords];
+    int row;                                                       // by lane: a key's row in the cache, below 0: hidden
+    float k_factor;
+    uint32_t v_factor, v_rest;
+  };
+  // The table's entry for this lane's key of a chunk, -1 where the key is hidden or behind the table.
+  auto look_up = [&](int key0) {
+    const int key = key0 + lane;
+    return lane < kChunk && key < end ? page_of_block(table, table_width, key / cache.page_size, cache.pages) : -1;
+  };
+  auto fetch = [&](int key0, int page, Chunk& c) {
+    const int key = key0 + lane;
+    c.row = page >= 0 ? page * cache.page_size + key % cache.page_size : -1;
+    c.k_factor = 0.0f;
+    c.v_factor = c.v_rest = 0x3f803f80u;                           // 1
+    if (page >= 0) {
+      c.k_factor = cache.k_scales[(size_t)page * cache.kv_heads + kv_head] * scale_log2;
+      const int e = ((__float_as_int(cache.v_scales[(size_t)page * cache.kv_heads + kv_head]) >> 23) & 0xff) - 127;
+      c.v_factor = power_pair(min(e, 7) + 120);
+      c.v_rest = power_pair(max(e - 7, 0));
+    }
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = __shfl_sync(0xffffffffu, c.row, step * 16 + 8 * i + g);
+        const uint4* at = reinterpret_cast<const uint4*>(cache.k + ((size_t)max(row, 0) * cache.kv_heads + kv_head) * DIM + t * (DIM / 4));
+#pragma unroll
+        for (int w = 0; w < kWords / 4; ++w) {
+          const uint4 raw = row >= 0 ? at[w] : make_uint4(0u, 0u, 0u, 0u);
+          c.k[step][i][4 * w] = raw.x; c.k[step][i][4 * w + 1] = raw.y; c.k[step][i][4 * w + 2] = raw.z; c.k[step][i][4 * w + 3] = raw.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {                                // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the step
+        const int row = __shfl_sync(0xffffffffu, c.row, step * 16 + 2 * t + (i & 1) + 8 * (i >> 1));
+        const uint2* at = reinterpret_cast<const uint2*>(cache.v + ((size_t)max(row, 0) * cache.kv_heads + kv_head) * DIM + g * (DIM / 8));
+#pragma unroll
+        for (int w = 0; w < kValueWords / 2; ++w) {
+          const uint2 raw = row >= 0 ? at[w] : make_uint2(0u, 0u);
+          c.v[step][i][2 * w] = raw.x; c.v[step][i][2 * w + 1] = raw.y;
+        }
+      }
+    }
+  };
+  // The four numbers of a word as two pairs of bf16 times a power of two.
+  auto widen = [&](uint32_t word, uint32_t factor, uint32_t rest, uint32_t (&pair)[2]) {
+    pair[0] = times(times(lifted<0x9180>(word), factor), rest);
+    pair[1] = times(times(lifted<0xb3a2>(word), factor), rest);
+    const uint32_t nans = nan_bytes(word);
+    if (nans != 0u) {                                              // (the lifted number of a NaN is 480)
+      if (nans & 0x80u) pair[0] |= 0x7fffu;
+      if (nans & 0x8000u) pair[0] |= 0x7fff0000u;
+      if (nans & 0x800000u) pair[1] |= 0x7fffu;
+      if (nans & 0x80000000u) pair[1] |= 0x7fff0000u;
+    }
+  };
+  float o[DIM / 8][4];
+#pragma unroll
+  for (int n = 0; n < DIM / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+  constexpr int kStride = kWarps * kChunk;
+  const uint32_t lift = power_pair(120), one = 0x3f803f80u;
+  int key0 = from + warp * kChunk;
+  Chunk now, next;
+  fetch(key0, look_up(key0), now);
+  int page = look_up(key0 + kStride);
+  for (; key0 < end; key0 += kStride) {
+    fetch(key0 + kStride, page, next);
+    page = look_up(min(key0 + kStride, 0x7fffff00) + kStride);
+    float s[2 * kSteps][4], best[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < 2 * kSteps; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[j][i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        uint32_t pair[2];
+        widen(now.k[j / 2][j & 1][w], lift, one, pair);
+        mma_bf16(s[j], query[w], pair[0], pair[1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {                                // key 8j + 2t + i, of both rows
+        const int from_lane = 8 * j + 2 * t + i;
+        const bool visible = __shfl_sync(0xffffffffu, now.row, from_lane) >= 0;
+        const float factor = __shfl_sync(0xffffffffu, now.k_factor, from_lane);
+        s[j][i] = visible ? s[j][i] * factor : -INFINITY;
+        s[j][i + 2] = visible ? s[j][i + 2] * factor : -INFINITY;
+        best[0] = fmaxf(best[0], s[j][i]);
+        best[1] = fmaxf(best[1], s[j][i + 2]);
+      }
+    }
+    float shift[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float highest = fmaxf(top[i], quad_max(best[i]));
+      const float factor = highest == top[i] ? 1.0f : approximate_exp2(top[i] - highest);      // 0 where nothing was seen before
+      top[i] = highest;
+      sum[i] *= factor;
+      shift[i] = highest == -INFINITY ? 0.0f : highest;
+      if (__any_sync(0xffffffffu, factor != 1.0f)) {
+#pragma unroll
+        for (int n = 0; n < DIM / 8; ++n) {
+          o[n][2 * i] *= factor;
+          o[n][2 * i + 1] *= factor;
+        }
+      }
+    }
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      uint32_t weights[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float(&p)[4] = s[2 * step + h];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = approximate_exp2(p[i] - shift[i >> 1]);
+          sum[i >> 1] += p[i];
+        }
+        weights[2 * h] = pack(p[0], p[1]);
+        weights[2 * h + 1] = pack(p[2], p[3]);
+      }
+      uint32_t factor[4], rest[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int from_lane = step * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
+        factor[i] = __shfl_sync(0xffffffffu, now.v_factor, from_lane);
+        rest[i] = __shfl_sync(0xffffffffu, now.v_rest, from_lane);
+      }
+#pragma unroll
+      for (int w = 0; w < kValueWords; ++w) {
+        uint32_t wide[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) widen(now.v[step][i][w], factor[i], rest[i], wide[i]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {                              // element 4w + n of this thread's piece: of two keys side by side
+          const uint32_t pick = n & 1 ? 0x7632u : 0x5410u;
+          mma_bf16(o[4 * w + n], weights, __byte_perm(wide[0][n >> 1], wide[1][n >> 1], pick), __byte_perm(wide[2][n >> 1], wide[3][n >> 1], pick));
+        }
+      }
+    }
+    now = next;
+  }
+
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float total = quad_sum(sum[i]);
+    if (t == 0) {
+      ml_shared[warp][g + 8 * i][0] = top[i];
+      ml_shared[warp][g + 8 * i][1] = total;
+    }
+#pragma unroll
+    for (int n = 0; n < DIM / 8; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) o_shared[warp][g + 8 * i][(2 * t + j) * (DIM / 8) + n] = o[n][2 * i + j];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * DIM; i += 128) {
+    const int row = i / DIM, element = i % DIM;
+    float highest = -INFINITY, total = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      if (ml_shared[w][row][1] != 0.0f) highest = fmaxf(highest, ml_shared[w][row][0]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (ml_shared[w][row][1] == 0.0f) continue;                  // (no key of this warp was visible)
+      const float factor = exp2f(ml_shared[w][row][0] - highest);
+      total += ml_shared[w][row][1] * factor;
+      value += o_shared[w][row][element] * factor;
+    }
+    const size_t at = (size_t)request * heads + first_head + row;
+    if (num_partitions == 1) {
+      if (total != 0.0f && sinks != nullptr) total += exp2f(sinks[first_head + row] * kLog2e - highest);
+      out[at * DIM + element] = __float2bfloat16_rn(total == 0.0f ? 0.0f : value / total);
+    } else {
+      partial_o[(at * num_partitions + part) * DIM + element] = value;
+      if (element == 0) *reinterpret_cast<float2*>(partial_ml + (at * num_partitions + part) * 2) = make_float2(highest, total);
+    }
+  }
+}
+
 // A warp for each token and head: the partitions' parts, each relative to a maximum of its own, to one result.  A part
 // whose denominator is 0 holds nothing (no key of it was visible) and is not read.
 template <int DIM>
@@ -337,9 +554,21 @@ int mir_merge_8bit(const Attention8& a, int tokens) {
 
 int mir_attention_8bit_general(const Attention8& a, int tokens) {
   const int group = a.heads / a.cache.kv_heads;
+  if (a.query_starts == nullptr) {
+    const long long blocks = (long long)a.num_rows * ((group + 15) / 16) * a.num_partitions;
+    if (blocks > 0x7fffffffll || a.cache.kv_heads > 65535) {
+      mir_set_error("%s: %d tokens are more than one launch takes", a.what, tokens);
+      return MIR_BAD_ARGUMENT;
+    }
+    const int status = mir_launch("single_8bit", a.head_dim == 128 ? single_8bit_kernel<128> : single_8bit_kernel<64>,
+                                  dim3((unsigned)blocks, a.cache.kv_heads), dim3(128), 0, a.stream, 0, (const bf16*)a.q, a.q_stride, (bf16*)a.out,
+                                  a.cache, a.block_table, a.table_width, a.positions, group, a.scale * kLog2e, a.window, a.partition,
+                                  a.num_partitions, a.partial_o(tokens), a.partial_ml(tokens), a.sinks);
+    if (status != MIR_OK || a.num_partitions == 1) return status;
+    return mir_merge_8bit(a, tokens);
+  }
   // tiles of 64 rows; of portions an upper bound (spare ones find no request and end)
-  const long long tiles = a.query_starts == nullptr ? (long long)a.num_rows * ((group + kRows - 1) / kRows)
-                                                    : ((long long)tokens * group + kRows - 1) / kRows + a.num_rows;
+  const long long tiles = ((long long)tokens * group + kRows - 1) / kRows + a.num_rows;
   if (tiles * a.num_partitions > 0x7fffffffll || a.cache.kv_heads > 65535) {
     mir_set_error("%s: %d tokens are more than one launch takes", a.what, tokens);
     return MIR_BAD_ARGUMENT;
@@ -347,7 +576,7 @@ int mir_attention_8bit_general(const Attention8& a, int tokens) {
   const dim3 grid((unsigned)(tiles * a.num_partitions), a.cache.kv_heads);
   const int status = mir_launch("attention_8bit", a.head_dim == 128 ? attention_8bit_kernel<128> : attention_8bit_kernel<64>, grid,
                                 dim3(kThreads), 0, a.stream, 0, (const bf16*)a.q, a.q_stride, (bf16*)a.out, a.cache, a.block_table,
-                                a.table_width, a.positions, a.query_starts, a.context_lens, a.num_rows, group,
+                                a.table_width, a.query_starts, a.context_lens, a.num_rows, group,
                                 a.scale * kLog2e, a.window, a.partition, a.num_partitions, a.partial_o(tokens), a.partial_ml(tokens),
                                 a.sinks, tokens);
   if (status != MIR_OK || a.num_partitions == 1) return status;
@@ -391,7 +620,7 @@ MIR_EXPORT int mir_decode_attention_8bit_plan(int rows, int heads, int kv_heads,
     *floats = mir_decode_8bit_floats(*count, group);
     return MIR_OK;
   }
-  const long long ctas = std::max(1ll, (long long)rows * kv_heads * ((group + kRows - 1) / kRows));
+  const long long ctas = std::max(1ll, (long long)rows * kv_heads * ((group + 15) / 16));
   const long long wanted = std::max(1ll, (long long)mir_sm_count() * 4 / ctas);
   const long long tiles = std::max(1ll, (max_context + 127ll) / 128);
   const long long each = std::max(1ll, (tiles + wanted - 1) / wanted);

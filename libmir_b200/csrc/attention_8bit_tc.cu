@@ -131,20 +131,6 @@ struct Counter {                                            // stage and phase o
   }
 };
 
-// Two e4m3 numbers (bytes `selector` of `word`, spread with their signs) as bf16 numbers 2^-120 times as large.
-template <uint32_t SELECTOR> __device__ __forceinline__ uint32_t lifted(uint32_t word) {
-  uint32_t spread;
-  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(spread) : "r"(word), "n"(SELECTOR));
-  return (spread << 4) & 0x87f087f0u;
-}
-__device__ __forceinline__ uint32_t times(uint32_t pair, uint32_t factor) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(pair), "r"(factor));
-  return d;
-}
-// bf16 pair of 2^e, e from -126 to 127.
-__device__ __forceinline__ uint32_t power_pair(int e) { return (uint32_t)(e + 127) << 7 | (uint32_t)(e + 127) << 23; }
-
 __device__ __forceinline__ float max_of_three(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

@@ -61,6 +61,20 @@ __device__ __forceinline__ float approximate_exp2(float x) {
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t word) { return ((word & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ uint32_t without_nans(uint32_t word) { return word & ~((nan_bytes(word) >> 7) * 0xffu); }
 
+// Two e4m3 numbers (bytes `selector` of `word`, spread with their signs) as bf16 numbers 2^-120 times as large.
+template <uint32_t SELECTOR> __device__ __forceinline__ uint32_t lifted(uint32_t word) {
+  uint32_t spread;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(spread) : "r"(word), "n"(SELECTOR));
+  return (spread << 4) & 0x87f087f0u;
+}
+__device__ __forceinline__ uint32_t times(uint32_t pair, uint32_t factor) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(pair), "r"(factor));
+  return d;
+}
+// bf16 pair of 2^e, e from -126 to 127.
+__device__ __forceinline__ uint32_t power_pair(int e) { return (uint32_t)(e + 127) << 7 | (uint32_t)(e + 127) << 23; }
+
 // The inverse of a query row's scale 2^e for splitting it: NaN where the row holds an infinity, whose scores are no numbers.
 __device__ __forceinline__ float query_inverse(float largest, int e) {
   return largest < INFINITY ? power_of_two(-e) : __int_as_float(0x7fffffff);
