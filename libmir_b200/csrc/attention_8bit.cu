@@ -1,4 +1,5 @@
-// Attention over the 8-bit cache on mma.sync, for every size the operators take (head_dim 64 and 128, any page size):
+// Attention over the 8-bit cache on mma.sync, for every size the operators take (head_dim 64 and 128, any page size), portions and single
+// tokens, and the entry points:
 //
 //   out = sum_j p_j S_v[page of j] V_j / sum_j p_j,   p_j = exp(scale q . (S_k[page of j] K_j) - max)
 //
@@ -7,7 +8,7 @@
 // scaled on its way into shared memory and everything behind that is bf16 attention with 32-bit scores, maxima,
 // exponentials and sums (the weights p are rounded to bf16 for the product with V, as in the kernels over bf16 pages).
 //
-// A CTA takes 64 rows of one request and one kv head, and one partition of the keys.  A row is a (token, query head of the
+// Portions: a CTA takes 64 rows of one request and one kv head, and one partition of the keys.  A row is a (token, query head of the
 // group) pair: all heads of the group share the tile's keys, so that the cache is read once per group.  Four warps of 16
 // rows; the next tile's bytes are on their way in registers while this one is worked on.  Partitions' results are joined by
 // a second kernel (merge_8bit_kernel), a warp for each token and head.
@@ -289,7 +290,9 @@ attention_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __re
 // neither shared memory nor a barrier until the end.  The fragments come from the cache as they are: which element of a head is which
 // index of a product is free as long as queries and keys (values and results) agree, so a thread takes DIM / 4 neighbouring bytes of a key
 // for the scores, and DIM / 8 of each of four keys for the result.  The next chunk's bytes are on their way while this one is worked on, the
-// table's entries a chunk ahead of those.  A hidden key's values are zeros.  (64 contexts of 2,048 keys, 16 heads of 64 over 4, 67 MB: NN us.)
+// table's entries a chunk ahead of those.  A hidden key's values are zeros.  64 contexts of 2,048 keys, 16 heads of 64 over 4 (67 MB): 70 us (150
+// by tiles of 64 rows in shared memory, of which a group of four fills four); heads of 128 in pages of 24, 32 over 8 (268 MB): 204 us, 324
+// before.  Bound by the chain of a chunk (shuffles, widening, two products, a rescaled sum), not by the CTAs an SM: three to six were the same.
 template <int DIM>
 __global__ void __launch_bounds__(128)
 single_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __restrict__ out, Cache8 cache, const int* __restrict__ block_table,
@@ -323,24 +326,22 @@ single_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __restr
   struct Chunk {
     uint32_t k[kSteps][2][kWords], v[kSteps][4][kValueWords];
     int row;                                                       // by lane: a key's row in the cache, below 0: hidden
-    float k_factor;
-    uint32_t v_factor, v_rest;
+    float k_scale, v_scale;                                        // its page's
   };
+  // (What is loaded is looked at only where it is used, an iteration later: a comparison or a product here would wait for it.)
   // The table's entry for this lane's key of a chunk, -1 where the key is hidden or behind the table.
   auto look_up = [&](int key0) {
     const int key = key0 + lane;
-    return lane < kChunk && key < end ? page_of_block(table, table_width, key / cache.page_size, cache.pages) : -1;
+    return lane < kChunk && key < end ? table[key / cache.page_size] : -1;            // (end is no further than the table)
   };
   auto fetch = [&](int key0, int page, Chunk& c) {
     const int key = key0 + lane;
-    c.row = page >= 0 ? page * cache.page_size + key % cache.page_size : -1;
-    c.k_factor = 0.0f;
-    c.v_factor = c.v_rest = 0x3f803f80u;                           // 1
-    if (page >= 0) {
-      c.k_factor = cache.k_scales[(size_t)page * cache.kv_heads + kv_head] * scale_log2;
-      const int e = ((__float_as_int(cache.v_scales[(size_t)page * cache.kv_heads + kv_head]) >> 23) & 0xff) - 127;
-      c.v_factor = power_pair(min(e, 7) + 120);
-      c.v_rest = power_pair(max(e - 7, 0));
+    const bool there = page >= 0 && page < cache.pages;
+    c.row = there ? page * cache.page_size + key % cache.page_size : -1;
+    c.k_scale = c.v_scale = 1.0f;
+    if (there) {
+      c.k_scale = cache.k_scales[(size_t)page * cache.kv_heads + kv_head];
+      c.v_scale = cache.v_scales[(size_t)page * cache.kv_heads + kv_head];
     }
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
@@ -393,6 +394,9 @@ single_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __restr
   for (; key0 < end; key0 += kStride) {
     fetch(key0 + kStride, page, next);
     page = look_up(min(key0 + kStride, 0x7fffff00) + kStride);
+    const float k_factor = now.k_scale * scale_log2;
+    const int v_exponent = ((__float_as_int(now.v_scale) >> 23) & 0xff) - 127;
+    const uint32_t v_factor = power_pair(min(v_exponent, 7) + 120), v_rest = power_pair(max(v_exponent - 7, 0));
     float s[2 * kSteps][4], best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int j = 0; j < 2 * kSteps; ++j) {
@@ -408,7 +412,7 @@ single_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __restr
       for (int i = 0; i < 2; ++i) {                                // key 8j + 2t + i, of both rows
         const int from_lane = 8 * j + 2 * t + i;
         const bool visible = __shfl_sync(0xffffffffu, now.row, from_lane) >= 0;
-        const float factor = __shfl_sync(0xffffffffu, now.k_factor, from_lane);
+        const float factor = __shfl_sync(0xffffffffu, k_factor, from_lane);
         s[j][i] = visible ? s[j][i] * factor : -INFINITY;
         s[j][i + 2] = visible ? s[j][i + 2] * factor : -INFINITY;
         best[0] = fmaxf(best[0], s[j][i]);
@@ -449,8 +453,8 @@ single_8bit_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __restr
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int from_lane = step * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
-        factor[i] = __shfl_sync(0xffffffffu, now.v_factor, from_lane);
-        rest[i] = __shfl_sync(0xffffffffu, now.v_rest, from_lane);
+        factor[i] = __shfl_sync(0xffffffffu, v_factor, from_lane);
+        rest[i] = __shfl_sync(0xffffffffu, v_rest, from_lane);
       }
 #pragma unroll
       for (int w = 0; w < kValueWords; ++w) {

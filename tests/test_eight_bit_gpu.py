@@ -847,3 +847,10 @@ def test_prefill_attention_of_many_short_portions(dim):
     want, bound = with_bound(batch.prefill(new, 0.1))
     close(out[:sum(new)], want, bound)
     assert (out[sum(new):] == 7.0).all()
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, page", [(8, 2, 128, 16), (8, 2, 64, 16), (8, 2, 128, 24)])
+def test_decode_attention_at_positions_far_beyond_the_table(heads, kv_heads, dim, page):
+    batch = Batch(99, [96, 96, 96], heads, kv_heads, dim, page)
+    want, bound = with_bound(batch.decode([95, 95, 95], 0.1))
+    close(run_decode(batch, batch.on_gpu(), [95, 2 ** 31 - 1, 2 ** 31 - 2], 0.1, plan_context=2 ** 20), want, bound)
