@@ -754,7 +754,7 @@ int mir_attention_8bit_decode(const Attention8& a) {
   }
   const int columns = std::min(group, kHeads);
   const int status = columns <= 4 ? launch<4>(a, maps) : (columns <= 8 ? launch<8>(a, maps) : launch<16>(a, maps));
-  if (status != MIR_OK) return status;
+  if (status != MIR_OK || a.num_partitions == units) return status;          // (one team cuts nothing)
   return mir_launch("join_8bit", join_8bit_kernel, dim3(a.heads, a.num_rows), dim3(kJoinWarps * 32), 0, a.stream, 0, (const float*)a.scratch, a.positions,
                     a.num_rows, a.heads, a.cache.kv_heads, a.window, (int)table_keys, a.num_partitions / units, (bf16*)a.out, a.sinks);
 }

@@ -138,7 +138,7 @@ def prefill_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.
     """prefill_attention over an 8-bit cache, causal: request r has the tokens query_starts[r] .. query_starts[r + 1] - 1 of
     qkv and out, and its context_lens[r] cached tokens include them.  Rows that no request has are left as they are; missing
     pages and rows without a visible key as in decode_attention_8bit.  `max_context`: the longest context, where the caller
-    knows it better than the block table's width says; `alloc(shape, dtype)`: where scratch comes from (torch's caching
+    knows it better than the block table's width says (keys from there on need not be seen); `alloc(shape, dtype)`: where scratch comes from (torch's caching
     allocator by default)."""
     what = "prefill_attention_8bit"
     _on_this_device(what, qkv, out, k_pages, v_pages, k_scales, v_scales, block_table, query_starts, context_lens, sinks)
@@ -203,7 +203,7 @@ def linear_8bit(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, out
     makes both, and checkpoints bring them).  `x`: bfloat16 [M, K]; every row's runs of 128 columns are rounded to e4m3 with
     the least power of two as their scale (2^-118 or more) that keeps them within 448; infinities are taken as 448 times it.
     Sums are 32-bit.  `out`: bfloat16 or, the only one that accumulates, float32; `bias` has out's dtype.  x and out may be
-    row-strided views.  `alloc(shape, dtype)`: where the workspace comes from (torch's caching allocator by default)."""
+    row-strided views; x's rows begin on 8-byte boundaries.  `alloc(shape, dtype)`: where the workspace comes from (torch's caching allocator by default)."""
     _on_this_device("linear_8bit", x, weight, scales, out, bias)
     if not (x.dim() == 2 and weight.dim() == 2 and x.dtype is torch.bfloat16 and weight.dtype is E4M3):
         raise KernelError("linear_8bit: x is bfloat16 [M, K], weight float8_e4m3fn [N, K]")
