@@ -12,24 +12,32 @@
 //
 //   S^T = K Q^T    kind::f8f6f4, A = the key tile as the cache holds it (a key is a row of 128 bytes), B = the queries in two parts:
 //                  q = hi + lo, hi = e4m3(q 2^-e), lo = e5m2 of what hi leaves.  A bf16 number has eight significant bits, hi takes
-//                  four and lo the signed rest, so the two are exact down to 2^-14 of the head's largest element (e puts that
-//                  below 448) and off by at most 2^-25 of it below;
-//   O^T += V^T P   A = the value tile as the cache holds it (MN-major: nothing is transposed), B = the softmax's weights in the same
-//                  two parts: 2^-4 from hi, 2^-3 of that from lo, so a weight is off by at most 2^-7 of itself.
+//                  four and lo the signed rest, so the two are exact down to 2^-13 of the head's largest element (e puts that
+//                  below 448) and off by at most 2^-21.8 of it below (2^-14 of a largest one of 224);
+//   O^T = V^T P    A = the value tile as the cache holds it (MN-major: nothing is transposed), B = the softmax's weights in two parts
+//                  again.
 //
 // The scales: a score is multiplied by its key's page's scale on its way out of tensor memory, in 32 bits.  A value's scale 2^f goes
-// into the weight, exp2(s + f - M) with a reference M of its own (the running maximum of s + f), so that the weights of loud pages
-// stay below 448 and those of quiet ones are no smaller than their share of the result; the denominator sums exp2(s - m) in 32
-// bits.  Both references rise only when a tile's maximum exceeds them by 2^8.
+// into the weight, exp2(s + f - M), M the tile's own maximum of s + f less 8, so that the largest weight is 256.  The two parts hold
+// a weight of 2^-6 or more up to 2^-8 of itself (2^-4 from hi, 2^-4 of that from lo); smaller ones run into the formats' least numbers.
+// So the weights lie in four bands of 14 binades, band b multiplied by 2^(14 b), each with columns of its own (with up to four heads
+// the product has them anyway): whatever is 2^-56 of the tile's largest or more, 38 nats, is off by at most 2^-8 of itself, and what is
+// less by at most 2^-67 of the largest.  One reference for a whole stretch and one band lost what lay 14 nats below the largest weight,
+// or was 2^20 less loud, from the result and not from the denominator: where the keys that are ahead hold small values, or a page is
+// loud for one channel's sake, the others are all there is.
+// A tile's products start from zero; the softmax threads, one for each element of the head, add them up in 32-bit registers, relative
+// to the running maximum m of s, as the denominator is, the sum of exp2(s - m).
 //
 // Roles: four warps of softmax (a thread is a key of the tile, then an element of the head); a scout, which reads block table, scales
 // and queries ahead of everyone and leaves them in shared memory (read where they are used, those dependent loads cost every
 // tile 2,000 to 3,400 of its 4,000 cycles); a loader each for keys and values (TMA, one box for each page, or one for the tile
-// where its pages lie one behind the other); an issuer.  Two score accumulators and two weight buffers: the scores of the next tile
+// where its pages lie one behind the other); an issuer.  Two score accumulators, so that the scores of the next tile
 // are formed while the softmax works on this one, across the borders of requests and heads too.  Three stages of keys and
 // values, two CTAs an SM.  A hidden key's score becomes -inf by selection, and its row of values is zeroed in shared memory (0
 // times what lies behind a context could be NaN).  The kernel is bound by the cache's bytes: 64 contexts of 1,000 to 2,048 keys (204 MB)
-// take 48 us, 4.2 TB/s, four of up to 32,768 with 64 heads (219 MB) 52 us; a page of 16 rows is 16 pieces of 128 bytes for a head.
+// take 50 us, 4.0 TB/s, four of up to 32,768 with 64 heads (219 MB) 57 us; a page of 16 rows is 16 pieces of 128 bytes for a head.
+// (The bands and the sums in registers are 2 and 4 us of that.  Going over a tile again for what lies below two bands, instead of four
+// bands at once, took 67 and 108 us.)
 #include <algorithm>
 #include "eight_bit_tc.cuh"
 
@@ -43,18 +51,22 @@ constexpr int kKeys = 128, kDim = 128, kHeads = 16;
 constexpr int kTile = kKeys * kDim;                    // bytes of a tile of keys or of values
 constexpr int kSoftmaxThreads = 128, kThreads = kSoftmaxThreads + 4 * 32;
 constexpr int kKeyLoader = 4, kValueLoader = 5, kIssuer = 6, kScout = 7;      // warps
-constexpr uint32_t kTmemColumns = 64;                  // S^T of even and odd tiles at 0 and 16, O^T at 32
-constexpr float kRises = 8.0f, kHeadroom = 4.0f;       // log2: a reference rises when it is exceeded by kRises; M to kHeadroom below the maximum
+constexpr int kBands = 4;
+constexpr float kTop = 8.0f, kBand = 14.0f;            // log2 of a tile's largest weight; binades of a band
 constexpr int kChunk = 4, kSlots = 16;                 // tiles that the scout looks up together, pages of a tile at most
-constexpr int kHeldRows = 512;                         // positions that a CTA keeps in shared memory
 
-// Shared memory for G heads.  A part (hi or lo) of Q or P is 16 rows of 128 bytes, the columns of the products; up to 8 heads need only
-// 8 of them, and the product then reads the next part's (or what follows) as the other columns, which nobody looks at.
+// Shared memory for G heads.  A part (hi or lo) of Q is 16 rows of 128 bytes, the columns of the products; up to 8 heads need only
+// 8 of them, and the product then reads the next part's (or what follows) as the other columns, which nobody looks at.  A part of P is
+// G rows for each band.
 template <int G> struct Layout {
   static constexpr int kStages = G <= 8 ? 3 : 2;
-  static constexpr int kPart = (G <= 8 ? 8 : 16) * 128;
+  static constexpr int kPart = (G <= 8 ? 8 : 16) * 128, kWeightPart = kBands * G * 128;
   static constexpr int kOffK = 0, kOffV = kStages * kTile, kOffQ = 2 * kStages * kTile, kOffP = kOffQ + 4 * kPart;
-  static constexpr int kSmemBytes = kOffP + 4 * kPart + 1024 /* what the last part's product reads */ + 1024 /* alignment */;
+  static constexpr int kSmemBytes = kOffP + 2 * kWeightPart + 1024 /* alignment */;
+  static constexpr int kHeldRows = G == 8 ? 256 : 512;       // positions that a CTA keeps there (8 heads leave no room for more, with two CTAs)
+  // S^T of even and odd tiles at 0 and 16, O^T at 32
+  static constexpr int kValueColumns = kBands * G;
+  static constexpr uint32_t kTmemColumns = 32 + kValueColumns <= 64 ? 64 : 128;
 };
 static_assert(Layout<16>::kSmemBytes >= kLeastSharedBeside, "never beside a kernel that takes all tensor memory");
 
@@ -92,15 +104,7 @@ template <> __device__ __forceinline__ void tmem_load<8>(uint32_t address, float
 }
 template <> __device__ __forceinline__ void tmem_load<16>(uint32_t address, float (&v)[16]) { tmem_load_16(address, v); }
 
-template <int N> __device__ __forceinline__ void tmem_store(uint32_t address, const float (&v)[N]) {
-#pragma unroll
-  for (int c = 0; c < N; c += 4)
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(address + (uint32_t)c), "r"(__float_as_uint(v[c])),
-                 "r"(__float_as_uint(v[c + 1])), "r"(__float_as_uint(v[c + 2])), "r"(__float_as_uint(v[c + 3]))
-                 : "memory");
-}
-
-// Byte offset of element (row, column) of 16 rows of 128 bytes with the 128-byte swizzle.
+// Byte offset of element (row, column) of rows of 128 bytes with the 128-byte swizzle.
 __device__ __forceinline__ uint32_t swizzled(int row, int column) {
   return (uint32_t)(row * 128 + (((column >> 4) ^ (row & 7)) << 4) + (column & 15));
 }
@@ -178,7 +182,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   __shared__ uint32_t tmem_slot;
   __shared__ Stretch stretch;
   __shared__ Chunk chunks[2];
-  __shared__ int held_positions[kHeldRows];
+  __shared__ int held_positions[L::kHeldRows];
   __shared__ __align__(16) float exchange[2][2 * G][4];        // [tile parity][maxima of s, then of s + f][warp]
   __shared__ float sums[4][G];
   // Of a head's scores: scale, log2 e, and the power of two taken out of its queries, by n & 3: part n + 4's are written when the scores
@@ -201,14 +205,14 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kIssuer) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemColumns)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(L::kTmemColumns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   grid_dependency_wait();                              // the cache, the queries and the positions may come from the kernel in front
-  for (int r = threadIdx.x; r < min(num_rows, kHeldRows); r += kThreads) held_positions[r] = all_positions[r];
+  for (int r = threadIdx.x; r < min(num_rows, L::kHeldRows); r += kThreads) held_positions[r] = all_positions[r];
   __syncthreads();
-  const int* positions = num_rows <= kHeldRows ? held_positions : all_positions;
+  const int* positions = num_rows <= L::kHeldRows ? held_positions : all_positions;
   if (warp == 0) {
     // this team's stretch: all tiles over the teams, then the row that the first one lies in
     unsigned total = 0;
@@ -419,17 +423,17 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
     // ------------------------------------------------------------------ issuer (tcgen05.cuh: from a whole warp)
     constexpr uint32_t scores_hi = instruction_descriptor_8bit(kKeys, kHeads, E4M3, E4M3);
     constexpr uint32_t scores_lo = instruction_descriptor_8bit(kKeys, kHeads, E4M3, E5M2);
-    constexpr uint32_t values_hi = instruction_descriptor_8bit(kDim, kHeads, E4M3, E4M3, true);
-    constexpr uint32_t values_lo = instruction_descriptor_8bit(kDim, kHeads, E4M3, E5M2, true);
+    constexpr uint32_t values_hi = instruction_descriptor_8bit(kDim, L::kValueColumns, E4M3, E4M3, true);
+    constexpr uint32_t values_lo = instruction_descriptor_8bit(kDim, L::kValueColumns, E4M3, E5M2, true);
     const uint32_t elected = elect_one();
     const uint32_t k_low = operand_low(smem_base + L::kOffK), q_low = operand_low(smem_base + L::kOffQ);
     const uint32_t v_low = operand_low_mn_major(smem_base + L::kOffV, kTile), p_low = operand_low(smem_base + L::kOffP);
-    constexpr uint32_t kPartStep = kPart >> 4, kTileStep = kTile >> 4;
+    constexpr uint32_t kPartStep = kPart >> 4, kWeightStep = L::kWeightPart >> 4, kTileStep = kTile >> 4;
     bool alive = true;
     auto check = [&](int index, uint32_t parity) {
       if (alive && !wait_barrier(bar(index), parity)) { g_error = 2; alive = false; }
     };
-    uint32_t k_stage = 0, k_parity = 0, v_stage = 0, v_parity = 0, first_tiles = 0;
+    uint32_t k_stage = 0, k_parity = 0, v_stage = 0, v_parity = 0;
     int n = 0;                                         // parts whose scores are under way
     auto issue_scores = [&](int g) {
       const int buffer = g / kChunk & 1;
@@ -454,7 +458,6 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
         mma_commit_elected(bar(Q_FREE + (n & 1)), elected);
         ++n;
       }
-      first_tiles = (first_tiles & ~(1u << (g & 3))) | ((first ? 1u : 0u) << (g & 3));
       if (++k_stage == (uint32_t)kStages) { k_stage = 0; k_parity ^= 1u; }
     };
     // Whether all lanes see the phase with this parity complete, without waiting for it.
@@ -480,20 +483,18 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
       }
       __syncwarp();
       tensor_fence_after_sync();
-      const uint32_t a = v_low + v_stage * kTileStep, b = p_low + (uint32_t)(g & 1) * 2u * kPartStep;
-      const uint32_t begins = first_tiles >> (g & 3) & 1u;
+      const uint32_t a = v_low + v_stage * kTileStep;
       // 32 keys are 32 rows of 128 bytes further down the values, 32 bytes further along the weights
 #pragma unroll
       for (int kk = 0; kk < kKeys / 32; ++kk)
-        mma_8bit_ss_halves(tmem_o, a + (uint32_t)kk * (4096u >> 4), b + 2u * kk, values_hi, kk > 0 ? 1u : begins ^ 1u, elected);
+        mma_8bit_ss_halves(tmem_o, a + (uint32_t)kk * (4096u >> 4), p_low + 2u * kk, values_hi, kk > 0 ? 1u : 0u, elected);
 #pragma unroll
       for (int kk = 0; kk < kKeys / 32; ++kk)
-        mma_8bit_ss_halves(tmem_o, a + (uint32_t)kk * (4096u >> 4), b + kPartStep + 2u * kk, values_lo, 1u, elected);
+        mma_8bit_ss_halves(tmem_o, a + (uint32_t)kk * (4096u >> 4), p_low + kWeightStep + 2u * kk, values_lo, 1u, elected);
       mma_commit_elected(bar(V_FREE + (int)v_stage), elected);
       mma_commit_elected(bar(PV_DONE + (g & 1)), elected);
       if (++v_stage == (uint32_t)kStages) { v_stage = 0; v_parity ^= 1u; }
-      // (The scores of the tile after next take the accumulator that the softmax has read: P_READY says so.  Issued behind this
-      // product, their barrier also says that the weights' buffer is free.)
+      // (The scores of the tile after next take the accumulator that the softmax has read: P_READY says so.)
     }
   } else {
     // ------------------------------------------------------------------ softmax: thread = key of the tile, then element
@@ -501,18 +502,55 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
     const uint32_t lane_bits = (uint32_t)(warp * 32) << 16;
     bool alive = true;
     uint32_t stage = 0, stage_parity = 0;
+    // The products of a tile are added while the next one's maxima are on their way; with 16 heads before that, their scores and sums do not
+    // fit the registers together (32 contexts of 2,048 to 4,096 keys, 32 heads over 2: 42 us, 47 the other way; with 4 heads 52 and 50).
+    constexpr bool kAddsFirst = G > 8;
+    // The weights' bytes of this thread's key, zeros but for one band of each head; which it is (two bits a head).
+    unsigned char* p_smem = smem + L::kOffP;
+    uint32_t bands = 0u;
+#pragma unroll
+    for (int row = 0; row < kBands * G; ++row) p_smem[swizzled(row, r)] = p_smem[L::kWeightPart + swizzled(row, r)] = 0;
     int g = 0;
     for (int n = 0; walk.next(part); ++n) {
       const Row& of = part.of;
-      float top[G], top_weight[G], denominator[G];
+      float top[G], denominator[G], sum[G];              // of s; of exp2(s - top); this thread's element of the head, relative to top
 #pragma unroll
       for (int h = 0; h < G; ++h) {
-        top[h] = top_weight[h] = -INFINITY;
-        denominator[h] = 0.0f;
+        top[h] = -INFINITY;
+        denominator[h] = sum[h] = 0.0f;
       }
+      float reference[G];
+      // Adds the products of tile `of_tile`, whose references are still there.
+      auto add = [&](int of_tile) {
+        if (alive && !wait_barrier(bar(PV_DONE + (of_tile & 1)), (uint32_t)(of_tile >> 1 & 1))) { g_error = 3; alive = false; }
+        __syncwarp();
+        tensor_fence_after_sync();
+        float value[G];
+        constexpr int kAtOnce = 16 / G;                      // bands, the last ones first
+#pragma unroll
+        for (int b = kBands - kAtOnce; b >= 0; b -= kAtOnce) {
+          float o[16];
+          tmem_load_16(tmem_o + (uint32_t)(b * G) + lane_bits, o);
+#pragma unroll
+          for (int i = kAtOnce - 1; i >= 0; --i)
+#pragma unroll
+            for (int h = 0; h < G; ++h) value[h] = b + i == kBands - 1 ? o[i * G + h] : fmaf(value[h], 6.103515625e-5f, o[i * G + h]);      // 2^-14
+        }
+        tensor_fence_before_sync();                          // (the next product writes there behind P_READY)
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          // (2^e may lie below the 32-bit numbers where what it is multiplied with does not.  Without a visible key the products are
+          // zeros, or NaN where the only visible scores are.)
+          const float e = reference[h] > -INFINITY ? reference[h] - top[h] : 0.0f;
+          value[h] *= approximate_exp2(fmaxf(e, -100.0f));
+          if (e < -100.0f) value[h] *= approximate_exp2(e + 100.0f);
+          sum[h] += value[h];
+        }
+      };
       const float* factor_of = factors[n & 3];
       if (alive && !wait_barrier(bar(Q_READY + (n & 3)), (uint32_t)(n >> 2 & 1))) { g_error = 3; alive = false; }
       for (int t = part.first; t < part.last; ++t, ++g) {
+        if (kAddsFirst && t > part.first) add(g - 1);
         const int buffer = g / kChunk & 1, key = of.begin + t * kKeys + r;
         if (g % kChunk == 0 && alive && !wait_barrier(bar(CHUNK_FULL + buffer), (uint32_t)(g / kChunk >> 1 & 1))) { g_error = 3; alive = false; }
         const bool visible = chunks[buffer].row[g % kChunk][slot] >= 0 && key <= of.position && key >= of.first_key;
@@ -543,50 +581,42 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
         }
         if (lane < 2 * G) seen[lane][warp] = mine;
         asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");
-        float rescale[G];
-        bool grow = false;
+        if (!kAddsFirst && t > part.first) add(g - 1);         // (its weights' places are free then)
 #pragma unroll
         for (int h = 0; h < G; ++h) {
           const float4 four = *reinterpret_cast<const float4*>(seen[h]), more = *reinterpret_cast<const float4*>(seen[G + h]);
-          const float a = fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)), b = fmaxf(fmaxf(more.x, more.y), fmaxf(more.z, more.w));
-          if (a > top[h] + kRises) {
-            denominator[h] *= approximate_exp2(top[h] - a);    // 0 when nothing was seen before
+          const float a = fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w));
+          reference[h] = fmaxf(fmaxf(more.x, more.y), fmaxf(more.z, more.w)) - kTop;
+          if (a > top[h]) {
+            const float factor = approximate_exp2(top[h] - a);                          // 0 when nothing was seen before
+            denominator[h] *= factor;
+            sum[h] *= factor;
             top[h] = a;
           }
-          const bool rises = b > top_weight[h] + kRises;
-          rescale[h] = rises ? approximate_exp2(top_weight[h] - (b - kHeadroom)) : 1.0f;
-          top_weight[h] = rises ? b - kHeadroom : top_weight[h];
-          grow = grow || rises;
+          denominator[h] += visible ? approximate_exp2(s[h] - top[h]) : 0.0f;
         }
-        // O^T may be rescaled when the product with the last tile's weights is over: this thread's lane is an element of the head, its
-        // columns are the heads (all threads agree: the maxima are the same for all).
-        if (t > part.first && grow) {
-          if (alive && !wait_barrier(bar(PV_DONE + ((g - 1) & 1)), (uint32_t)(g - 1 >> 1 & 1))) { g_error = 3; alive = false; }
-          __syncwarp();
-          tensor_fence_after_sync();
-          float o[G];
-          tmem_load<G>(tmem_o + lane_bits, o);
-#pragma unroll
-          for (int h = 0; h < G; ++h) o[h] *= rescale[h];
-          tmem_store<G>(tmem_o + lane_bits, o);
-          tmem_store_wait();
-        }
-        unsigned char* p_smem = smem + L::kOffP + (g & 1) * 2 * kPart;
 #pragma unroll
         for (int h = 0; h < G; h += 2) {
           float w[2];
+          int band[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            denominator[h + i] += visible ? approximate_exp2(s[h + i] - top[h + i]) : 0.0f;
-            w[i] = visible ? approximate_exp2(s[h + i] + shift_v - top_weight[h + i]) : 0.0f;
+            // the band is the whole number next to (kTop - x) / kBand - 1/2, from 0 (a NaN's too) to the last one's
+            const float x = s[h + i] + shift_v - reference[h + i];
+            const float whole = fminf(fmaxf(fmaf(x, -1.0f / kBand, kTop / kBand - 0.5f), 0.0f), (float)(kBands - 1)) + 12582912.0f;      // 1.5 * 2^23
+            band[i] = __float_as_int(whole) & (kBands - 1);
+            w[i] = visible ? approximate_exp2(fmaf(whole - 12582912.0f, kBand, x)) : 0.0f;
           }
           uint32_t hi, lo;
           split_e4m3_e5m2(w[0], w[1], hi, lo);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            unsigned char* to = p_smem + swizzled(h + i, r);
+            const int before = (int)(bands >> (2 * (h + i)) & 3u);
+            unsigned char *to = p_smem + swizzled(band[i] * G + h + i, r), *old = p_smem + swizzled(before * G + h + i, r);
+            if (before != band[i]) old[0] = old[L::kWeightPart] = 0;
             to[0] = (unsigned char)(hi >> (8 * i));
-            to[kPart] = (unsigned char)(lo >> (8 * i));
+            to[L::kWeightPart] = (unsigned char)(lo >> (8 * i));
+            bands ^= (uint32_t)(before ^ band[i]) << (2 * (h + i));
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -600,12 +630,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
         if (lane == 0) sums[warp][h] = total;
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory");
-      if (alive && !wait_barrier(bar(PV_DONE + ((g - 1) & 1)), (uint32_t)(g - 1 >> 1 & 1))) { g_error = 3; alive = false; }
-      __syncwarp();
-      tensor_fence_after_sync();
-      float o[G];
-      tmem_load<G>(tmem_o + lane_bits, o);
-      // (the next part's first product waits for its weights, which these threads write behind this)
+      add(g - 1);
       if (alive) {
         // a part that is not the whole: in its CTA's second place if it begins here, in the first if it goes on from the team before
         const int heads_of_unit = min(group, kHeads);
@@ -614,8 +639,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
         for (int h = 0; h < G; ++h) {
           if (h >= valid_heads) break;
           float total = (sums[0][h] + sums[1][h]) + (sums[2][h] + sums[3][h]);
-          // the products are relative to 2^top_weight, the sum to 2^top
-          const float value = total == 0.0f ? 0.0f : o[h] * exp2f(top_weight[h] - top[h]);    // (NaN stays NaN)
+          const float value = sum[h];
           if (part.whole()) {
             if (total != 0.0f && sinks != nullptr) total += exp2f(sinks[head0 + h] * kLog2e - top[h]);
             out[((size_t)part.row * heads + head0 + h) * kDim + r] = __float2bfloat16_rn(total == 0.0f ? 0.0f : value / total);
@@ -635,7 +659,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   __syncthreads();
   if (warp == kIssuer) {
     tensor_fence_after_sync();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(kTmemColumns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(L::kTmemColumns) : "memory");
   }
 }
 
