@@ -601,8 +601,8 @@ static bool attention_8bit_refused(const Attention8& a, int tokens, bool shared_
     return true;
   }
   const long long need = shared_out ? mir_decode_8bit_floats(a.num_partitions, a.heads / a.cache.kv_heads) : a.num_partitions == 1 ? 0 : (long long)tokens * a.heads * a.num_partitions * (a.head_dim + 2);
-  if (need > 0 && (a.scratch == nullptr || a.scratch_floats < need)) {
-    mir_set_error("%s: scratch of %lld floats is needed, got %lld", a.what, need, a.scratch_floats);
+  if (need > 0 && (a.scratch == nullptr || a.scratch_floats < need || ((uintptr_t)a.scratch & 15))) {      // (read 16 bytes at a time)
+    mir_set_error("%s: scratch of %lld floats on a 16-byte boundary is needed, got %lld", a.what, need, a.scratch_floats);
     return true;
   }
   return false;

@@ -113,8 +113,8 @@ def decode_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.T
     its own (inside the window).  A position below 0 is a padding row: its row of `out` is left as it is.  Keys whose page the
     block table does not have (an entry below 0 or beyond the pool, or a block behind its last column) are not seen; a row
     that sees none gets zeros.  `partition`, `num_partitions`: decode_attention_8bit_plan's; where partition is not 0, keys behind
-    partition * num_partitions are not seen either.  `scratch`: float32, the plan's size; calls that may run at the same
-    time, or graphs, take one each.  `sinks`: one number per query head in the softmax's denominator."""
+    partition * num_partitions are not seen either.  `scratch`: float32, the plan's size, on a 16-byte boundary; calls that
+    may run at the same time, or graphs, take one each.  `sinks`: one number per query head in the softmax's denominator."""
     what = "decode_attention_8bit"
     _on_this_device(what, qkv, out, k_pages, v_pages, k_scales, v_scales, block_table, positions, scratch, sinks)
     rows = out.shape[0]
@@ -139,7 +139,7 @@ def prefill_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.
     qkv and out, and its context_lens[r] cached tokens include them.  Rows that no request has are left as they are; missing
     pages and rows without a visible key as in decode_attention_8bit.  `max_context`: the longest context, where the caller
     knows it better than the block table's width says (keys from there on need not be seen); `alloc(shape, dtype)`: where scratch comes from (torch's caching
-    allocator by default)."""
+    allocator by default), on a 16-byte boundary."""
     what = "prefill_attention_8bit"
     _on_this_device(what, qkv, out, k_pages, v_pages, k_scales, v_scales, block_table, query_starts, context_lens, sinks)
     rows, tokens = context_lens.numel(), out.shape[0]
