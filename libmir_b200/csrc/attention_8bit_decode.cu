@@ -737,9 +737,7 @@ int launch(const Attention8& a, const CUtensorMap (&maps)[4]) {
 
 // 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 loader, 2 issuer, 3 softmax).  Synchronises the device.
 MIR_EXPORT int mir_decode_attention_8bit_error() {
-  int flag = 0;
-  if (cudaMemcpyFromSymbol(&flag, g_error, sizeof(int)) != cudaSuccess) return -1;
-  return flag;
+  return read_flag(g_error);
 }
 
 // Whether the kernel takes these sizes: head_dim 128, pages of 8 to 128 keys that divide 128.

@@ -706,9 +706,7 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 // 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 scout or loader, 2 issuer, 3 softmax, 4 converters).
 // Synchronises the device.
 MIR_EXPORT int mir_prefill_attention_8bit_error() {
-  int flag = 0;
-  if (cudaMemcpyFromSymbol(&flag, g_error, sizeof(int)) != cudaSuccess) return -1;
-  return flag;
+  return read_flag(g_error);
 }
 
 int mir_attention_8bit_prefill(const Attention8& a, int tokens) {

@@ -96,6 +96,14 @@ inline int reserve_shared(Kernel kernel, int bytes, const char* what) {
   return MIR_OK;
 }
 
+// A kernel's error flag, once everything on the device is done: a copy alone waits for the default stream, and not for streams that do
+// not wait for that one.  -1: the flag could not be read.
+inline int read_flag(const int& flag) {
+  int value = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&value, flag, sizeof(int)) != cudaSuccess) return -1;
+  return value;
+}
+
 // The end of a loader whose next copy would go to `stage` of a ring in `phase`: the last copies into every stage are waited for (their
 // readers did already, unless one gave up), so that none is on its way when the CTA ends.
 __device__ __forceinline__ void wait_for_copies(uint32_t full0, uint32_t stages, uint32_t stage, uint32_t phase) {

@@ -335,9 +335,7 @@ int g_forced_splits = 0;          // for measurements (0: the launcher chooses)
 
 // 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 loader, 2 issuer, 3 workers).  Synchronises the device.
 MIR_EXPORT int mir_linear_8bit_few_error() {
-  int flag = 0;
-  if (cudaMemcpyFromSymbol(&flag, g_error, sizeof(int)) != cudaSuccess) return -1;
-  return flag;
+  return read_flag(g_error);
 }
 
 // Whether the kernel takes the sizes: a CTA keeps its share of K as rounded rows and scales, 40 blocks at most of it; and whether it

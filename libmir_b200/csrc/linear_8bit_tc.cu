@@ -305,9 +305,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
 // 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 loader, 2 issuer, 3 adders).
 // Synchronises the device.
 MIR_EXPORT int mir_linear_8bit_tiles_error() {
-  int flag = 0;
-  if (cudaMemcpyFromSymbol(&flag, g_error, sizeof(int)) != cudaSuccess) return -1;
-  return flag;
+  return read_flag(g_error);
 }
 
 int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, int scale_stride, const uint8_t* weight, const float* w_scales, const void* bias,

@@ -35,3 +35,15 @@ def test_scratch_cut_from_an_arena_at_an_odd_element_is_refused(dim):
         call(4)
         assert not (out == 7.0).any()
         out.fill_(7.0)
+
+
+def test_the_error_is_read_when_every_stream_is_done():
+    """A kernel on a stream of its own, which a copy on the default stream does not wait for, might still give up."""
+    from libmir_b200 import kernels
+    assert kernels.eight_bit_error() == 0                              # (loads the library)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(200_000_000)                                 # a tenth of a second
+    assert kernels.eight_bit_error() == 0
+    assert stream.query()
