@@ -514,9 +514,10 @@ template <int DIM>
 __global__ void __launch_bounds__(256)
 merge_8bit_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, bf16* __restrict__ out,
                   const int* __restrict__ positions, const int* __restrict__ query_starts, int num_rows, int tokens, int heads,
-                  int num_partitions, const float* __restrict__ sinks) {
+                  int num_partitions, const float* __restrict__ sinks, const int* __restrict__ error) {
   grid_dependency_wait();
   grid_launch_dependents();
+  if (error != nullptr && *reinterpret_cast<const volatile int*>(error) != 0) return;
   const int lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= (long long)tokens * heads) return;
@@ -553,7 +554,7 @@ int mir_merge_8bit(const Attention8& a, int tokens) {
   const long long blocks = ((long long)tokens * a.heads + 7) / 8;
   return mir_launch("merge_8bit", a.head_dim == 128 ? merge_8bit_kernel<128> : merge_8bit_kernel<64>, dim3((unsigned)blocks),
                     dim3(256), 0, a.stream, 0, a.partial_o(tokens), a.partial_ml(tokens), (bf16*)a.out, a.positions, a.query_starts,
-                    a.num_rows, tokens, a.heads, a.num_partitions, a.sinks);
+                    a.num_rows, tokens, a.heads, a.num_partitions, a.sinks, a.error);
 }
 
 int mir_attention_8bit_general(const Attention8& a, int tokens) {

@@ -670,6 +670,7 @@ join_8bit_kernel(const float* __restrict__ parts, const int* __restrict__ positi
                  int table_keys, int teams, bf16* __restrict__ out, const float* __restrict__ sinks) {
   grid_dependency_wait();
   grid_launch_dependents();
+  if (*reinterpret_cast<volatile int*>(&g_error) != 0) return;               // parts are missing
   __shared__ float4 sums_of[kJoinWarps][32];
   __shared__ float denominators[kJoinWarps];
   const int row = blockIdx.y, head = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -735,9 +736,9 @@ int launch(const Attention8& a, const CUtensorMap (&maps)[4]) {
 
 }  // namespace
 
-// 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 loader, 2 issuer, 3 softmax).  Synchronises the device.
-MIR_EXPORT int mir_decode_attention_8bit_error() {
-  return read_flag(g_error);
+// 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 loader, 2 issuer, 3 softmax).  Synchronises the device.  `next`: exchange_flag.
+MIR_EXPORT int mir_decode_attention_8bit_error(int next) {
+  return exchange_flag(g_error, next);
 }
 
 // Whether the kernel takes these sizes: head_dim 128, pages of 8 to 128 keys that divide 128.

@@ -704,9 +704,9 @@ prefill_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 }  // namespace
 
 // 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 scout or loader, 2 issuer, 3 softmax, 4 converters).
-// Synchronises the device.
-MIR_EXPORT int mir_prefill_attention_8bit_error() {
-  return read_flag(g_error);
+// Synchronises the device.  `next`: exchange_flag.
+MIR_EXPORT int mir_prefill_attention_8bit_error(int next) {
+  return exchange_flag(g_error, next);
 }
 
 int mir_attention_8bit_prefill(const Attention8& a, int tokens) {
@@ -731,5 +731,13 @@ int mir_attention_8bit_prefill(const Attention8& a, int tokens) {
                       a.table_width, a.query_starts, a.context_lens, a.num_rows, tokens, Divider(a.cache.kv_heads), Divider(group),
                       Divider(a.num_partitions), a.scale * kLog2e, a.window, a.partition, a.partial_o(tokens), a.partial_ml(tokens), (bf16*)a.out, a.sinks);
   if (status != MIR_OK || a.num_partitions == 1) return status;
-  return mir_merge_8bit(a, tokens);
+  Attention8 parts = a;
+  void* error = nullptr;
+  const cudaError_t found = cudaGetSymbolAddress(&error, g_error);
+  if (found != cudaSuccess) {
+    mir_set_error("%s: %s", a.what, cudaGetErrorString(found));
+    return MIR_CUDA_ERROR;
+  }
+  parts.error = static_cast<const int*>(error);
+  return mir_merge_8bit(parts, tokens);
 }

@@ -21,6 +21,7 @@ struct Attention8 {
   float* scratch = nullptr;
   long long scratch_floats = 0;
   const float* sinks = nullptr;        // [heads] or null
+  const int* error = nullptr;          // not 0: partitions may be missing, nothing is joined; null: none ever is
   cudaStream_t stream = nullptr;
 
   float* partial_o(long long) const { return scratch; }

@@ -97,10 +97,11 @@ inline int reserve_shared(Kernel kernel, int bytes, const char* what) {
 }
 
 // A kernel's error flag, once everything on the device is done: a copy alone waits for the default stream, and not for streams that do
-// not wait for that one.  -1: the flag could not be read.
-inline int read_flag(const int& flag) {
+// not wait for that one.  `next`: what it is from then on (0: the kernel works again), below 0: what it was.  -1: it could not be read.
+inline int exchange_flag(const int& flag, int next) {
   int value = 0;
   if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&value, flag, sizeof(int)) != cudaSuccess) return -1;
+  if (next >= 0 && (cudaMemcpyToSymbol(flag, &next, sizeof(int)) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess)) return -1;
   return value;
 }
 

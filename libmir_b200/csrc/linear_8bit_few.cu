@@ -48,6 +48,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
   __shared__ __align__(8) unsigned long long barriers[BARRIERS];
   __shared__ uint32_t tmem_slot;
   __shared__ bool go_slot;
+  __shared__ int gave_up_slot;                                // a wait of this CTA ran out, or nothing was begun: no result comes of it
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // without a cluster the CTAs walk over the tiles of 128 weight rows
   const int first_tile = blockIdx.x / splits, tile_step = gridDim.x / splits, rank = blockIdx.x % splits;
@@ -65,6 +66,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
   auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
   if (threadIdx.x == 0) {
     go_slot = *reinterpret_cast<volatile int*>(&g_error) == 0;             // an earlier wait ran out: nothing is begun
+    gave_up_slot = go_slot ? 0 : 1;
     for (int i = 0; i < BARRIERS; ++i)
       barrier_init(bar(i), i >= SUM_FREE && i < SUM_FREE + 4 ? 4u : (i >= X_READY ? (uint32_t)kWorkers : 1u));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -80,6 +82,12 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
   grid_dependency_wait();
   grid_launch_dependents();
   const bool go = go_slot;
+  volatile int* gave_up = &gave_up_slot;
+  auto give_up = [&](int role) {
+    g_error = role;
+    *gave_up = 1;
+    __threadfence_block();                                    // (before whatever this thread lets the others go on with)
+  };
 
   if (warp == kLoader) {
     if (lane == 0 && go) {
@@ -87,7 +95,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
       bool alive = true;
       for (int tile = first_tile; tile < tiles && alive; tile += tile_step)
       for (int b = 0; b < mine; ++b) {
-        if (!wait_barrier(bar(EMPTY + (int)stage), parity ^ 1u)) { g_error = 1; alive = false; break; }
+        if (!wait_barrier(bar(EMPTY + (int)stage), parity ^ 1u)) { give_up(1); alive = false; break; }
         const uint32_t full = bar(FULL + (int)stage), to = smem_base + stage * (uint32_t)stage_bytes;
         barrier_expect_bytes(full, (uint32_t)stage_bytes);
         tma_load_2d(to, &w_map, full, (first + b) * kBlock, tile * kRows);
@@ -103,7 +111,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
       const uint32_t a0 = operand_low(smem_base), x0 = operand_low(smem_u32(own_x));
       bool alive = true;
       auto check = [&](int index, uint32_t phase) {
-        if (alive && !wait_barrier(bar(index), phase)) { g_error = 2; alive = false; }
+        if (alive && !wait_barrier(bar(index), phase)) { give_up(2); alive = false; }
       };
       uint32_t stage = 0, parity = 0, buffer = 0, buffer_parity = 0;
       const int quarter = (mine + kQuarters - 1) / kQuarters;
@@ -189,7 +197,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
       for (int i = 0; i < N; ++i) total[i] = 0.0f;
       for (int b = 0; b < mine; ++b) {
         const float w_scale = __shfl_sync(0xffffffffu, b < 32 ? held[0] : held[1], b & 31);
-        if (alive && !wait_barrier(bar(SUM_FULL + (int)buffer), buffer_parity)) { g_error = 3; alive = false; }
+        if (alive && !wait_barrier(bar(SUM_FULL + (int)buffer), buffer_parity)) { give_up(3); alive = false; }
         __syncwarp();
         tensor_fence_after_sync();
         const uint32_t from = tmem + buffer * (uint32_t)N + lane_bits;
@@ -221,7 +229,7 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
 #pragma unroll
         for (int i = 0; i < N; ++i)
           if (i < m) sums[i * kRows + threadIdx.x] = total[i];
-      } else if (column < n && alive) {
+      } else if (column < n && alive && *gave_up == 0) {
         const float extra = bias == nullptr ? 0.0f : (out_float ? static_cast<const float*>(bias)[column]
                                                                 : __bfloat162float(static_cast<const bf16*>(bias)[column]));
 #pragma unroll
@@ -244,7 +252,15 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     const int column = first_tile * kRows + threadIdx.x;
-    if (threadIdx.x < kWorkers && column < n && go) {
+    // a rank that gave up has no sums: then nothing is stored, whichever rank's rows they are (a lane asks a rank)
+    int missing = 0;
+    if (warp < kWorkers / 32 && lane < splits) {
+      uint32_t there;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(&gave_up_slot)), "r"(lane));
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(missing) : "r"(there) : "memory");
+    }
+    missing = __any_sync(0xffffffffu, missing != 0);
+    if (threadIdx.x < kWorkers && column < n && missing == 0) {
       const float extra = bias == nullptr ? 0.0f : (out_float ? static_cast<const float*>(bias)[column]
                                                               : __bfloat162float(static_cast<const bf16*>(bias)[column]));
       for (int row = rank; row < m; row += splits) {
@@ -333,9 +349,9 @@ int g_forced_splits = 0;          // for measurements (0: the launcher chooses)
 
 }  // namespace
 
-// 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 loader, 2 issuer, 3 workers).  Synchronises the device.
-MIR_EXPORT int mir_linear_8bit_few_error() {
-  return read_flag(g_error);
+// 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 loader, 2 issuer, 3 workers).  Synchronises the device.  `next`: exchange_flag.
+MIR_EXPORT int mir_linear_8bit_few_error(int next) {
+  return exchange_flag(g_error, next);
 }
 
 // Whether the kernel takes the sizes: a CTA keeps its share of K as rounded rows and scales, 40 blocks at most of it; and whether it

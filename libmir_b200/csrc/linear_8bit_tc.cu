@@ -63,13 +63,14 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
   __shared__ __align__(8) unsigned long long barriers[BARRIERS];
   __shared__ __align__(16) float scales_here[kScaleSlots * kRows];
   __shared__ uint32_t tmem_slot;
-  __shared__ int tiles_slot;
+  __shared__ int tiles_slot, gave_up_slot;                    // (gave_up: a wait of this CTA ran out, no tile from then on is stored)
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem_base = smem_u32(smem), bar0 = smem_u32(&barriers[0]);
   auto bar = [&](int index) { return bar0 + 8u * (uint32_t)index; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int blocks = (k + kBlock - 1) / kBlock;
   if (threadIdx.x == 0) {
+    gave_up_slot = 0;
     tiles_slot = *reinterpret_cast<volatile int*>(&g_error) != 0 ? 0 : all_tiles;       // an earlier wait ran out: nothing is begun
     for (int i = 0; i < BARRIERS; ++i) barrier_init(bar(i), i >= SUM_FREE ? (uint32_t)kAddingWarps : (i >= SUM_FULL ? 2u : 1u));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -84,6 +85,12 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
   tensor_fence_after_sync();
   const uint32_t tmem = tmem_slot;
   const int tiles = tiles_slot;
+  volatile int* gave_up = &gave_up_slot;
+  auto give_up = [&](int role) {
+    g_error = role;
+    *gave_up = 1;
+    __threadfence_block();                                    // (before whatever this thread lets the others go on with)
+  };
   grid_dependency_wait();
   grid_launch_dependents();
 
@@ -97,7 +104,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
       for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
         const int row0 = tile % row_tiles * kRows, column0 = tile / row_tiles * kColumns;
         for (int b = 0; b < blocks; ++b) {
-          if (!wait_barrier(bar(EMPTY + stage), parity ^ 1u)) { g_error = 1; alive = false; break; }
+          if (!wait_barrier(bar(EMPTY + stage), parity ^ 1u)) { give_up(1); alive = false; break; }
           const uint32_t full = bar(FULL + stage), to = smem_base + stage * (uint32_t)kStageBytes;
           barrier_expect_bytes(full, (uint32_t)(kStageBytes + kRows * sizeof(float)));
           tma_load_2d(to, &x_map, full, b * kBlock, row0);
@@ -120,7 +127,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
     uint32_t stage = 0, parity = 0, sum = 0, sum_parity = 0;
     bool alive = true;
     auto check = [&](int index, uint32_t phase) {
-      if (alive && !wait_barrier(bar(index), phase)) { g_error = 2; alive = false; }
+      if (alive && !wait_barrier(bar(index), phase)) { give_up(2); alive = false; }
     };
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x)
       for (int b = 0; b < blocks; ++b) {
@@ -162,7 +169,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
           w_held = w_next;
           w_next = theirs[min(b + 32 + lane, blocks - 1)];
         }
-        if (alive && !wait_barrier(bar(SUM_FULL + (int)sum), sum_parity)) { g_error = 3; alive = false; }
+        if (alive && !wait_barrier(bar(SUM_FULL + (int)sum), sum_parity)) { give_up(3); alive = false; }
         __syncwarp();
         tensor_fence_after_sync();
         from = tmem + sum * (uint32_t)kColumns + (uint32_t)(half * 128) + lane_bits;
@@ -190,7 +197,7 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
                                         total[c * 16 + i]);
         }
       }
-      alive = __all_sync(0xffffffffu, alive);
+      alive = __all_sync(0xffffffffu, alive && *gave_up == 0);
       if (boxes) {
         // Results by way of shared memory, a box of 32 rows of 64 bytes a warp: the stores are whole sectors, and the next tile's
         // sums are waited for while they are on their way (a thread that stores its own row, 16 bytes of a line at a time, took
@@ -303,9 +310,9 @@ linear_8bit_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid
 }  // namespace
 
 // 0 if no bounded wait of the kernel ever ran out; else which role gave up last (1 loader, 2 issuer, 3 adders).
-// Synchronises the device.
-MIR_EXPORT int mir_linear_8bit_tiles_error() {
-  return read_flag(g_error);
+// Synchronises the device.  `next`: exchange_flag.
+MIR_EXPORT int mir_linear_8bit_tiles_error(int next) {
+  return exchange_flag(g_error, next);
 }
 
 int mir_linear_8bit_tiles(const uint8_t* codes, const float* scales, int scale_stride, const uint8_t* weight, const float* w_scales, const void* bias,

@@ -240,10 +240,10 @@ _SIGNATURES = {
         "mir_prefill_attention_8bit": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
                                        c_void_p, c_longlong, c_void_p, c_void_p],
-        "mir_decode_attention_8bit_error": [],
-        "mir_prefill_attention_8bit_error": [],
-        "mir_linear_8bit_tiles_error": [],
-        "mir_linear_8bit_few_error": [],
+        "mir_decode_attention_8bit_error": [c_int],
+        "mir_prefill_attention_8bit_error": [c_int],
+        "mir_linear_8bit_tiles_error": [c_int],
+        "mir_linear_8bit_few_error": [c_int],
         "mir_linear_8bit_few_set_splits": [c_int],
         "mir_linear_8bit_workspace": [c_int, c_int],
         "mir_quantize_weight_8bit": [c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],

@@ -166,12 +166,17 @@ def prefill_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.
         0 if scratch is None else scratch.numel(), _ptr(sinks), _stream()))
 
 
-def eight_bit_error() -> int:
-    """0 unless a bounded wait of one of the tcgen05 kernels ran out (synchronises the device); such a kernel does no work from
-    then on."""
+_ERRORS = ("mir_decode_attention_8bit_error", "mir_prefill_attention_8bit_error", "mir_linear_8bit_tiles_error", "mir_linear_8bit_few_error")
+
+
+def eight_bit_error(reset: bool = False) -> int:
+    """0 unless a bounded wait of one of the tcgen05 kernels ran out on the current device (waits for all its streams).  The calls
+    return before their kernels run, so that this alone says it: whoever relies on results asks at times, as after a step.  The
+    results of the call whose wait ran out are undefined (of linear_8bit: as they were, or right, element by element), and that
+    kernel stores nothing more from then on, until `reset` lets it work again."""
     lib = library("eight_bit")
-    return int(lib.mir_decode_attention_8bit_error() or lib.mir_prefill_attention_8bit_error()
-               or lib.mir_linear_8bit_tiles_error() or lib.mir_linear_8bit_few_error())
+    found = [getattr(lib, name)(0 if reset else -1) for name in _ERRORS]
+    return next((error for error in found if error), 0)
 
 
 def quantize_weight_8bit(weight: torch.Tensor) -> tuple:

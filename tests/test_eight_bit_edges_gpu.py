@@ -47,3 +47,55 @@ def test_the_error_is_read_when_every_stream_is_done():
         torch.cuda._sleep(200_000_000)                                 # a tenth of a second
     assert kernels.eight_bit_error() == 0
     assert stream.query()
+
+
+def test_a_kernel_that_gave_up_stores_nothing_until_it_is_reset():
+    """The flag that a wait which runs out sets, set by the reader here (no wait runs out): every call leaves its result as it is, what
+    it adds to among them, and joins nothing; afterwards all is as before."""
+    from libmir_b200 import kernels
+    from libmir_b200.kernels import eight_bit
+    lib = kernels.library("eight_bit")
+    heads, kv_heads, page = 8, 2, 16
+    batch = Batch(2, [3000, 40], heads, kv_heads, 128, page)
+    cache, table = batch.on_gpu(), batch.table.cuda()
+    positions = torch.tensor([2999, 39], dtype=torch.int32).cuda()
+    plan = kernels.decode_attention_8bit_plan(2, heads, kv_heads, 128, page, 3000)
+    scratch = torch.zeros(plan[2], device="cuda")
+    codes = torch.ones(1000, 1024, device="cuda").to(eight_bit.E4M3)
+    scales = torch.ones(8, 8, device="cuda")
+
+    def decode(out):
+        kernels.decode_attention_8bit(batch.qkv[:2].cuda(), out, *cache, table, positions, page, heads, kv_heads, 128, 0.1, None, plan[0],
+                                      plan[1], scratch)
+
+    def prefill(counts):
+        def call(out):
+            starts = torch.tensor([0, counts[0], sum(counts)], dtype=torch.int32).cuda()
+            kernels.prefill_attention_8bit(batch.qkv[:sum(counts)].cuda(), out, *cache, table, starts, positions + 1, page, heads, kv_heads,
+                                           128, 0.1, None)
+        return call
+
+    def linear(out):
+        kernels.linear_8bit(torch.ones(out.shape[0], 1024, dtype=torch.bfloat16, device="cuda"), codes, scales, out,
+                            accumulate=out.dtype == torch.float32)
+    calls = [(decode, 2, heads * 128, torch.bfloat16), (prefill([2, 1]), 3, heads * 128, torch.bfloat16),
+             (prefill([2900, 40]), 2940, heads * 128, torch.bfloat16)]
+    calls += [(linear, m, 1000, dtype) for m in (1, 16, 40, 128, 129, 300) for dtype in (torch.bfloat16, torch.float32)]
+    try:
+        for name in eight_bit._ERRORS:
+            assert getattr(lib, name)(3) == 0
+        assert kernels.eight_bit_error() == 3
+        for call, rows, width, dtype in calls:
+            out = torch.full((rows, width), 7.0, dtype=dtype, device="cuda")
+            call(out)
+            assert (out == 7.0).all()
+        assert kernels.eight_bit_error(reset=True) == 3 and kernels.eight_bit_error() == 0
+    finally:
+        kernels.eight_bit_error(reset=True)
+    for call, rows, width, dtype in calls:
+        out = torch.full((rows, width), 7.0, dtype=dtype, device="cuda")
+        call(out)
+        assert not (out == 7.0).any() if call is linear else (out != 7.0).any(dim=1).all()
+        if call is linear:
+            assert (out == 1024.0 + (7.0 if dtype == torch.float32 else 0.0)).all()
+    assert kernels.eight_bit_error() == 0
