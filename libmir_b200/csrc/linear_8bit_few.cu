@@ -212,12 +212,13 @@ linear_8bit_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_c
           }
 #pragma unroll
           for (int i = 0; i < kChunk; i += 4) {
-            // (a row's scale is a power of two: only the addition rounds, and the product with the weight's scale)
+            // the two scales first: sums times a row's scale alone may lie beyond the 32-bit numbers where the results do not (a row's
+            // scale is a power of two, so only the addition rounds)
             const float4 x_scale = *reinterpret_cast<const float4*>(scales + b * N + c + i);
-            total[c + i] = fmaf(v[i] * x_scale.x, w_scale, total[c + i]);
-            total[c + i + 1] = fmaf(v[i + 1] * x_scale.y, w_scale, total[c + i + 1]);
-            total[c + i + 2] = fmaf(v[i + 2] * x_scale.z, w_scale, total[c + i + 2]);
-            total[c + i + 3] = fmaf(v[i + 3] * x_scale.w, w_scale, total[c + i + 3]);
+            total[c + i] = fmaf(v[i], x_scale.x * w_scale, total[c + i]);
+            total[c + i + 1] = fmaf(v[i + 1], x_scale.y * w_scale, total[c + i + 1]);
+            total[c + i + 2] = fmaf(v[i + 2], x_scale.z * w_scale, total[c + i + 2]);
+            total[c + i + 3] = fmaf(v[i + 3], x_scale.w * w_scale, total[c + i + 3]);
           }
         }
         if (++buffer == (uint32_t)kBuffers) { buffer = 0; buffer_parity ^= 1u; }

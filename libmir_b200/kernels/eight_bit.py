@@ -207,7 +207,7 @@ def linear_8bit(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, out
     `weight`: e4m3 [N, K] with K a multiple of 16, `scales`: any float32 [ceil(N / 128), ceil(K / 128)] (quantize_weight_8bit
     makes both, and checkpoints bring them).  `x`: bfloat16 [M, K]; every row's runs of 128 columns are rounded to e4m3 with
     the least power of two as their scale (2^-118 or more) that keeps them within 448; infinities are taken as 448 times it.
-    Sums are 32-bit.  `out`: bfloat16 or, the only one that accumulates, float32; `bias` has out's dtype.  x and out may be
+    Sums are 32-bit, and so is the product of a block's two scales (below 2^-126 it loses bits).  `out`: bfloat16 or, the only one that accumulates, float32; `bias` has out's dtype.  x and out may be
     row-strided views; x's rows begin on 8-byte boundaries.  `alloc(shape, dtype)`: where the workspace comes from (torch's caching allocator by default)."""
     _on_this_device("linear_8bit", x, weight, scales, out, bias)
     if not (x.dim() == 2 and weight.dim() == 2 and x.dtype is torch.bfloat16 and weight.dtype is E4M3):

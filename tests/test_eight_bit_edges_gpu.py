@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from test_eight_bit_gpu import Batch
+import plain_eight_bit as plain
+from test_eight_bit_gpu import E4M3, Batch, close, product_bound, seeded
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +100,24 @@ def test_a_kernel_that_gave_up_stores_nothing_until_it_is_reset():
         if call is linear:
             assert (out == 1024.0 + (7.0 if dtype == torch.float32 else 0.0)).all()
     assert kernels.eight_bit_error() == 0
+
+
+@pytest.mark.parametrize("size", [1e35, 1e-35])
+@pytest.mark.parametrize("n", [200, 19000])
+@pytest.mark.parametrize("m", [1, 16, 17, 128, 129])
+def test_products_of_very_large_and_very_small_rows(m, n, size):
+    """Rows near both ends of the 32-bit numbers whose results are ordinary ones: what is on the way there is, too, with few rows and with
+    many.  (Blocks' scales that multiply to less than the normal numbers, 2^-126, are held to 2^-150: 2^25 times that at most for 128
+    products of two numbers of 448, for each block.)"""
+    from libmir_b200 import kernels
+    g = seeded(m)
+    k = 272
+    x = (torch.randn(m, k, generator=g) * size).bfloat16()
+    codes = (torch.randn(n, k, generator=g) * 100).clamp(-448, 448).to(E4M3)
+    scales = torch.rand(-(-n // 128), -(-k // 128), generator=g) * 1e-3 + 1e-4
+    weight = plain.weight_values(codes, scales)
+    out = torch.full((m, n), 7.0, device="cuda")
+    kernels.linear_8bit(x.cuda(), codes.cuda(), scales.cuda(), out)
+    want = plain.rounded_rows(x) @ weight.t()
+    bound = product_bound(x, weight, torch.float32, torch.zeros(1, dtype=torch.float64))(want)
+    close(out, want, bound - 1e-35 + 3 * 2.0 ** -125)
