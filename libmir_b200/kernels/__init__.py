@@ -308,6 +308,9 @@ def read_prompt_attention_trace():
     return np.array(host, dtype=np.int64).reshape(rows, 16)
 
 
+_LAUNCH_MODE = None              # what set_programmatic_launch was told last
+
+
 def library(name: str) -> ctypes.CDLL:
     """The loaded native library `name`, compiled first if its sources changed or it was never built."""
     lib = _LIBS.get(name)
@@ -324,6 +327,10 @@ def library(name: str) -> ctypes.CDLL:
         function = getattr(lib, symbol)
         function.argtypes = argtypes
         function.restype = _RESULTS.get(symbol, c_int)
+    lib.mir_set_pdl.argtypes = [c_int]
+    lib.mir_set_pdl.restype = None
+    if _LAUNCH_MODE is not None:
+        lib.mir_set_pdl(_LAUNCH_MODE)
     _LIBS[name] = lib
     return lib
 
@@ -344,11 +351,12 @@ def set_programmatic_launch(mode) -> None:
     first weights are then on their way while the kernel before them drains.  What is read ahead of that wait (weights of
     products and norms, slots, positions, block tables) must not come from the launches in front of it: between the kernel
     that writes it and the one that reads it lies a copy, a library's kernel or decode_prepare, and one launch more."""
-    for name in ("core", "bf16", "eight_bit"):
-        lib = library(name)
-        lib.mir_set_pdl.argtypes = [c_int]
-        lib.mir_set_pdl.restype = None
-        lib.mir_set_pdl(int(mode))
+    global _LAUNCH_MODE
+    _LAUNCH_MODE = int(mode)
+    for name in ("core", "bf16"):
+        library(name)
+    for lib in _LIBS.values():             # (libraries that are loaded later are told then)
+        lib.mir_set_pdl(_LAUNCH_MODE)
 
 
 def launch_counts(reset: bool = False) -> dict:

@@ -1,5 +1,9 @@
 """The 8-bit operators without a GPU: addresses, empty batches and libraries that nobody asked for."""
 
+import pathlib
+import subprocess
+import sys
+
 import pytest
 
 from libmir_b200 import kernels
@@ -15,3 +19,18 @@ def test_scratch_off_its_16_bytes_is_refused(off):
     assert native_prefill(dim=64, parts=2, scratch=AT + off, floats=1 << 24) == BAD_ARGUMENT
     message = kernels.library("eight_bit").mir_last_error().decode()
     assert "scratch" in message and "16-byte" in message
+
+
+def test_a_launch_mode_is_told_to_the_8bit_library_when_it_is_loaded():
+    """set_programmatic_launch neither compiles nor loads the library for callers that never use it; those who do get the mode that was
+    set last, before or after."""
+    program = """
+from libmir_b200 import kernels
+kernels.set_programmatic_launch(2)
+assert sorted(kernels.loaded_libraries()) == ["bf16", "core"], kernels.loaded_libraries()
+assert kernels.library("eight_bit").mir_get_pdl() == kernels.library("core").mir_get_pdl() == 2
+kernels.set_programmatic_launch(False)
+assert [kernels.library(name).mir_get_pdl() for name in ("core", "bf16", "eight_bit")] == [0, 0, 0]
+"""
+    done = subprocess.run([sys.executable, "-c", program], cwd=pathlib.Path(__file__).parents[1], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
