@@ -591,7 +591,7 @@ int mir_attention_8bit_general(const Attention8& a, int tokens) {
 static bool attention_8bit_refused(const Attention8& a, int tokens, bool shared_out) {
   const bool bad =
       (a.head_dim != 64 && a.head_dim != 128) || a.heads <= 0 || a.cache.kv_heads <= 0 || a.heads % a.cache.kv_heads ||
-      a.cache.page_size <= 0 || a.cache.pages <= 0 || (long long)a.cache.pages * a.cache.page_size > 0x7fffffffll || a.table_width <= 0 ||
+      a.cache.page_size <= 0 || a.cache.pages <= 0 || (long long)a.cache.pages * a.cache.page_size > 0x7fffffffll || a.table_width < 0 || (a.table_width == 0 && a.num_rows > 0) ||
       !(a.scale > 0.0f) || a.window < 0 || (a.q_stride % 8) || a.q_stride < (long long)a.heads * a.head_dim || ((uintptr_t)a.q & 15) ||
       ((uintptr_t)a.out & 15) || ((uintptr_t)a.cache.k & 15) || ((uintptr_t)a.cache.v & 15) ||
       (shared_out ? a.partition != 0 : a.partition <= 0 || a.partition % 128 != 0) || a.num_partitions <= 0 || a.num_partitions > 65535 || a.num_rows < 0 || tokens < 0;

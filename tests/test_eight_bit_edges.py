@@ -34,3 +34,11 @@ assert [kernels.library(name).mir_get_pdl() for name in ("core", "bf16", "eight_
 """
     done = subprocess.run([sys.executable, "-c", program], cwd=pathlib.Path(__file__).parents[1], capture_output=True, text=True)
     assert done.returncode == 0, done.stderr
+
+
+def test_an_empty_batch_has_an_empty_table():
+    """No rows, and a table of no columns, as a step without requests has them: nothing to do, nothing to refuse.  With rows it is refused."""
+    assert native_decode(rows=0, table=None, width=0) == 0 and native_decode(dim=64, rows=0, table=None, width=0) == 0
+    assert native_prefill(rows=0, tokens=0, table=None, width=0) == 0
+    for call in (native_decode, native_prefill):
+        assert call(width=0) == call(width=-1) == call(rows=0, width=-1) == BAD_ARGUMENT

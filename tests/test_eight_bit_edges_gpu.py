@@ -121,3 +121,18 @@ def test_products_of_very_large_and_very_small_rows(m, n, size):
     want = plain.rounded_rows(x) @ weight.t()
     bound = product_bound(x, weight, torch.float32, torch.zeros(1, dtype=torch.float64))(want)
     close(out, want, bound - 1e-35 + 3 * 2.0 ** -125)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_step_without_requests(dim):
+    from libmir_b200 import kernels
+    batch = Batch(3, [40], 8, 2, dim, 16)
+    cache, empty = batch.on_gpu(), torch.zeros(0, dtype=torch.int32, device="cuda")
+    qkv, out = batch.qkv[:0].cuda(), torch.zeros(0, 8 * dim, dtype=torch.bfloat16, device="cuda")
+    plan = kernels.decode_attention_8bit_plan(0, 8, 2, dim, 16, 0)
+    for width in (0, 5):
+        table = torch.zeros(0, width, dtype=torch.int32, device="cuda")
+        kernels.decode_attention_8bit(qkv, out, *cache, table, empty, 16, 8, 2, dim, 0.1, None, plan[0], plan[1],
+                                      torch.empty(plan[2], device="cuda"))
+        kernels.prefill_attention_8bit(qkv, out, *cache, table, torch.zeros(1, dtype=torch.int32, device="cuda"), empty, 16, 8, 2, dim, 0.1, None)
+        kernels.store_kv_8bit(qkv, empty, *cache, 16, 8, 2, dim)
