@@ -229,6 +229,7 @@ def linear_8bit(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, out
     workspace = None
     if size:                    # (up to 16 rows are rounded where they are used)
         workspace = alloc((size,), torch.uint8) if alloc is not None else torch.empty((size,), dtype=torch.uint8, device=x.device)
+        size = workspace.numel() * workspace.element_size()          # (what there is, which the launcher checks)
     _check(lib, lib.mir_linear_8bit(x.data_ptr(), x.stride(0), weight.data_ptr(), scales.data_ptr(), _ptr(bias), out.data_ptr(),
                                     out.stride(0), int(out.dtype is torch.float32), int(accumulate), m, n, k, _ptr(workspace),
                                     size, _stream()))

@@ -136,3 +136,17 @@ def test_a_step_without_requests(dim):
                                       torch.empty(plan[2], device="cuda"))
         kernels.prefill_attention_8bit(qkv, out, *cache, table, torch.zeros(1, dtype=torch.int32, device="cuda"), empty, 16, 8, 2, dim, 0.1, None)
         kernels.store_kv_8bit(qkv, empty, *cache, 16, 8, 2, dim)
+
+
+def test_a_workspace_that_is_too_small_or_off_its_16_bytes_is_refused():
+    from libmir_b200 import kernels
+    from libmir_b200.errors import KernelError
+    x = torch.ones(20, 256, dtype=torch.bfloat16, device="cuda")
+    codes, scales = torch.ones(130, 256, device="cuda").to(E4M3), torch.ones(2, 2, device="cuda")
+    out = torch.full((20, 130), 7.0, device="cuda")
+    for take in (lambda n: slice(0, n - 1), lambda n: slice(8, n + 8), lambda n: slice(0, 0)):
+        with pytest.raises(KernelError, match="workspace"):
+            kernels.linear_8bit(x, codes, scales, out, alloc=lambda shape, dtype: torch.empty(shape[0] + 64, dtype=dtype, device="cuda")[take(shape[0])])
+    assert (out == 7.0).all()
+    kernels.linear_8bit(x, codes, scales, out, alloc=lambda shape, dtype: torch.empty(shape[0] + 64, dtype=dtype, device="cuda")[16:])
+    assert (out == 256.0).all()
