@@ -593,7 +593,8 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
             sum[h] *= factor;
             top[h] = a;
           }
-          denominator[h] += visible ? approximate_exp2(s[h] - top[h]) : 0.0f;
+          // (scores of -inf weigh nothing, also where there is no other yet)
+          denominator[h] += visible ? approximate_exp2(s[h] - (top[h] > -INFINITY ? top[h] : 0.0f)) : 0.0f;
         }
 #pragma unroll
         for (int h = 0; h < G; h += 2) {
@@ -602,7 +603,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             // the band is the whole number next to (kTop - x) / kBand - 1/2, from 0 (a NaN's too) to the last one's
-            const float x = s[h + i] + shift_v - reference[h + i];
+            const float x = s[h + i] + shift_v - (reference[h + i] > -INFINITY ? reference[h + i] : 0.0f);
             const float whole = fminf(fmaxf(fmaf(x, -1.0f / kBand, kTop / kBand - 0.5f), 0.0f), (float)(kBands - 1)) + 12582912.0f;      // 1.5 * 2^23
             band[i] = __float_as_int(whole) & (kBands - 1);
             w[i] = visible ? approximate_exp2(fmaf(whole - 12582912.0f, kBand, x)) : 0.0f;

@@ -127,3 +127,27 @@ def test_many_requests_some_of_them_with_a_key_ahead(heads, kv_heads):
     picked = [i for i in range(0, 40, 3) if positions[i] >= 0] + [1, 20]
     want, size = batch.decode([p if i in picked else -1 for i, p in enumerate(positions)], scale)
     close(first[picked], want[picked], attention_bound(want, size)[picked] + floor(batch, 900))
+
+
+def hidden_by_their_scores(form, block):
+    """Keys whose scores are -inf in 32 bits, alone in their tile; the others' scores are 0."""
+    heads, kv_heads, dim, page = form
+    keys = 384 + page
+    batch = Batch(13, [keys], heads, kv_heads, dim, page)
+    batch.qkv[:, :heads * dim] = 1e30
+    batch.k.codes[:] = 0.0
+    for at in range(0, 128 // page * page) if block == "first" else range(-(-384 // page) * page, keys):
+        where = int(batch.table[0, at // page]), at % page
+        batch.k.codes[where] = -448.0
+        batch.k.scales[where[0]] = 2.0 ** 60
+    return batch, keys
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("block", ["first", "last"])
+def test_single_tokens_with_scores_below_the_32_bit_numbers(form, block):
+    """They weigh nothing, the others all the same."""
+    batch, keys = hidden_by_their_scores(form, block)
+    out = run_decode(batch, batch.on_gpu(), [keys - 1], 0.1)
+    want, size = batch.decode([keys - 1], 0.1)
+    close(out, want, attention_bound(want, size))
