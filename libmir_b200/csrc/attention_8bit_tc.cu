@@ -211,7 +211,7 @@ __device__ __forceinline__ float softmax_tile(uint32_t scores, int first, int lo
   factor = grow ? approximate_exp2(before - now) : 1.0f;                  // 0 when nothing was seen before
   own_factor = reference == now ? 1.0f : approximate_exp2(reference - now);
   reference = now;
-  const float down = (MASKED && reference == -INFINITY) ? 0.0f : -reference;       // (a row that has seen nothing yet)
+  const float down = reference == -INFINITY ? 0.0f : -reference;       // (a row that has seen nothing yet, or scores of -inf alone)
   const float2 downs = make_float2(down, down);
   float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll

@@ -14,7 +14,7 @@ import pytest
 import torch
 
 import plain_eight_bit as plain
-from test_eight_bit_gpu import Batch, attention_bound, close, run_decode, seeded
+from test_eight_bit_gpu import Batch, attention_bound, close, run_decode, run_prefill, seeded
 
 pytestmark = pytest.mark.gpu
 
@@ -151,3 +151,13 @@ def test_single_tokens_with_scores_below_the_32_bit_numbers(form, block):
     out = run_decode(batch, batch.on_gpu(), [keys - 1], 0.1)
     want, size = batch.decode([keys - 1], 0.1)
     close(out, want, attention_bound(want, size))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("block", ["first", "last"])
+def test_portions_with_scores_below_the_32_bit_numbers(form, block):
+    batch, keys = hidden_by_their_scores(form, block)
+    for new in (5, 150):
+        out = run_prefill(batch, batch.on_gpu(), [new], 0.1)
+        want, size = batch.prefill([new], 0.1)
+        close(out, want, attention_bound(want, size))
