@@ -655,8 +655,12 @@ MIR_EXPORT int mir_decode_attention_8bit(const void* q, long long q_stride, void
   return shared_out ? mir_attention_8bit_decode(a) : mir_attention_8bit_general(a, rows);
 }
 
-// How portions are split over the keys: not at all where their tiles of rows and kv heads fill the SMs; a few tokens behind a long context
-// are fewer items than SMs, and each would walk over all of it (16 tokens at 16,384, 32 heads over 8: 8 items).
+// How portions are split over the keys: a few tokens behind a long context are fewer items (tiles of rows and kv heads) than CTAs that run
+// at once, and each would walk over all of it (16 tokens at 16,384, 32 heads over 8: 8 items).  The cut is the one with the least
+// time in tiles of keys: as many rounds as the items take, each a partition's tiles and the start of an item, which is worth some four
+// tiles of the tcgen05 kernel and one of the other, and the joining; a sixth has to be gained.  Heads of 128: 16 tokens at 16,384 take 165 us
+// in one part, 34 in 17 (one round), 51 in 26 (two); 300 tokens 180 and in 3 parts 135; 512 tokens, 128 items, 171 and in 2 parts 187.  Heads of
+// 64, 16 over 4: 16 tokens at 1,000 65 and in 2 parts 37, 400 at 16,384 in 2 parts 573 and in 5 472.
 MIR_EXPORT int mir_prefill_attention_8bit_plan(int rows, int tokens, int heads, int kv_heads, int head_dim, int page_size, int max_context,
                                                int* keys, int* count, long long* floats) {
   if (rows < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context < 0 || page_size <= 0) {
@@ -667,11 +671,24 @@ MIR_EXPORT int mir_prefill_attention_8bit_plan(int rows, int tokens, int heads, 
   const long long group = heads / kv_heads, tile = mir_decode_8bit_takes(head_dim, page_size) ? 128 : kRows;
   const long long items = std::max(1ll, (tokens * group + tile - 1) / tile) * kv_heads;       // (at least as many as that)
   const long long tiles = std::max(1ll, (max_context + 127ll) / 128);
-  // up to two partitions' items an SM, at least four tiles of keys each
-  const long long wanted = std::max(1ll, std::min(2ll * mir_sm_count() / items, tiles / 4));
-  const long long each = (tiles + wanted - 1) / wanted;
+  // one CTA an SM of the tcgen05 kernel, two of the other
+  const bool tensor_memory = mir_decode_8bit_takes(head_dim, page_size);
+  const long long at_once = mir_sm_count() * (tensor_memory ? 1ll : 2ll), start = tensor_memory ? 4 : 1, join = tensor_memory ? 2 : 1;
+  long long each = tiles, parts = 1, least = (items + at_once - 1) / at_once * (tiles + start) * 5 / 6 + 1;
+  // as many partitions as one or two rounds take, at least four tiles of keys each
+  for (long long rounds = 1; rounds <= 2; ++rounds) {
+    const long long wanted = std::min(rounds * at_once / items, tiles / 4);
+    if (wanted < 2) continue;
+    const long long keys_each = (tiles + wanted - 1) / wanted, there = (tiles + keys_each - 1) / keys_each;
+    const long long time = (items * there + at_once - 1) / at_once * (keys_each + start) + join;
+    if (time < least) {
+      least = time;
+      each = keys_each;
+      parts = there;
+    }
+  }
   *keys = (int)(each * 128);
-  *count = (int)((tiles + each - 1) / each);
+  *count = (int)parts;
   *floats = *count == 1 ? 0 : (long long)tokens * heads * *count * (head_dim + 2);
   return MIR_OK;
 }

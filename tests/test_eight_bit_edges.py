@@ -1,5 +1,6 @@
 """The 8-bit operators without a GPU: addresses, empty batches and libraries that nobody asked for."""
 
+import ctypes
 import pathlib
 import subprocess
 import sys
@@ -42,3 +43,32 @@ def test_an_empty_batch_has_an_empty_table():
     assert native_prefill(rows=0, tokens=0, table=None, width=0) == 0
     for call in (native_decode, native_prefill):
         assert call(width=0) == call(width=-1) == call(rows=0, width=-1) == BAD_ARGUMENT
+
+
+def prefill_plan(tokens, heads, kv_heads, dim, context):
+    keys, count, floats = ctypes.c_int(), ctypes.c_int(), ctypes.c_longlong()
+    assert kernels.library("eight_bit").mir_prefill_attention_8bit_plan(1, tokens, heads, kv_heads, dim, 16, context, ctypes.byref(keys),
+                                                                        ctypes.byref(count), ctypes.byref(floats)) == 0
+    return keys.value, count.value, floats.value
+
+
+@pytest.mark.parametrize("dim, rows, at_once, start", [(128, 128, 148, 4), (64, 64, 296, 1)])
+@pytest.mark.parametrize("tokens, heads, kv_heads", [(1, 32, 8), (4, 32, 8), (16, 32, 8), (100, 28, 4), (300, 32, 8), (400, 32, 8), (512, 32, 8),
+                                                     (2048, 32, 8), (3, 1, 1), (5000, 64, 8)])
+@pytest.mark.parametrize("context", [1, 500, 5000, 16513, 131072, 2147483391])
+def test_portions_are_cut_over_the_keys_only_where_that_takes_less_time(dim, rows, at_once, start, tokens, heads, kv_heads, context):
+    """Partitions cover the context in whole tiles of 128 keys, and their items, each some tiles' time longer than its keys, take a sixth
+    less time on the CTAs that run at once than uncut ones."""
+    keys, count, floats = prefill_plan(tokens, heads, kv_heads, dim, context)
+    tiles, items = -(-context // 128), -(-tokens * heads // kv_heads // rows) * kv_heads
+    assert keys % 128 == 0 and keys * count >= context and (count == 1 or keys * (count - 1) < context) and count <= 65535
+    assert floats == (0 if count == 1 else tokens * heads * count * (dim + 2))
+    time = -(-items * count // at_once) * (keys // 128 + start)
+    assert count == 1 or time < -(-items // at_once) * (tiles + start) * 5 / 6 + 1
+    if tiles >= 16 and items * 4 <= at_once:
+        assert count >= 2
+
+
+def test_a_portion_whose_items_fill_the_machine_is_not_cut():
+    """512 tokens behind 16,001 keys, 32 heads over 8: 128 items on 148 SMs."""
+    assert prefill_plan(512, 32, 8, 128, 16513)[1] == 1
