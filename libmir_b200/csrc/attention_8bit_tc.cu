@@ -7,7 +7,7 @@
 // A CTA per SM walks over items, heaviest first; every ring and barrier runs on across them.  Per tile of 128 keys:
 //
 //   S = Q K^T     kind::f8f6f4, K as the cache holds it, Q in two parts q = hi + lo, hi = e4m3(q 2^-e), lo = e5m2 of what hi leaves (a
-//                 bf16 number's eight significant bits fit into the two; off by at most 2^-25 of the row's largest element);
+//                 bf16 number's eight significant bits fit into the two; off by at most 2^-21.8 of the row's largest element);
 //   P = exp2(S S_k scale log2 e - reference), rounded to bf16, over the scores in tensor memory;
 //   O += P V      kind::f16, V as bf16: an e4m3 number times a power of two is exact in bf16, so the page's scale is in it.
 //
@@ -15,9 +15,8 @@
 // which is the bf16 number of the same exponent field, 2^-120 times the e4m3 one (subnormals too); a product in bf16 with 2^120
 // times the page's scale puts that right.  Both products take as long as they would in bf16.
 //
-// Measured: 512 tokens at 16,384 (32 heads over 8, pages of 16): 195 us, 172 with the cache in the L2, 700 TFLOP/s; three prompts of up to
-// 2,048: 162 us.  The tensor cores are busy for a third of the time; the schedulers' slots (two thirds are taken) and the chain of
-// hand-overs of a tile, of which the widening is the longest, bound the kernel, and it is close to the instruction caches: writing a
+// Measured: 512 tokens at 16,384 (32 heads over 8, pages of 16; 128 items): 171 us, 800 TFLOP/s; three prompts of up to 2,048: 159 us.
+// The tensor cores are busy for two fifths of the time; the schedulers' slots (seven tenths are taken) and the chain of hand-overs of a tile, of which the widening is the longest, bound the kernel, and it is close to the instruction caches: writing a
 // loop out that is short now (the widening's, twice as long) takes 25% more.  Every wait left out was worth 1 to 3%.
 //
 // Roles: a scout reads block table and scales ahead and leaves them in shared memory; two loaders (TMA) for keys and values; an
@@ -75,7 +74,7 @@ struct Info {
   int whole, one_factor;                                   // all pages are there; v_rest is 1 throughout
 };
 
-// n / d for 0 <= n < 2^31 as (n + n m / 2^32) >> s: s the bits of d - 1, m = floor(2^32 (2^s - d) / d) + 1 (a division takes some 25
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery, 1994), (n + n m / 2^32) >> s: s the bits of d - 1, m = floor(2^32 (2^s - d) / d) + 1 (a division takes some 25
 // instructions, and every role works out its items by itself).
 struct Divider {
   uint32_t factor;

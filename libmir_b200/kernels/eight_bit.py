@@ -114,7 +114,9 @@ def decode_attention_8bit(qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.T
     block table does not have (an entry below 0 or beyond the pool, or a block behind its last column) are not seen; a row
     that sees none gets zeros.  `partition`, `num_partitions`: decode_attention_8bit_plan's; where partition is not 0, keys behind
     partition * num_partitions are not seen either.  `scratch`: float32, the plan's size, on a 16-byte boundary; calls that
-    may run at the same time, or graphs, take one each.  `sinks`: one number per query head in the softmax's denominator."""
+    may run at the same time, or graphs, take one each.  `sinks`: one number per query head in the softmax's denominator.  A key's
+    weight is rounded on its way into the product with the values, by at most 2^-8 of itself (where partition is 0: down to
+    2^-56 of the largest among 128 keys, times their pages' scales, and by 2^-67 of that below)."""
     what = "decode_attention_8bit"
     _on_this_device(what, qkv, out, k_pages, v_pages, k_scales, v_scales, block_table, positions, scratch, sinks)
     rows = out.shape[0]
